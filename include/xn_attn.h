@@ -321,6 +321,95 @@ XN_API int64_t xn_stream_len(xn_ctx* ctx, xn_stream* stream, int32_t layer);
 /* Copies the stream's page table (page ids in position order) into `out`; returns the count. */
 XN_API int64_t xn_stream_pages(xn_ctx* ctx, xn_stream* stream, int32_t* out, int64_t max_out);
 
+/* ---- reading a cache without appending, and bounding it by what was read ----------------------- */
+
+/* No counterpart in the reference, whose attention always appends and whose only bound on a cache
+ * is the ring (CpuRingCache.max_seq_len: the OLDEST position goes, fast_attention.rs:112).  These
+ * calls serve a memory that is written once and read by many tokens (an encoder's states, a shared
+ * document), and a decoder's own cache that is to keep the positions its queries look at.
+ * None of them may be made while the context's CUDA stream is being captured (XN_ERR_ARG).
+ *
+ * Writes n rows of K and V at positions t0.. of one layer, without any attention: k and v are
+ * [num_kv_heads, n, head_dim], or [n, num_kv_heads * head_dim] with XN_REQ_SEQ_MAJOR.  flags:
+ * XN_REQ_DEVICE_PTRS (enqueues; else host pointers, blocks until they are read), XN_REQ_SEQ_MAJOR,
+ * XN_REQ_ROPE (rotate k with the context's tables).  t0 + n <= max_seq_len (no folding).  Positions
+ * between the stream's length and t0 read as zeros.  Writing position t forgets the account of
+ * attention weight (below) from t on. */
+XN_API int32_t xn_kv_write(xn_ctx* ctx, xn_stream* stream, int32_t layer, int64_t t0, int64_t n,
+                           const float* k, const float* v, uint32_t flags);
+
+/* Flags of xn_read_req, beside XN_REQ_DEVICE_PTRS and XN_REQ_SEQ_MAJOR (q and out are
+ * [rows, num_heads * head_dim]). */
+enum {
+    XN_READ_CAUSAL = 1u << 8,      /* row t sees positions 0 .. kv_len - rows + t (rows that see     */
+                                   /* nothing give zeros); without it every row sees 0 .. kv_len - 1 */
+    XN_READ_ACCOUNT = 1u << 9,     /* add the rows' attention weights to the stream's account        */
+    XN_READ_ACCOUNT_SET = 1u << 10 /* ... which starts afresh with this call                         */
+};
+
+typedef struct xn_read_req {
+    xn_stream* stream;  /* may occur more than once, but an account only once per layer and call     */
+    int32_t layer;
+    int32_t rows;       /* query rows                                                                */
+    int64_t kv_len;     /* positions 0 .. kv_len - 1 are read; -1: all that the layer holds          */
+    const float* q;     /* [num_heads, rows, head_dim], rotated already where the model rotates      */
+    float* out;         /* same layout; kv_len = 0 gives zeros                                       */
+    float* weights;     /* NULL, or [num_kv_heads][weights_stride]: receives, for every KV head and  */
+                        /* position j < kv_len, the account after this call (without an account      */
+                        /* flag: this call's own weights)                                            */
+    int64_t weights_stride; /* floats between two KV heads' rows; 0: kv_len                          */
+    uint32_t flags;
+    uint32_t reserved;  /* 0 */
+} xn_read_req;
+
+/* Attention of n groups of query rows over what their streams hold, appending nothing: scale
+ * 1/sqrt(head_dim), softmax, weighted V sum; query head h reads KV head h / (num_heads /
+ * num_kv_heads).  With XN_REQ_DEVICE_PTRS on every request the call returns after enqueueing;
+ * otherwise it blocks until the host outputs are written.  Results are f32-grade in every variant
+ * (split f16 operands on the tensor cores for many rows, f32 arithmetic for few).
+ *
+ * The account of attention weight, per layer, KV head and position j, is the sum over the
+ * accounted rows and the heads of the KV head's group of the weight they gave j.  It is kept in
+ * f32 beside the cache pages.  A stream longer than its capacity (folded) can be read without
+ * XN_READ_CAUSAL and without an account only.  With the u8 cache format and head_dim > 128 no weights
+ * are available (XN_ERR_SHAPE). */
+XN_API int32_t xn_cross_attention(xn_ctx* ctx, int32_t n, const xn_read_req* reqs);
+
+/* The account of positions [t0, t0+n), [num_kv_heads, n]: read it, or replace it (positions before t0
+ * that had none get zeros; those from t0+n on are forgotten).  flags: XN_REQ_DEVICE_PTRS or 0. */
+XN_API int32_t xn_kv_account_get(xn_ctx* ctx, xn_stream* stream, int32_t layer, int64_t t0, int64_t n,
+                                 float* out, uint32_t flags);
+XN_API int32_t xn_kv_account_set(xn_ctx* ctx, xn_stream* stream, int32_t layer, int64_t t0, int64_t n,
+                                 const float* in, uint32_t flags);
+
+enum { XN_EVICT_COPY = 1u << 11 }; /* the kept rows go to k_out / v_out and the stream stays as it is */
+
+typedef struct xn_evict_req {
+    xn_stream* stream;   /* each stream once per call                                                */
+    int32_t layer;       /* -1: every layer (they must hold equally many positions)                  */
+    int32_t reserved0;   /* 0 */
+    int64_t keep;        /* positions to keep per KV head, >= 1; at most the length are kept         */
+    int64_t recent;      /* of them the last positions, whatever their account; 0 .. keep            */
+    int32_t* kept;       /* NULL, or [layers, num_kv_heads, kept]: the kept positions, ascending     */
+    float* k_out;        /* XN_EVICT_COPY: [layers, num_kv_heads, kept, head_dim]; else NULL         */
+    float* v_out;
+    float* weights_out;  /* NULL, or [layers, num_kv_heads, kept]: the kept positions' accounts      */
+    uint32_t flags;      /* XN_REQ_DEVICE_PTRS (enqueues; else host pointers, blocks), XN_EVICT_COPY */
+    uint32_t reserved;   /* 0 */
+} xn_evict_req;
+
+/* Eviction by accumulated attention weight.  Every layer and KV head keeps its `recent` last positions
+ * and, of the others, those with the largest account (equal accounts: the lowest position; NaN counts
+ * as lowest), `keep` in all, in their old order.  Their rows move to positions 0 .. keep-1, their
+ * accounts with them, the stream's length becomes keep and its pages behind it return to the pool:
+ * decoding goes on at index_pos = xn_stream_len.  The library remembers how many positions left
+ * (xn_stream_evicted), and XN_REQ_ROPE / XN_REQ_QKV_PROJ rotate by index_pos plus that number, i.e.
+ * by the token's true position; the kept keys stay as they were rotated.  A layer that holds no more
+ * than `keep` positions is left alone (all its positions are "kept").  Folded streams are refused. */
+XN_API int32_t xn_kv_evict(xn_ctx* ctx, int32_t n, const xn_evict_req* reqs);
+/* Positions that evictions took from one layer of a stream since its creation or last reset. */
+XN_API int64_t xn_stream_evicted(xn_ctx* ctx, xn_stream* stream, int32_t layer);
+
 /* ---- attention output block: sub-norm + ternary o_proj ---------------------------------------- */
 
 /* Packing of ternary weights, TernaryPackType (src/bit1_58/quantization.rs:1-5). */

@@ -1,0 +1,692 @@
+"""Reads that do not append (cross attention), the account of attention weight, eviction: against
+plain implementations in 64 bits.
+
+Tolerances.  Inputs are N(0, 1), so a score q.k / sqrt(D) is of order 1.  On the tensor-core path
+an operand keeps 22 significand bits (relative error 2^-23 each) and the lo * lo term (2^-22) is
+dropped: independent errors of at most 4 * 2^-23 per product give a score error of rms
+4 * 2^-23 * |q| |k| / D ~ 5e-7; the 24 accumulation steps add at most 24 * 2^-24 ~ 1.4e-6 of the
+score.  exp, the sum and the second product add 2^-22 each.  In all below 4e-6 relative to the
+result's norm; the f32 path is closer.  A single output (up to ~4) may be off by four times that."""
+import os
+
+import numpy as np
+import pytest
+
+import oracle as xo
+import xor_net_b200 as xn
+from gpu_util import errs
+
+pytestmark = pytest.mark.gpu
+
+REL, ABS = 4e-6, 2e-5
+
+
+def near(got, want, what="", rel=REL, abs_tol=ABS):
+    a, r = errs(got, want)
+    assert np.all(np.isfinite(np.asarray(got))) and r <= rel and a <= abs_tol, f"{what}: max abs {a:.3e}, rel {r:.3e}"
+
+
+def plain(q, k, v, causal=False):
+    """q [Hq, R, D], k, v [Hkv, n, D] -> out [Hq, R, D], weights summed per KV head [Hkv, n], in f64."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    Hq, R, D = q.shape
+    Hkv, n, _ = k.shape
+    G = Hq // Hkv
+    out, w = np.zeros((Hq, R, D)), np.zeros((Hkv, n))
+    for h in range(Hq):
+        for t in range(R):
+            m = max(0, n - R + t + 1) if causal else n
+            if m == 0:
+                continue
+            s = k[h // G, :m] @ q[h, t] / np.sqrt(D)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[h, t] = p @ v[h // G, :m]
+            w[h // G, :m] += p
+    return out, w
+
+
+def context(monkeypatch, path, *args, **kw):
+    """path: "few" and "tc" force the f32 and the tensor-core kernels, "auto" leaves the choice."""
+    if path != "auto":
+        monkeypatch.setenv("XORNET_ATTN_READ_TC_MIN_ROWS", "1" if path == "tc" else "1000000000")
+    return xn.Context(*args, **kw)
+
+
+def rows(rng, *shape):
+    return rng.standard_normal(shape).astype(np.float32)
+
+
+def filled(ctx, rng, n, layer=0, cap=None):
+    st = ctx.new_stream(cap or max(n, 1))
+    k, v = rows(rng, ctx.num_kv_heads, n, ctx.head_dim), rows(rng, ctx.num_kv_heads, n, ctx.head_dim)
+    if n:
+        st.write(layer, 0, k, v)
+    return st, k, v
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(20, 5, 128), (4, 4, 64), (6, 2, 100), (5, 1, 33), (8, 2, 8), (16, 2, 80), (3, 1, 1)])
+def test_write_and_read_shapes(monkeypatch, path, Hq, Hkv, D):
+    rng = np.random.default_rng(D + Hq)
+    ctx = context(monkeypatch, path, 2, Hq, Hkv, D, pool_pages=64, shuffle_seed=5)
+    for n, R in [(1, 1), (1, 3), (63, 2), (64, 1), (65, 7), (127, 33), (129, 1), (200, 130), (300, 5)]:
+        st, k, v = filled(ctx, rng, n, layer=1)
+        assert np.array_equal(st.read_range(1, 0, n)[0], k) and np.array_equal(st.read_range(1, 0, n)[1], v)
+        q = rows(rng, Hq, R, D)
+        (out,), (w,) = ctx.cross_attention([st], 1, [q], weights=True)
+        want, want_w = plain(q, k, v)
+        near(out, want, f"n={n} R={R}")
+        near(w, want_w, f"weights n={n} R={R}", abs_tol=ABS * max(1, R * Hq // Hkv))
+        (out2,) = ctx.cross_attention([st], 1, [q])
+        near(out2, want, f"without weights n={n} R={R}")
+        # a shorter prefix; the rest of the stream is not seen
+        m = max(1, n // 2)
+        (out,) = ctx.cross_attention([st], 1, [q], kv_lens=[m])
+        near(out, plain(q, k[:, :m], v[:, :m])[0], f"prefix {m} of {n}")
+        st.destroy()
+    ctx.close()
+
+
+@pytest.mark.parametrize("D", [129, 200, 256])
+def test_long_rows_of_the_cache(D):
+    rng = np.random.default_rng(D)
+    ctx = xn.Context(1, 4, 2, D, pool_pages=16)
+    st, k, v = filled(ctx, rng, 150)
+    q = rows(rng, 4, 40, D)
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], weights=True, causal=True)
+    want, want_w = plain(q, k, v, causal=True)
+    near(out, want)
+    near(w, want_w, abs_tol=40 * 2 * ABS)
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+@pytest.mark.parametrize("n,R", [(1, 1), (64, 64), (70, 3), (129, 129), (200, 40), (40, 90), (1, 130), (300, 257)])
+def test_causal_rows_and_rows_that_see_nothing(monkeypatch, path, n, R):
+    rng = np.random.default_rng(n * 1000 + R)
+    ctx = context(monkeypatch, path, 1, 6, 2, 64, pool_pages=16)
+    st, k, v = filled(ctx, rng, n)
+    q = rows(rng, 6, R, 64)
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+    want, want_w = plain(q, k, v, causal=True)
+    near(out, want)
+    near(w, want_w, abs_tol=ABS * R)
+    if R > n:
+        assert np.array_equal(out[:, : R - n], np.zeros_like(out[:, : R - n]))
+    (out,) = ctx.cross_attention([st], 0, [q], causal=True)
+    near(out, want)
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+def test_batches_share_streams_mix_lengths_and_leave_neighbours_alone(monkeypatch, path):
+    import torch
+
+    rng = np.random.default_rng(3)
+    Hq, Hkv, D = 8, 2, 64
+    ctx = context(monkeypatch, path, 2, Hq, Hkv, D, pool_pages=64, shuffle_seed=11)
+    a, ka, va = filled(ctx, rng, 500, layer=0)
+    b, kb, vb = filled(ctx, rng, 77, layer=1)
+    c = ctx.new_stream(10)   # holds nothing
+    cases = [(a, 0, ka, va, 1, 500), (a, 0, ka, va, 5, 65), (b, 1, kb, vb, 33, 77), (c, 0, ka, va, 4, 0), (b, 1, kb, vb, 0, 77),
+             (a, 0, ka, va, 140, 300), (a, 0, ka, va, 2, 0)]
+    for seq_major in (False, True):
+        entries, outs, keep = [], [], []
+        for st, layer, k, v, R, n in cases:
+            q = rows(rng, Hq, R, D)
+            src = q.transpose(1, 0, 2) if seq_major else q
+            # odd alignment: every tensor starts one float into its buffer, between guard values
+            buf = torch.full((q.size + 2,), 7.0, device="cuda")
+            buf[1:-1] = torch.from_numpy(np.ascontiguousarray(src)).reshape(-1)
+            out = torch.full((q.size + 2,), 9.0, device="cuda")
+            w = torch.full((Hkv * 600 + 1,), 3.0, device="cuda")
+            entries.append((st, layer, R, n, buf[1:].data_ptr(), out[1:].data_ptr(), w[1:].data_ptr(), 600))
+            outs.append((q, k, v, R, n, out, w))
+            keep.append(buf)
+        torch.cuda.synchronize()
+        flags = xn.REQ_DEVICE_PTRS | (xn.REQ_SEQ_MAJOR if seq_major else 0)
+        ctx.submit_reads(ctx.make_read_batch(entries, flags))
+        ctx.synchronize()
+        for q, k, v, R, n, out, w in outs:
+            got = out.cpu().numpy()
+            assert got[0] == 9.0 and got[-1] == 9.0
+            got = got[1:-1].reshape((R, Hq, D) if seq_major else (Hq, R, D))
+            got = got.transpose(1, 0, 2) if seq_major else got
+            wn = w.cpu().numpy()
+            want, want_w = plain(q, k[:, :n], v[:, :n])
+            if R:
+                near(got, want, f"R={R} n={n}") if n else np.testing.assert_array_equal(got, 0.0)
+            for h in range(Hkv):
+                row = wn[1 + h * 600: 1 + h * 600 + 600]
+                assert np.all(row[n:] == 3.0)
+                if n and R:
+                    near(row[:n], want_w[h], abs_tol=ABS * R * 4)
+                elif n:
+                    assert np.array_equal(row[:n], np.zeros(n, np.float32))
+            assert wn[0] == 3.0
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+def test_account_adds_up_is_set_and_follows_writes(monkeypatch, path):
+    rng = np.random.default_rng(8)
+    Hq, Hkv, D, n = 6, 3, 64, 150
+    ctx = context(monkeypatch, path, 2, Hq, Hkv, D, pool_pages=16, shuffle_seed=2)
+    st, k, v = filled(ctx, rng, n, layer=1, cap=400)
+    assert np.array_equal(st.account(1), np.zeros((Hkv, n), np.float32))
+    total = np.zeros((Hkv, n))
+    for R, m, causal in [(3, 100, False), (40, 150, True), (1, 20, False), (2, 150, False)]:
+        q = rows(rng, Hq, R, D)
+        _, (w,) = ctx.cross_attention([st], 1, [q], kv_lens=[m], causal=causal, account="add", weights=True)
+        total[:, :m] += plain(q, k[:, :m], v[:, :m], causal)[1]
+        near(st.account(1), total, abs_tol=1e-4)
+        assert np.array_equal(w, st.account(1, 0, m))
+    assert np.array_equal(st.account(0, 0, 0), np.zeros((Hkv, 0), np.float32))
+    # without an account flag the weights are this call's own and nothing is kept
+    before = st.account(1)
+    q = rows(rng, Hq, 4, D)
+    _, (w,) = ctx.cross_attention([st], 1, [q], weights=True)
+    near(w, plain(q, k, v)[1], abs_tol=1e-4)
+    assert np.array_equal(st.account(1), before)
+    # set: starts afresh, positions behind the prefix have none
+    ctx.cross_attention([st], 1, [q], kv_lens=[70], account="set")
+    got = st.account(1)
+    near(got[:, :70], plain(q, k[:, :70], v[:, :70])[1], abs_tol=1e-4)
+    assert np.array_equal(got[:, 70:], np.zeros_like(got[:, 70:]))
+    # rows written at 30 take the account from there on with them
+    st.write(1, 30, k[:, 30:40], v[:, 30:40])
+    after = st.account(1)
+    assert np.array_equal(after[:, :30], got[:, :30]) and not after[:, 30:].any()
+    # ... and so does an appending attention, also one that reuses the plan of the step before
+    st.set_account(1, 0, np.ones((Hkv, n)))
+    x = rows(rng, 1, Hq, 1, D)
+    kv = rows(rng, 1, Hkv, 1, D)
+    ctx.attention(st, 1, 140, x, kv, kv)
+    assert st.account(1)[:, :140].all() and not st.account(1)[:, 140:].any()
+    # set in the middle: what lies before and had none is zero, what lies behind is forgotten
+    st.set_account(1, 145, np.full((Hkv, 3), 2.0))
+    got = st.account(1)
+    assert np.all(got[:, :140] == 1) and not got[:, 140:145].any() and np.all(got[:, 145:148] == 2) and not got[:, 148:].any()
+    st.reset()
+    assert st.length(1) == 0 and st.evicted(1) == 0
+    ctx.close()
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 2), (100, 3, 3), (128, 8, 2), (16, 2, 1)])
+def test_u8_cache_format(D, Hq, Hkv):
+    rng = np.random.default_rng(D)
+    ctx = xn.Context(1, Hq, Hkv, D, pool_pages=32, kv_format=xn.KV_U8, shuffle_seed=3)
+    for n, R in [(1, 1), (70, 2), (200, 64), (131, 9)]:
+        st, k, v = filled(ctx, rng, n)
+        kd, vd = st.read_range(0, 0, n)   # the dequantised rows: what attention runs over
+        q = rows(rng, Hq, R, D)
+        for causal in (False, True):
+            want, want_w = plain(q, kd, vd, causal)
+            (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=causal, weights=True, account="set")
+            near(out, want, f"{n} {R}")
+            near(w, want_w, abs_tol=ABS * R * Hq)
+            (out,) = ctx.cross_attention([st], 0, [q], causal=causal)
+            near(out, want, f"{n} {R} without weights")
+        kept, ck, cv, cw = st.evict_copy(max(1, n // 3), recent=min(4, max(1, n // 3)))
+        u = st.read_u8(0, 0, n)
+        acct = st.account(0)
+        for h in range(Hkv):
+            assert np.array_equal(ck[0, h], kd[h, kept[0, h]]) and np.array_equal(cv[0, h], vd[h, kept[0, h]])
+            assert np.array_equal(cw[0, h], acct[h, kept[0, h]])
+        kept2 = st.evict(max(1, n // 3), recent=min(4, max(1, n // 3)))
+        assert np.array_equal(kept, kept2)
+        u2 = st.read_u8(0, 0, kept.shape[2])
+        for h in range(Hkv):
+            for x, y in zip(u, u2):
+                assert np.array_equal(x[h][kept[0, h]], y[h])
+        st.destroy()
+    ctx.close()
+
+
+def test_u8_weights_need_a_head_dim_the_tensor_cores_take():
+    rng = np.random.default_rng(0)
+    ctx = xn.Context(1, 2, 1, 200, pool_pages=4, kv_format=xn.KV_U8)
+    st, _, _ = filled(ctx, rng, 10)
+    q = rows(rng, 2, 3, 200)
+    kd, vd = st.read_range(0, 0, 10)
+    (out,) = ctx.cross_attention([st], 0, [q])
+    near(out, plain(q, kd, vd)[0])
+    with pytest.raises(xn.XnError) as e:
+        ctx.cross_attention([st], 0, [q], account="add")
+    assert e.value.code == 2
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+def test_values_over_many_orders_of_magnitude(monkeypatch, path):
+    """K, V and Q rows of very different sizes (a page's largest element sets its scale), zero rows."""
+    rng = np.random.default_rng(17)
+    Hq, Hkv, D, n, R = 4, 1, 64, 200, 40
+    ctx = context(monkeypatch, path, 1, Hq, Hkv, D, pool_pages=8)
+    st = ctx.new_stream(n)
+    k, v, q = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D), rows(rng, Hq, R, D)
+    k *= np.exp2(rng.integers(-6, 2, size=(Hkv, n, 1))).astype(np.float32)
+    v *= np.exp2(rng.integers(-12, 1, size=(Hkv, n, 1))).astype(np.float32)
+    v[:, 64:128] *= np.float32(2.0 ** 14)
+    k[:, 5] = 0
+    v[:, 6] = 0
+    k[:, 128:192] = 0
+    q *= np.exp2(rng.integers(-20, 1, size=(Hq, R, 1))).astype(np.float32)
+    q[:, 3] = 0
+    q[0, 0] *= np.float32(1e-30)
+    st.write(0, 0, k, v)
+    (out,) = ctx.cross_attention([st], 0, [q], causal=True)
+    want = plain(q, k, v, True)[0]
+    near(out, want, abs_tol=4 * REL * np.abs(want).max())
+    # row by row: every row's own norm, not the largest row's
+    for h in range(Hq):
+        for t in range(R):
+            near(out[h, t], want[h, t], f"row {h} {t}", abs_tol=np.inf)
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_infinities_and_nan_stay_where_they_are_seen(monkeypatch, path, value):
+    rng = np.random.default_rng(4)
+    Hq, Hkv, D, n, R = 4, 2, 64, 140, 70
+    ctx = context(monkeypatch, path, 1, Hq, Hkv, D, pool_pages=8)
+    k, v, q = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D), rows(rng, Hq, R, D)
+    q = np.abs(q)   # (so that an infinite K element gives a score of one sign)
+    for which in ("k", "v"):
+        kb, vb = k.copy(), v.copy()
+        (kb if which == "k" else vb)[1, 120, 7] = value
+        st = ctx.new_stream(n)
+        st.write(0, 0, kb, vb)
+        (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+        with np.errstate(all="ignore"):
+            want, want_w = plain(q, kb, vb, True)
+        first = 120 - (n - R)   # rows from here on see the position
+        near(out[:2], want[:2])                     # the other KV head
+        near(out[2:, :first], want[2:, :first])     # rows before it
+        got, ref = out[2:, first:], want[2:, first:]
+        assert np.array_equal(np.isfinite(got), np.isfinite(ref)), which
+        assert np.array_equal(np.isnan(got), np.isnan(ref)), which
+        if which == "v":
+            near(w, want_w, abs_tol=ABS * R)
+            np.testing.assert_allclose(got[np.isfinite(ref)], ref[np.isfinite(ref)], atol=ABS, rtol=REL * 4)
+        st.destroy()
+    # behind the prefix anything may lie
+    kb, vb = k.copy(), v.copy()
+    kb[:, 100:], vb[:, 100:] = value, value
+    st = ctx.new_stream(n)
+    st.write(0, 0, kb, vb)
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], kv_lens=[100], weights=True)
+    want, want_w = plain(q, k[:, :100], v[:, :100])
+    near(out, want)
+    near(w, want_w, abs_tol=ABS * R)
+    # a query row with an infinity spoils itself alone
+    st.write(0, 0, k, v)
+    qb = q.copy()
+    qb[0, 9, 3] = value
+    (out,) = ctx.cross_attention([st], 0, [qb])
+    want = plain(q, k, v)[0]
+    assert not np.isfinite(out[0, 9]).any()
+    keep = np.ones((Hq, R), bool)
+    keep[0, 9] = False
+    near(out[keep], want[keep])
+    ctx.close()
+
+
+def kept_of(account, keep, recent):
+    """The definition: account [n] -> kept positions."""
+    n = len(account)
+    keep = min(keep, n)
+    recent = min(recent, keep)
+    a = np.where(np.isnan(account), -np.inf, account.astype(np.float64))
+    nan = np.isnan(account)
+    old = n - recent
+    order = np.lexsort((np.arange(old), ~nan[:old] * -1, -a[:old]))   # value, then numbers before NaN, then position
+    return np.concatenate([np.sort(order[: keep - recent]), np.arange(old, n)]).astype(np.int32)
+
+
+@pytest.mark.parametrize("n,keep,recent", [(1, 1, 0), (10, 3, 0), (64, 64, 5), (65, 64, 0), (100, 40, 40), (130, 65, 64), (300, 299, 7),
+                                           (1000, 1, 0), (1000, 700, 3), (5000, 5000, 10), (5000, 9000, 10), (9000, 4097, 4096),
+                                           (20000, 777, 5), (70000, 33333, 1)])
+def test_evict_keeps_what_the_account_says(n, keep, recent):
+    rng = np.random.default_rng(n + keep)
+    Hkv, D, L = 2, 12, 2
+    ctx = xn.Context(L, 4, Hkv, D, pool_pages=(n + 63) // 64 + 3, shuffle_seed=9)
+    st = ctx.new_stream(n + 100)
+    k, v = rows(rng, L, Hkv, n, D), rows(rng, L, Hkv, n, D)
+    w = np.exp(2 * rows(rng, L, Hkv, n))
+    w[:, 0] = np.round(w[:, 0])            # many equal accounts, zeros among them
+    w[1, 1] *= rng.choice([-1, 1], n).astype(np.float32)
+    w[1, 1, rng.random(n) < 0.05] = np.nan
+    w[0, 1, rng.random(n) < 0.05] = np.inf
+    w[1, 0, rng.random(n) < 0.3] = -0.0
+    for l in range(L):
+        st.write(l, 0, k[l], v[l])
+        st.set_account(l, 0, w[l])
+    want = np.stack([np.stack([kept_of(w[l, h], keep, recent) for h in range(Hkv)]) for l in range(L)])
+    kept, ck, cv, cw = st.evict_copy(keep, recent)
+    assert np.array_equal(kept, want)
+    for l in range(L):
+        for h in range(Hkv):
+            assert np.array_equal(ck[l, h], k[l, h, want[l, h]]) and np.array_equal(cv[l, h], v[l, h, want[l, h]])
+            assert np.array_equal(cw[l, h], w[l, h, want[l, h]], equal_nan=True)
+    assert [st.length(l) for l in range(L)] == [n] * L      # a copy changes nothing
+    assert np.array_equal(st.read_range(1, 0, n)[0], k[1])
+    in_use = ctx.stats()["pages_in_use"]
+    one = st.evict(keep, recent, layer=1)                   # one layer: the other stays, and so do the pages
+    assert np.array_equal(one[0], want[1]) and st.length(0) == n
+    m = want.shape[2]
+    assert st.length(1) == m and st.evicted(1) == n - m and st.evicted(0) == 0
+    assert ctx.stats()["pages_in_use"] == in_use
+    assert np.array_equal(st.evict(keep, recent, layer=0)[0], want[0])
+    assert ctx.stats()["pages_in_use"] == (m + 63) // 64
+    for l in range(L):
+        gk, gv = st.read_range(l, 0, m)
+        for h in range(Hkv):
+            assert np.array_equal(gk[h], k[l, h, want[l, h]]) and np.array_equal(gv[h], v[l, h, want[l, h]])
+            assert np.array_equal(st.account(l)[h], w[l, h, want[l, h]], equal_nan=True)
+    ctx.close()
+
+
+def test_evict_without_an_account_keeps_the_first_and_the_last():
+    rng = np.random.default_rng(1)
+    ctx = xn.Context(1, 2, 1, 32, pool_pages=8)
+    st, k, v = filled(ctx, rng, 100)
+    assert np.array_equal(st.evict(10, recent=6)[0, 0], [0, 1, 2, 3, 94, 95, 96, 97, 98, 99])
+    empty = ctx.new_stream(8)
+    assert empty.evict(4).shape == (1, 1, 0)
+    ctx.close()
+
+
+def test_many_streams_in_one_eviction():
+    import torch
+
+    rng = np.random.default_rng(6)
+    Hkv, D = 3, 64
+    ctx = xn.Context(1, 3, Hkv, D, pool_pages=64, shuffle_seed=4)
+    sts = []
+    for i, n in enumerate([30, 200, 64, 131, 1]):
+        st, k, v = filled(ctx, rng, n)
+        w = rows(rng, Hkv, n)
+        st.set_account(0, 0, w)
+        sts.append((st, k, v, w, n))
+    kept = [torch.full((Hkv * 64,), -1, dtype=torch.int32, device="cuda") for _ in sts]
+    torch.cuda.synchronize()
+    ctx.submit_evict(ctx.make_evict_batch([(st, 0, 64, 10, t.data_ptr(), None, None, None) for (st, *_), t in zip(sts, kept)],
+                                          xn.REQ_DEVICE_PTRS))
+    ctx.synchronize()
+    for (st, k, v, w, n), t in zip(sts, kept):
+        m = min(64, n)
+        got = t.cpu().numpy()[: Hkv * m].reshape(Hkv, m)
+        for h in range(Hkv):
+            want = kept_of(w[h], 64, 10)
+            assert np.array_equal(got[h], want)
+            assert np.array_equal(st.read_range(0, 0, m)[0][h], k[h, want])
+        assert np.all(t.cpu().numpy()[Hkv * m:] == -1)
+    ctx.close()
+
+
+@pytest.mark.parametrize("fmt", [xn.KV_F32, xn.KV_U8])
+def test_prompt_account_eviction_and_decode_together(fmt):
+    """A prompt is written and accounted, the cache cut down, and decoding goes on with the fused rotary
+    path at the tokens' true positions, next to a second stream that takes the freed pages."""
+    rng = np.random.default_rng(12)
+    Hq, Hkv, D, n, keep, recent, R = 8, 2, 64, 260, 100, 16, 64
+    cos, sin = xn.rope_tables(10000.0, D, 1024)
+    ctx = xn.Context(1, Hq, Hkv, D, pool_pages=7, rope=(cos, sin), kv_format=fmt, shuffle_seed=1)
+    st = ctx.new_stream(400)
+    k, v = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D)
+    st.write(0, 0, k, v, rope=True)
+    kd, vd = st.read_range(0, 0, n)
+
+    def rot(x, pos):   # [..., D] at positions pos
+        h = D // 2
+        c, s = cos[pos].astype(np.float64), sin[pos].astype(np.float64)
+        return np.concatenate([x[..., :h] * c - x[..., h:] * s, x[..., :h] * s + x[..., h:] * c], -1)
+
+    if fmt == xn.KV_F32:
+        near(kd, rot(k.astype(np.float64), np.arange(n)), abs_tol=1e-6)
+    q = rows(rng, Hq, R, D)
+    (out,) = ctx.cross_attention([st], 0, [q], causal=True, account="set")
+    want, want_w = plain(q, kd, vd, True)
+    near(out, want)
+    near(st.account(0), want_w, abs_tol=1e-4)
+    acct = st.account(0)
+    kept = st.evict(keep, recent)[0]
+    for h in range(Hkv):
+        assert np.array_equal(kept[h], kept_of(acct[h], keep, recent))
+    assert st.evicted(0) == n - keep and st.length(0) == keep
+    other, ko, vo = filled(ctx, rng, 300)   # five pages: only there because the eviction returned three
+    ck = np.stack([kd[h, kept[h]] for h in range(Hkv)]).astype(np.float64)
+    cv = np.stack([vd[h, kept[h]] for h in range(Hkv)]).astype(np.float64)
+    for step in range(3):
+        pos = n + step
+        x, kn, vn = rows(rng, 1, Hq, 1, D), rows(rng, 1, Hkv, 1, D), rows(rng, 1, Hkv, 1, D)
+        got = ctx.attention(st, 0, keep + step, x, kn, vn, rope=True)
+        sk, sv = st.read_range(0, keep + step, 1)
+        if fmt == xn.KV_F32:
+            near(sk, rot(kn[0].astype(np.float64), np.array([pos])), abs_tol=1e-6)
+            assert np.array_equal(sv, vn[0])
+        ck, cv = np.concatenate([ck, sk], 1), np.concatenate([cv, sv], 1)
+        near(got[0], plain(rot(x[0].astype(np.float64), np.array([pos])), ck, cv)[0], abs_tol=1e-4, rel=1e-5)
+    # a prompt chunk on the evicted stream: its query rows are rotated by the prefill kernel or the append
+    S = 150 if fmt == xn.KV_F32 else 5
+    x, kn, vn = rows(rng, 1, Hq, S, D), rows(rng, 1, Hkv, S, D), rows(rng, 1, Hkv, S, D)
+    other.destroy()
+    got = ctx.attention(st, 0, keep + 3, x, kn, vn, rope=True)
+    sk, sv = st.read_range(0, keep + 3, S)
+    ck, cv = np.concatenate([ck, sk], 1), np.concatenate([cv, sv], 1)
+    pos = n + 3 + np.arange(S)
+    near(got[0], plain(rot(x[0].astype(np.float64), pos), ck, cv, True)[0], abs_tol=2e-2, rel=5e-3)  # TF32 prefill
+    ctx.close()
+
+
+def test_positions_past_the_rope_table_are_refused_by_true_position():
+    rng = np.random.default_rng(2)
+    cos, sin = xn.rope_tables(10000.0, 32, 100)
+    ctx = xn.Context(1, 2, 1, 32, pool_pages=8, rope=(cos, sin))
+    st, k, v = filled(ctx, rng, 100, cap=200)
+    st.evict(20)
+    x, kv = rows(rng, 1, 2, 1, 32), rows(rng, 1, 1, 1, 32)
+    with pytest.raises(xn.XnError) as e:
+        ctx.attention(st, 0, 20, x, kv, kv, rope=True)
+    assert e.value.code == 5
+    with pytest.raises(xn.XnError) as e:
+        st.write(0, 20, kv[0], kv[0], rope=True)
+    assert e.value.code == 5
+    ctx.attention(st, 0, 20, x, kv, kv)   # rotated by the caller: no table, no limit
+    ctx.close()
+
+
+def test_plan_reuse_does_not_outlive_an_eviction():
+    """Two decode submissions of one geometry: the second may reuse the first one's plan, but not across
+    an eviction, nor on a layer whose positions are shifted differently."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    Hq, Hkv, D = 8, 2, 128
+    cos, sin = xn.rope_tables(10000.0, D, 512)
+    ctx = xn.Context(2, Hq, Hkv, D, pool_pages=16, rope=(cos, sin))
+    st = ctx.new_stream(400)
+    for l in range(2):
+        st.write(l, 0, rows(rng, Hkv, 200, D), rows(rng, Hkv, 200, D))
+    st.evict(64, layer=1)
+    st.write(1, 64, rows(rng, Hkv, 136, D), rows(rng, Hkv, 136, D))
+    x = torch.from_numpy(rows(rng, Hq, 1, D)).cuda()
+    kv = torch.from_numpy(rows(rng, 2, Hkv, 1, D)).cuda()
+    out = torch.zeros(2, Hq, 1, D, device="cuda")
+    torch.cuda.synchronize()
+    for l in range(2):
+        ctx.submit(ctx.make_batch([(st, l, 200, 1, x.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out[l].data_ptr())],
+                                  xn.REQ_DEVICE_PTRS | xn.REQ_ROPE))
+    ctx.synchronize()
+    h = D // 2
+    for l in range(2):
+        pos = 200 + st.evicted(l)
+        a = kv[0].cpu().numpy().astype(np.float64)
+        want = np.concatenate([a[..., :h] * cos[pos] - a[..., h:] * sin[pos], a[..., :h] * sin[pos] + a[..., h:] * cos[pos]], -1)
+        near(st.read_range(l, 200, 1)[0], want, f"layer {l}", abs_tol=1e-6)
+    # the same submission after an eviction that leaves it another length must not see the old plan
+    st.evict(100)
+    assert st.length(0) == 100
+    with pytest.raises(xn.XnError):
+        ctx.cross_attention([st], 0, [rows(rng, Hq, 1, D)], kv_lens=[201])
+    ctx.close()
+
+
+def test_folded_streams_and_bad_arguments_are_refused():
+    rng = np.random.default_rng(0)
+    ctx = xn.Context(2, 4, 2, 64, pool_pages=8)
+    st, k, v = filled(ctx, rng, 60, cap=64)
+    q = rows(rng, 4, 2, 64)
+
+    def refused(code, fn, *a, **kw):
+        with pytest.raises(xn.XnError) as e:
+            fn(*a, **kw)
+        assert e.value.code == code, str(e.value)
+
+    read = lambda *e, flags=0: ctx.submit_reads(ctx.make_read_batch(list(e), flags))
+    o = np.zeros_like(q)
+    good = (st, 0, 2, 60, q.ctypes.data, o.ctypes.data, None, 0)
+    read(good)
+    refused(1, read, (st, 0, 2, 61, q.ctypes.data, o.ctypes.data, None, 0))
+    refused(1, read, (st, 0, 2, -2, q.ctypes.data, o.ctypes.data, None, 0))
+    refused(1, read, (st, 0, -1, 60, q.ctypes.data, o.ctypes.data, None, 0))
+    refused(1, read, (st, 2, 2, 0, q.ctypes.data, o.ctypes.data, None, 0))
+    refused(1, read, (st, 0, 2, 60, None, o.ctypes.data, None, 0))
+    refused(1, read, (st, 0, 2, 60, q.ctypes.data, None, None, 0))
+    refused(1, read, (st, 0, 2, 60, q.ctypes.data, o.ctypes.data, o.ctypes.data, 59))
+    refused(1, read, good, flags=xn.REQ_ROPE)
+    refused(1, read, good, good, flags=xn.READ_ACCOUNT)       # one account, twice in a call
+    mixed = ctx.make_read_batch([good, good])
+    mixed[1].flags = xn.REQ_DEVICE_PTRS
+    refused(1, ctx.submit_reads, mixed)
+    with pytest.raises(ValueError):
+        ctx.cross_attention([st], 0, [q], account="maybe")
+    refused(1, st.write, 0, 10, k, v)                         # 10 + 60 > 64
+    refused(1, st.write, 5, 0, k, v)
+    refused(8, st.write, 0, 0, k, v, rope=True)
+    refused(1, st.account, 0, 50, 11)
+    refused(1, st.set_account, 0, 59, np.zeros((2, 2)))
+    refused(1, st.evict, 0)
+    refused(1, st.evict, 5, recent=6)
+    refused(1, st.evict, 5, recent=-1)
+    refused(1, st.evict, 5, layer=2)
+    refused(1, st.evict, 5)                                   # layers of 60 and 0 positions
+    ev = lambda *e, flags=0: ctx.submit_evict(ctx.make_evict_batch(list(e), flags))
+    refused(1, ev, (st, 0, 5, 0, None, None, None, None), (st, 1, 5, 0, None, None, None, None))
+    refused(1, ev, (st, 0, 5, 0, None, o.ctypes.data, o.ctypes.data, None))
+    refused(1, ev, (st, 0, 5, 0, None, None, None, None), flags=xn.EVICT_COPY)
+    dead = ctx.new_stream(8)
+    handle = dead.handle
+    other = xn.Context(1, 4, 2, 64, pool_pages=2)
+    foreign = other.new_stream(8)
+    refused(3, read, (foreign, 0, 2, 0, q.ctypes.data, o.ctypes.data, None, 0))
+    refused(3, ev, (foreign, 0, 5, 0, None, None, None, None))
+    assert handle
+    # nothing above changed the stream
+    assert st.length(0) == 60 and np.array_equal(st.read_range(0, 0, 60)[0], k)
+    # a stream that folds around its capacity: plain reads only
+    x, kv = rows(rng, 1, 4, 10, 64), rows(rng, 1, 2, 10, 64)
+    ctx.attention(st, 0, 60, x, kv, kv)
+    fk, fv = st.read_range(0, 0, 64)
+    (out,) = ctx.cross_attention([st], 0, [q])
+    near(out, plain(q, fk, fv)[0])
+    refused(5, ctx.cross_attention, [st], 0, [q], causal=True)
+    refused(5, ctx.cross_attention, [st], 0, [q], account="add")
+    refused(5, st.evict, 5, layer=0)
+    refused(5, st.write, 0, 0, k[:, :1], v[:, :1])
+    other.close()
+    ctx.close()
+
+
+def test_pool_exhaustion_by_a_write_leaves_the_stream_as_it_was():
+    rng = np.random.default_rng(0)
+    ctx = xn.Context(1, 2, 1, 16, pool_pages=2)
+    st, k, v = filled(ctx, rng, 70, cap=1000)
+    big = rows(rng, 1, 200, 16)
+    with pytest.raises(xn.XnError) as e:
+        st.write(0, 70, big, big)
+    assert e.value.code == 4
+    assert st.length(0) == 70 and len(st.pages()) == 2
+    st.write(0, 100, big[:, :20], big[:, :20])    # positions 70..99 were skipped: zeros
+    got = st.read_range(0, 0, 120)[0]
+    assert np.array_equal(got[:, :70], k) and not got[:, 70:100].any() and np.array_equal(got[:, 100:], big[:, :20])
+    ctx.close()
+
+
+def test_calls_are_refused_inside_a_capture_and_work_after_it():
+    import torch
+
+    rng = np.random.default_rng(0)
+    s = torch.cuda.Stream()
+    ctx = xn.Context(1, 4, 2, 64, pool_pages=4, cuda_stream=s.cuda_stream)
+    st, k, v = filled(ctx, rng, 100)
+    q = torch.from_numpy(rows(rng, 4, 1, 64)).cuda()
+    o = torch.zeros_like(q)
+    reqs = ctx.make_read_batch([(st, 0, 1, 100, q.data_ptr(), o.data_ptr(), None, 0)], xn.REQ_DEVICE_PTRS)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    codes = []
+    with torch.cuda.graph(g, stream=s):
+        z = o + 1
+        for fn in (lambda: ctx.submit_reads(reqs), lambda: st.evict(5), lambda: st.write(0, 0, k, v), lambda: st.account(0)):
+            try:
+                fn()
+            except xn.XnError as e:
+                codes.append(e.code)
+    assert codes == [1, 1, 1, 1]
+    g.replay()
+    ctx.submit_reads(reqs)
+    ctx.synchronize()
+    near(o.cpu().numpy(), plain(q.cpu().numpy(), k, v)[0])
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "tc"])
+def test_same_bits_every_time_and_work_of_two_threads(monkeypatch, path):
+    import threading
+
+    rng = np.random.default_rng(14)
+    ctx = context(monkeypatch, path, 1, 8, 2, 128, pool_pages=128, shuffle_seed=8)
+    made = [filled(ctx, rng, n) + (rows(rng, 8, 48, 128),) for n in (1500, 700)]
+    first = [ctx.cross_attention([st], 0, [q], causal=True, weights=True) for st, _, _, q in made]
+    bad = []
+
+    def work(i):
+        st, _, _, q = made[i]
+        for _ in range(10):
+            (o,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True, account="set")
+            if not (np.array_equal(o, first[i][0][0]) and np.array_equal(w, first[i][1][0])):
+                bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+    for i, (st, k, v, q) in enumerate(made):
+        want, want_w = plain(q, k, v, True)
+        near(first[i][0][0], want)
+        near(first[i][1][0], want_w, abs_tol=1e-3)
+        assert np.array_equal(st.account(0), first[i][1][0])
+    ctx.close()
+
+
+def test_reads_between_appends_see_what_was_appended():
+    rng = np.random.default_rng(30)
+    Hq, Hkv, D = 6, 2, 64
+    ctx = xn.Context(1, Hq, Hkv, D, pool_pages=8)
+    st = ctx.new_stream(300)
+    ref = xo.RingCache(1, Hkv, 300, D)
+    for pos, S in [(0, 100), (100, 1), (101, 1), (102, 30)]:
+        q, k, v = rows(rng, 1, Hq, S, D), rows(rng, 1, Hkv, S, D), rows(rng, 1, Hkv, S, D)
+        got = ctx.attention(st, 0, pos, q, k, v)
+        xo.fast_attention(q, k, v, 0, pos, ref, Hq, Hkv, D)
+        # the causal read of the same rows is the appending attention
+        (again,) = ctx.cross_attention([st], 0, [q[0]], causal=True)
+        near(again, got[0], abs_tol=1e-4, rel=1e-5)
+    kk, vv = st.read_range(0, 0, 132)
+    q = rows(rng, Hq, 3, D)
+    near(ctx.cross_attention([st], 0, [q])[0], plain(q, kk, vv)[0])
+    ctx.close()

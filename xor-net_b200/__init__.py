@@ -10,12 +10,13 @@ from .api import (Context, DeviceKvCache, FastTensor, Group, Stream, TernaryLine
                   rope_tables)
 from . import sharding
 from ._ffi import (PLACE_LEAST_LOADED, PLACE_ROUND_ROBIN, KV_F32, KV_U8, PACK4, PACK5, SPARSE, REQ_DEVICE_PTRS, REQ_HOST_PINNED, REQ_OUT_PROJ, REQ_QKV_PROJ, REQ_ROPE,
-                   REQ_SEQ_MAJOR, SIGNATURES, load)
+                   REQ_SEQ_MAJOR, READ_CAUSAL, READ_ACCOUNT, READ_ACCOUNT_SET, EVICT_COPY, SIGNATURES, load)
 
 __all__ = [
     "Context", "Stream", "Group", "default_group", "place_stream", "PLACE_LEAST_LOADED", "PLACE_ROUND_ROBIN",
     "DeviceKvCache", "FastTensor", "XnError", "fast_attention", "rope_tables",
     "default_context", "close_default_contexts", "build_library", "build_host_tool", "load", "LIB_PATH", "SIGNATURES",
-    "REQ_DEVICE_PTRS", "REQ_ROPE", "REQ_SEQ_MAJOR", "REQ_HOST_PINNED", "REQ_OUT_PROJ", "REQ_QKV_PROJ", "KV_F32", "KV_U8", "SPARSE", "PACK4",
+    "REQ_DEVICE_PTRS", "REQ_ROPE", "REQ_SEQ_MAJOR", "REQ_HOST_PINNED", "REQ_OUT_PROJ", "REQ_QKV_PROJ",
+    "READ_CAUSAL", "READ_ACCOUNT", "READ_ACCOUNT_SET", "EVICT_COPY", "KV_F32", "KV_U8", "SPARSE", "PACK4",
     "PACK5", "TernaryLinear", "sharding",
 ]

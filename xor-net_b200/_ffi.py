@@ -29,6 +29,22 @@ class Req(C.Structure):
     ]
 
 
+class ReadReq(C.Structure):
+    _fields_ = [
+        ("stream", C.c_void_p), ("layer", C.c_int32), ("rows", C.c_int32), ("kv_len", C.c_int64),
+        ("q", C.c_void_p), ("out", C.c_void_p), ("weights", C.c_void_p), ("weights_stride", C.c_int64),
+        ("flags", C.c_uint32), ("reserved", C.c_uint32),
+    ]
+
+
+class EvictReq(C.Structure):
+    _fields_ = [
+        ("stream", C.c_void_p), ("layer", C.c_int32), ("reserved0", C.c_int32), ("keep", C.c_int64),
+        ("recent", C.c_int64), ("kept", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("weights_out", C.c_void_p), ("flags", C.c_uint32), ("reserved", C.c_uint32),
+    ]
+
+
 class Stats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in (
         "calls", "batches", "kernel_launches", "decode_launches", "prefill_launches", "h2d_bytes",
@@ -50,6 +66,7 @@ class OutProjDesc(C.Structure):
 
 
 REQ_DEVICE_PTRS, REQ_ROPE, REQ_SEQ_MAJOR, REQ_HOST_PINNED, REQ_OUT_PROJ, REQ_QKV_PROJ = 1, 2, 4, 8, 16, 32
+READ_CAUSAL, READ_ACCOUNT, READ_ACCOUNT_SET, EVICT_COPY = 1 << 8, 1 << 9, 1 << 10, 1 << 11
 PACK4, PACK5, SPARSE = 4, 5, 64
 KV_F32, KV_U8 = 0, 1   # xn_ctx_desc.kv_format
 PLACE_LEAST_LOADED, PLACE_ROUND_ROBIN = 0, 1
@@ -79,6 +96,15 @@ SIGNATURES = {
     "xn_attention_rope": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32,
                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "xn_attention_batch": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(Req)]),
+    "xn_kv_write": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p,
+                                C.c_void_p, C.c_uint32]),
+    "xn_cross_attention": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(ReadReq)]),
+    "xn_kv_account_get": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
+                                      C.c_void_p, C.c_uint32]),
+    "xn_kv_account_set": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
+                                      C.c_void_p, C.c_uint32]),
+    "xn_kv_evict": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(EvictReq)]),
+    "xn_stream_evicted": (C.c_int64, [C.c_void_p, C.c_void_p, C.c_int32]),
     "xn_decode_attention_static": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                C.c_int32, C.c_int32, C.c_int32, C.c_int64,
                                                C.c_int64, C.c_void_p]),

@@ -22,7 +22,8 @@ import numpy as np
 
 from . import _ffi
 from ._ffi import (KV_F32, KV_U8, PACK4, PACK5, SPARSE, REQ_DEVICE_PTRS, REQ_HOST_PINNED, REQ_OUT_PROJ, REQ_QKV_PROJ, REQ_ROPE,
-                   REQ_SEQ_MAJOR, CtxDesc, OutProjDesc, QkvProjDesc, Req, Stats)
+                   REQ_SEQ_MAJOR, READ_ACCOUNT, READ_ACCOUNT_SET, READ_CAUSAL, EVICT_COPY, CtxDesc, EvictReq,
+                   OutProjDesc, QkvProjDesc, ReadReq, Req, Stats)
 
 
 class XnError(RuntimeError):
@@ -135,6 +136,70 @@ class Stream:
         c._check(c.lib.xn_kv_read_u8(c.handle, self.handle, layer, t0, n, k8.ctypes.data, v8.ctypes.data,
                                      _ptr(ks), _ptr(vs)))
         return k8, v8, ks, vs
+
+    # -- rows in without attention, the account of attention weight, eviction -------------------
+
+    def write(self, layer: int, t0: int, k, v, rope: bool = False, seq_major: bool = False):
+        """xn_kv_write: rows ``k``, ``v`` (``[Hkv, n, D]``, or ``[n, Hkv*D]`` with ``seq_major``) at
+        positions t0.. of one layer, without attention: an encoder's states, a restored cache."""
+        k, v = _f32(k), _f32(v)
+        width = self.ctx.num_kv_heads * self.ctx.head_dim
+        if k.shape != v.shape or k.size % width:
+            raise ValueError("k and v must both be [Hkv, n, D] (or [n, Hkv*D])")
+        flags = (REQ_ROPE if rope else 0) | (REQ_SEQ_MAJOR if seq_major else 0)
+        self.ctx._check(self.ctx.lib.xn_kv_write(self.ctx.handle, self.handle, layer, t0, k.size // width,
+                                                 _ptr(k), _ptr(v), flags))
+
+    def write_device(self, layer: int, t0: int, n: int, k_ptr: int, v_ptr: int, flags: int = 0):
+        """xn_kv_write on device pointers: enqueues on the context's stream."""
+        self.ctx._check(self.ctx.lib.xn_kv_write(self.ctx.handle, self.handle, layer, t0, n, k_ptr, v_ptr,
+                                                 flags | REQ_DEVICE_PTRS))
+
+    def account(self, layer: int, t0: int = 0, n: Optional[int] = None) -> np.ndarray:
+        """xn_kv_account_get: the accumulated attention weight ``[Hkv, n]`` of positions t0..t0+n."""
+        n = self.length(layer) - t0 if n is None else n
+        out = np.zeros((self.ctx.num_kv_heads, max(n, 0)), dtype=np.float32)
+        self.ctx._check(self.ctx.lib.xn_kv_account_get(self.ctx.handle, self.handle, layer, t0, n, _ptr(out), 0))
+        return out
+
+    def set_account(self, layer: int, t0: int, weights):
+        """xn_kv_account_set: replaces the account of positions t0.. by ``weights [Hkv, n]``."""
+        w = _f32(weights).reshape(self.ctx.num_kv_heads, -1)
+        self.ctx._check(self.ctx.lib.xn_kv_account_set(self.ctx.handle, self.handle, layer, t0, w.shape[1], _ptr(w), 0))
+
+    def account_device(self, layer: int, t0: int, n: int, out_ptr: int):
+        self.ctx._check(self.ctx.lib.xn_kv_account_get(self.ctx.handle, self.handle, layer, t0, n, out_ptr,
+                                                       REQ_DEVICE_PTRS))
+
+    def set_account_device(self, layer: int, t0: int, n: int, in_ptr: int):
+        self.ctx._check(self.ctx.lib.xn_kv_account_set(self.ctx.handle, self.handle, layer, t0, n, in_ptr,
+                                                       REQ_DEVICE_PTRS))
+
+    def evict(self, keep: int, recent: int = 0, layer: int = -1) -> np.ndarray:
+        """xn_kv_evict in place: every KV head of ``layer`` (-1: of every layer) keeps its ``recent``
+        last positions and those of the largest account, ``keep`` in all.  Returns the kept positions
+        ``[layers, Hkv, kept]``; decoding goes on at ``length(layer)``."""
+        c = self.ctx
+        layers = c.num_layers if layer < 0 else 1
+        kept = np.zeros((layers, c.num_kv_heads, max(0, min(keep, self.length(max(layer, 0))))), dtype=np.int32)
+        c.submit_evict(c.make_evict_batch([(self, layer, keep, recent, kept.ctypes.data, None, None, None)]))
+        return kept
+
+    def evict_copy(self, keep: int, recent: int = 0, layer: int = -1):
+        """The kept rows without touching the stream: (kept ``[layers, Hkv, kept]``, k and v
+        ``[layers, Hkv, kept, D]``, their accounts)."""
+        c = self.ctx
+        layers = c.num_layers if layer < 0 else 1
+        shape = (layers, c.num_kv_heads, max(0, min(keep, self.length(max(layer, 0)))))
+        kept, w = np.zeros(shape, dtype=np.int32), np.zeros(shape, dtype=np.float32)
+        k, v = np.zeros(shape + (c.head_dim,), dtype=np.float32), np.zeros(shape + (c.head_dim,), dtype=np.float32)
+        c.submit_evict(c.make_evict_batch([(self, layer, keep, recent, kept.ctypes.data, _ptr(k), _ptr(v), _ptr(w))],
+                                          EVICT_COPY))
+        return kept, k, v, w
+
+    def evicted(self, layer: int) -> int:
+        """Positions that evictions took from a layer since the stream was created or reset."""
+        return int(self.ctx.lib.xn_stream_evicted(self.ctx.handle, self.handle, layer))
 
     def read(self, layer: int, kv_head: int, t: int):
         c = self.ctx
@@ -333,6 +398,66 @@ class Context:
               _ptr(outs[i])) for i, st in enumerate(streams)], flags)
         self.submit(reqs)
         return outs
+
+
+    # -- reads that do not append, eviction -----------------------------------------------------
+
+    def make_read_batch(self, entries: Sequence[tuple], flags: int = 0):
+        """entries: (stream, layer, rows, kv_len, q_ptr, out_ptr, weights_ptr, weights_stride) -> ReadReq array."""
+        arr = (ReadReq * len(entries))()
+        for i, (st, layer, rows, kv_len, q, o, w, w_hs) in enumerate(entries):
+            r = arr[i]
+            r.stream, r.layer, r.rows, r.kv_len = st.handle, layer, rows, kv_len
+            r.q, r.out, r.weights, r.weights_stride, r.flags = q, o, w or None, w_hs, flags
+        return arr
+
+    def submit_reads(self, reqs, n: Optional[int] = None):
+        """xn_cross_attention on an array of ``make_read_batch``."""
+        self._check(self.lib.xn_cross_attention(self.handle, len(reqs) if n is None else n, reqs))
+
+    def cross_attention(self, streams, layer, qs, kv_lens=None, causal=False, account=None,
+                        weights=False, seq_major=False):
+        """xn_cross_attention on host arrays: attention of ``qs[i]`` (``[Hq, rows, D]``, or
+        ``[rows, Hq*D]`` with ``seq_major``) over the first ``kv_lens[i]`` (default: all) positions
+        that ``streams[i]`` holds, appending nothing.
+
+        ``causal``: row t of ``rows`` sees positions up to ``kv_len - rows + t``.  ``account``: None,
+        ``"add"`` (the attention weights are added to the streams' accounts) or ``"set"`` (the
+        accounts start afresh with this call).  Returns the list of outputs, shaped like ``qs``; with
+        ``weights`` the pair of that list and the list of accounts (or, without ``account``, of this
+        call's weights) ``[Hkv, kv_len]``."""
+        if account not in (None, "add", "set"):
+            raise ValueError('account must be None, "add" or "set"')
+        qs = [_f32(q) for q in qs]
+        width = self.num_heads * self.head_dim
+        for q in qs:
+            if q.size % width:
+                raise ValueError("q must be [Hq, rows, D] (or [rows, Hq*D])")
+        layers = layer if isinstance(layer, (list, tuple)) else [layer] * len(streams)
+        lens = [st.length(layers[i]) if kv_lens is None or kv_lens[i] < 0 else int(kv_lens[i])
+                for i, st in enumerate(streams)]
+        lens = [min(x, st.max_seq_len) for x, st in zip(lens, streams)]
+        outs = [np.empty_like(q) for q in qs]
+        accs = [np.zeros((self.num_kv_heads, max(n, 0)), dtype=np.float32) for n in lens] if weights else None
+        flags = (READ_CAUSAL if causal else 0) | (REQ_SEQ_MAJOR if seq_major else 0) | \
+            {None: 0, "add": READ_ACCOUNT, "set": READ_ACCOUNT_SET}[account]
+        self.submit_reads(self.make_read_batch(
+            [(st, layers[i], qs[i].size // width, lens[i], _ptr(qs[i]), _ptr(outs[i]),
+              _ptr(accs[i]) if weights and lens[i] > 0 else None, 0) for i, st in enumerate(streams)], flags))
+        return (outs, accs) if weights else outs
+
+    def make_evict_batch(self, entries: Sequence[tuple], flags: int = 0):
+        """entries: (stream, layer, keep, recent, kept_ptr, k_out_ptr, v_out_ptr, weights_ptr) -> EvictReq array."""
+        arr = (EvictReq * len(entries))()
+        for i, (st, layer, keep, recent, kept, k, v, w) in enumerate(entries):
+            r = arr[i]
+            r.stream, r.layer, r.keep, r.recent = st.handle, layer, keep, recent
+            r.kept, r.k_out, r.v_out, r.weights_out, r.flags = kept, k, v, w, flags
+        return arr
+
+    def submit_evict(self, reqs, n: Optional[int] = None):
+        """xn_kv_evict on an array of ``make_evict_batch``."""
+        self._check(self.lib.xn_kv_evict(self.handle, len(reqs) if n is None else n, reqs))
 
 
 # =============================================================================================

@@ -130,8 +130,8 @@ rope_append_kernel(const ReqDev* __restrict__ reqs, const int* __restrict__ page
             const int t = int(row / rows_per_tok);
             int rr = int(row % rows_per_tok);
             const int pos = r.index_pos + t;
-            c[u] = cos_t + size_t(pos) * half;
-            s[u] = sin_t + size_t(pos) * half;
+            c[u] = cos_t + size_t(pos + r.rope_off) * half;
+            s[u] = sin_t + size_t(pos + r.rope_off) * half;
             if (q_rows && rr < num_heads) {
                 // query row -> scratch (ReqDev::q points at it), rotated when the request asks for it
                 src[u] = r.q_in + size_t(rr) * r.qi_hs + size_t(t) * r.qi_ts;

@@ -20,6 +20,7 @@
 #include "xn_append.cuh"
 #include "xn_common.cuh"
 #include "xn_decode.cuh"
+#include "xn_evict.cuh"
 #include "xn_kv_u8.cuh"
 #include "xn_kv_u8_mma.cuh"
 #include "xn_outproj.cuh"
@@ -27,6 +28,8 @@
 #include "xn_plan.hpp"
 #include "xn_prefill_f32.cuh"
 #include "xn_prefill_tf32.cuh"
+#include "xn_read.cuh"
+#include "xn_read_tc.cuh"
 #include "xn_static_decode.cuh"
 #include "xn_ternary.hpp"
 
@@ -61,6 +64,7 @@ struct PlanCache {
         int64_t index_pos;
         uint32_t flags;
         int n_pages;
+        int64_t shift;
     };
     bool valid = false;
     bool host_mode = false, pinned = false;
@@ -125,6 +129,10 @@ struct xn_stream {
     int64_t cap = 0;
     std::vector<int32_t> pages;   // page id of slots [64*i, 64*i+64)
     std::vector<int64_t> hw;      // per layer: highest written position + 1
+    std::vector<int64_t> acc_len; // per layer: positions whose account of attention weight is valid
+                                  // (of those behind it the account is zero, whatever the pool holds)
+    std::vector<int64_t> shift;   // per layer: positions dropped by eviction; added to a position to
+                                  // get its row of the rotary tables
     int64_t expected = 0;         // tokens the creator said the stream will hold (placement only)
     // Page-locked, device-mapped buffer for the tensors of one blocking single-token call
     // [q | k | v | out]: the caller copies its pageable tensors in and out itself, in parallel
@@ -217,6 +225,12 @@ struct xn_ctx {
     bool defer_groups = true;
     std::vector<cudaEvent_t> done_events;   // idle events
     float* partials = nullptr; size_t partials_cap = 0;   // floats
+    // reads that do not append (xn_cross_attention) and eviction
+    float* read_ws = nullptr; size_t read_ws_cap = 0;      // floats: operand images, scores, partial records
+    float* acct_pool = nullptr;                            // account of attention weight, paged like K and V
+                                                           // (allocated by the first call that keeps one)
+    int read_tc_min_rows = 24;    // packed rows (rows x heads of a group) from which the tensor cores take a read
+    bool read_funcs_ready = false;
     // attention output block (sub-norm + ternary o_proj)
     std::vector<OutProj> out_proj;                         // per layer
     std::vector<OutProj> qkv_proj;                         // per layer: q, k, v rows stacked, no norm
@@ -346,27 +360,33 @@ struct SplitKernel {
     int tile_tokens;
 };
 
-template <int NV, int GT, bool EXACT>
+template <int NV, int GT, bool EXACT, bool EXT>
 SplitKernel make_split() {
-    return {attn_splitkv_kernel<NV, GT, EXACT>, DecodeSmem<NV, GT>::kBytes, DecodeCfg<NV>::kThreads,
+    return {attn_splitkv_kernel<NV, GT, EXACT, EXT>, DecodeSmem<NV, GT, EXT>::kBytes, DecodeCfg<NV>::kThreads,
             DecodeCfg<NV>::kTPS};
 }
 
 template <int NV, bool EXACT>
-SplitKernel pick_gt(int gt) {
-    if (gt == 4) return make_split<NV, 4, EXACT>();
-    if (gt == 2) return make_split<NV, 2, EXACT>();
-    return make_split<NV, 1, EXACT>();
+SplitKernel pick_gt(int gt, bool ext) {
+    if (ext) {
+        if (gt == 4) return make_split<NV, 4, EXACT, true>();
+        if (gt == 2) return make_split<NV, 2, EXACT, true>();
+        return make_split<NV, 1, EXACT, true>();
+    }
+    if (gt == 4) return make_split<NV, 4, EXACT, false>();
+    if (gt == 2) return make_split<NV, 2, EXACT, false>();
+    return make_split<NV, 1, EXACT, false>();
 }
 
 // Exact instantiations exist for the row lengths of head_dim 64, 100, 128 and 256.
-SplitKernel pick_split(int nv_class, int gt, bool exact) {
+// ext: the variant that also writes the scores and the log-sum-exps (reads that keep an account).
+SplitKernel pick_split(int nv_class, int gt, bool exact, bool ext = false) {
     switch (nv_class) {
-        case 8: return pick_gt<8, false>(gt);
-        case 16: return exact ? pick_gt<16, true>(gt) : pick_gt<16, false>(gt);
-        case 25: return pick_gt<25, true>(gt);
-        case 32: return exact ? pick_gt<32, true>(gt) : pick_gt<32, false>(gt);
-        default: return exact ? pick_gt<64, true>(gt) : pick_gt<64, false>(gt);
+        case 8: return pick_gt<8, false>(gt, ext);
+        case 16: return exact ? pick_gt<16, true>(gt, ext) : pick_gt<16, false>(gt, ext);
+        case 25: return pick_gt<25, true>(gt, ext);
+        case 32: return exact ? pick_gt<32, true>(gt, ext) : pick_gt<32, false>(gt, ext);
+        default: return exact ? pick_gt<64, true>(gt, ext) : pick_gt<64, false>(gt, ext);
     }
 }
 
@@ -542,11 +562,20 @@ void free_call_buffer(xn_stream* s) {
     s->call_cap = 0;
 }
 
+// Rows are about to be written from position t on: the account of attention weight of those
+// positions belonged to the rows they replace.
+void forget_account(xn_stream* s, int layer, int64_t t) {
+    int64_t& n = s->acc_len[size_t(layer)];
+    n = t >= s->cap ? 0 : std::min(n, t);   // (folded positions overwrite slots from the start)
+}
+
 void release_pages(xn_ctx* c, xn_stream* s) {
     c->pcache.valid = false;   // the kept plan may name this stream's pages
     for (auto it = s->pages.rbegin(); it != s->pages.rend(); ++it) c->free_pages.push_back(*it);
     s->pages.clear();
     std::fill(s->hw.begin(), s->hw.end(), 0);
+    std::fill(s->acc_len.begin(), s->acc_len.end(), 0);
+    std::fill(s->shift.begin(), s->shift.end(), 0);
 }
 
 int32_t check_device_status(xn_ctx* c) {
@@ -709,9 +738,9 @@ int32_t validate_req(xn_ctx* c, const xn_req& r) {
         return fail(c, XN_ERR_ARG, "XN_REQ_QKV_PROJ: layer %d has no q/k/v projections (xn_qkv_proj_set)", r.layer);
     if ((r.flags & XN_REQ_ROPE) || qkv) {
         if (!c->cos_d) return fail(c, XN_ERR_NO_TABLES, "context was created without RoPE tables");
-        if (r.index_pos + r.seq_len > c->max_pos)
-            return fail(c, XN_ERR_CAPACITY, "position %lld beyond the RoPE table (%d rows)",
-                        (long long)(r.index_pos + r.seq_len), c->max_pos);
+        const int64_t last = r.index_pos + r.stream->shift[size_t(r.layer)] + r.seq_len;
+        if (last > c->max_pos)
+            return fail(c, XN_ERR_CAPACITY, "position %lld beyond the RoPE table (%d rows)", (long long)last, c->max_pos);
     }
     if ((r.flags & XN_REQ_OUT_PROJ) && !c->out_proj[size_t(r.layer)].set)
         return fail(c, XN_ERR_ARG, "XN_REQ_OUT_PROJ: layer %d has no output block (xn_out_proj_set)", r.layer);
@@ -804,6 +833,7 @@ PrefillArgs make_prefill_args(const xn_ctx* c, const ReqDev& d, const int* pages
     pa.group = c->group;
     pa.seq_len = d.seq_len;
     pa.index_pos = d.index_pos;
+    pa.rope_off = d.rope_off;
     pa.head_dim = c->head_dim;
     pa.scale_log2 = c->scale * 1.4426950408889634f;
     pa.status = c->status_d;
@@ -826,7 +856,7 @@ bool submit_reusing_plan(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, i
         const PlanCache::Entry& e = pc.ent[size_t(i)];
         if (r.stream != e.stream || r.seq_len != 1 || r.index_pos != e.index_pos || r.flags != e.flags ||
             r.layer != layer || int(r.stream->pages.size()) != e.n_pages ||
-            r.index_pos > r.stream->hw[size_t(layer)])
+            r.index_pos > r.stream->hw[size_t(layer)] || r.stream->shift[size_t(layer)] != e.shift)
             return false;
         if ((reinterpret_cast<uintptr_t>(r.q) | reinterpret_cast<uintptr_t>(r.k) |
              reinterpret_cast<uintptr_t>(r.v)) & 15)
@@ -866,6 +896,7 @@ bool submit_reusing_plan(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, i
         for (int i = 0; i < n; ++i) {
             int64_t& hw = reqs[i].stream->hw[size_t(layer)];
             hw = std::max(hw, reqs[i].index_pos + 1);
+            forget_account(reqs[i].stream, layer, reqs[i].index_pos);
         }
         XN_CUDA(c, cudaEventRecord(pc.slot->ev, c->stream));
         pc.slot->used = true;
@@ -1145,6 +1176,7 @@ int32_t submit_locked(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, cuda
         d.n_pages = int(s->pages.size());
         page_ids.insert(page_ids.end(), s->pages.begin(), s->pages.end());
         d.layer = r.layer; d.seq_len = S; d.index_pos = int(r.index_pos);
+        d.rope_off = int(s->shift[size_t(r.layer)]);
         d.cap = int(std::min<int64_t>(s->cap, int64_t(1) << 30));
         if (r.index_pos + S > s->cap) {
             for (int t = 0; t < S; ++t) { ring_rows.push_back(i); ring_rows.push_back(t); }
@@ -1286,6 +1318,8 @@ int32_t submit_locked(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, cuda
 
     // -- launches: every sizing step above has succeeded, the cache positions are going to be written
     undo.commit();
+    for (int i = 0; i < n; ++i)
+        if (reqs[i].seq_len > 0) forget_account(reqs[i].stream, reqs[i].layer, reqs[i].index_pos);
     for (const OutRun& run : qkv_runs) {   // x -> [q | k | v] rows, before anything reads them
         const OutRowDev* rows_d = reinterpret_cast<const OutRowDev*>(slot->dev + o_qkv) + run.row_begin;
         if (c->profile && (rc = profile_begin(c, 3)) != XN_OK) return rc;
@@ -1355,7 +1389,8 @@ int32_t submit_locked(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, cuda
             for (int i = 0; i < n && all; ++i) {
                 if (reqs[i].seq_len != 1) { all = false; break; }
                 pc.ent[size_t(i)] = {reqs[i].stream, reqs[i].index_pos, reqs[i].flags,
-                                     int(reqs[i].stream->pages.size())};
+                                     int(reqs[i].stream->pages.size()),
+                                     reqs[i].stream->shift[size_t(reqs[i].layer)]};
             }
             if (all) {
                 pc.valid = true;
@@ -1699,6 +1734,8 @@ int32_t attention_blocking(xn_ctx* c, const xn_req& req) {
     return me.status;
 }
 
+#include "xn_read.hpp"
+
 }  // namespace
 
 // ============================================================================================
@@ -1812,6 +1849,7 @@ int32_t xn_ctx_create(const xn_ctx_desc* d, xn_ctx** out_ctx) {
     if (const char* env = getenv("XORNET_ATTN_OUTPROJ_PDL")) c->out_pdl = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_OUTPROJ_ROWS")) c->out_rows_kernel = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_PREFILL_PDL")) c->pf_pdl = atoi(env) != 0;
+    if (const char* env = getenv("XORNET_ATTN_READ_TC_MIN_ROWS")) c->read_tc_min_rows = std::max(1, atoi(env));
     if (const char* env = getenv("XORNET_ATTN_F32_TILED")) c->f32_tiled = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_F32_TILED_MIN_ROWS")) c->f32_tiled_min_rows = std::max(1, atoi(env));
 
@@ -1985,6 +2023,8 @@ int32_t xn_ctx_destroy(xn_ctx* c) {
     for (OutSlab& sl : c->slabs)
         if (sl.host) cudaFreeHost(sl.host);
     guarded_free(c, c->partials);
+    guarded_free(c, c->read_ws);
+    guarded_free(c, c->acct_pool);
     if (c->io_host) cudaFreeHost(c->io_host);
     guarded_free(c, c->io_dev);
     guarded_free(c, c->sync_d);
@@ -2077,6 +2117,8 @@ int32_t xn_stream_create(xn_ctx* c, int64_t max_seq_len, xn_stream** out) {
     s->ctx = c;
     s->cap = max_seq_len;
     s->hw.assign(size_t(c->num_layers), 0);
+    s->acc_len.assign(size_t(c->num_layers), 0);
+    s->shift.assign(size_t(c->num_layers), 0);
     {
         std::lock_guard<std::mutex> q(c->q_mu);
         c->streams.insert(s);
@@ -2458,6 +2500,7 @@ int32_t xn_kv_fill_normal(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, in
                                                          n, 1, seed + 0x632BE59BD9B4E019ull * uint64_t(l));
         c->stats.kernel_launches += 1;
         s->hw[size_t(l)] = std::max<int64_t>(s->hw[size_t(l)], t0 + n);
+        forget_account(s, l, t0);
     }
     XN_CUDA(c, cudaGetLastError());
     XN_CUDA(c, cudaEventRecord(slot->ev, c->stream));
@@ -2490,6 +2533,62 @@ int64_t xn_stream_pages(xn_ctx* c, xn_stream* s, int32_t* out, int64_t max_out) 
     const int64_t n = int64_t(s->pages.size());
     for (int64_t i = 0; i < n && i < max_out && out; ++i) out[i] = s->pages[size_t(i)];
     return n;
+}
+
+// ---- reads that do not append, account of attention weight, eviction --------------------------
+// (nothing leaves these entry points but a status: a failed host allocation is one too)
+
+#define XN_GUARDED(c, expr)                                                                    \
+    try {                                                                                      \
+        return expr;                                                                           \
+    } catch (const std::bad_alloc&) {                                                          \
+        return fail(c, XN_ERR_NOMEM, "out of host memory");                                    \
+    } catch (const std::exception& e) {                                                        \
+        return fail(c, XN_ERR_NOMEM, "%s", e.what());                                          \
+    }
+
+int32_t xn_kv_write(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, int64_t n, const float* k,
+                    const float* v, uint32_t flags) {
+    if (!ctx_ok(c)) return XN_ERR_HANDLE;
+    std::lock_guard<std::mutex> g(c->mu);
+    DeviceScope on(c->device);
+    XN_GUARDED(c, kv_write_locked(c, s, layer, t0, n, k, v, flags))
+}
+
+int32_t xn_cross_attention(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
+    if (!ctx_ok(c)) return XN_ERR_HANDLE;
+    std::lock_guard<std::mutex> g(c->mu);
+    DeviceScope on(c->device);
+    XN_GUARDED(c, read_locked(c, n, reqs))
+}
+
+int32_t xn_kv_account_get(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, int64_t n, float* out,
+                          uint32_t flags) {
+    if (!ctx_ok(c)) return XN_ERR_HANDLE;
+    std::lock_guard<std::mutex> g(c->mu);
+    DeviceScope on(c->device);
+    XN_GUARDED(c, account_copy_locked(c, s, layer, t0, n, out, nullptr, flags))
+}
+
+int32_t xn_kv_account_set(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, int64_t n, const float* in,
+                          uint32_t flags) {
+    if (!ctx_ok(c)) return XN_ERR_HANDLE;
+    std::lock_guard<std::mutex> g(c->mu);
+    DeviceScope on(c->device);
+    XN_GUARDED(c, account_copy_locked(c, s, layer, t0, n, nullptr, in, flags))
+}
+
+int32_t xn_kv_evict(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
+    if (!ctx_ok(c)) return XN_ERR_HANDLE;
+    std::lock_guard<std::mutex> g(c->mu);
+    DeviceScope on(c->device);
+    XN_GUARDED(c, evict_locked(c, n, reqs))
+}
+
+int64_t xn_stream_evicted(xn_ctx* c, xn_stream* s, int32_t layer) {
+    if (!ctx_ok(c) || !stream_ok(c, s) || layer < 0 || layer >= c->num_layers) return -1;
+    std::lock_guard<std::mutex> g(c->mu);
+    return s->shift[size_t(layer)];
 }
 
 // ---- attention output block ------------------------------------------------------------------

@@ -51,7 +51,14 @@ struct ReqDev {
                               // token, appended (and rotated) by the attention kernel itself;
                               // bit 4: the prefill kernel rotates the query rows (the append
                               // kernel leaves them alone)
-    int pad;
+    int rope_off;             // added to a position to get its row of the rotary tables (positions
+                              // that left the stream by eviction; 0 otherwise)
+    // Reads that also want the attention weights: raw scores of every (head, row, position) and the
+    // log-sum-exp of every (head, row); read by the kernel's EXT instantiations only.
+    float* scores;
+    long long sc_hs, sc_ts;   // head / row strides of `scores`
+    float* lse;
+    long long lse_hs;         // head stride of `lse` (rows are adjacent)
 };
 
 // What differs between two decode submissions of the same geometry (the same streams at the same

@@ -132,12 +132,23 @@ struct StageHdr {
     float* k_dst;     // cache rows the new token's K / V must be written to (nullptr: another
     float* v_dst;     //   unit of the same KV head does it)
 };
+// ... and, for launches that also want the scores and the log-sum-exp of every row:
+struct StageHdrExt : StageHdr {
+    float* scores;    // of the unit's first query head, at the tile's first token
+    long long sc_hs;
+    float* lse;       // of the unit's first query head
+    long long lse_hs;
+};
+template <bool EXT>
+struct HdrOf { using type = StageHdr; };
+template <>
+struct HdrOf<true> { using type = StageHdrExt; };
 enum : int { kHdrFirst = 1, kHdrLast = 2, kHdrQStaged = 4, kHdrEnd = 8, kHdrRope = 16 };
 
 // Words of the per-context synchronisation array used by the kernel.
 enum : int { kSyncChunk = 0, kSyncDone = 1, kSyncMerge0 = 2 };
 
-template <int NV, int GT>
+template <int NV, int GT, bool EXT = false>
 struct DecodeSmem {
     using Cfg = DecodeCfg<NV>;
     static constexpr bool kStageQ = NV <= 32;  // query rows travel with the first tile of an item
@@ -148,7 +159,7 @@ struct DecodeSmem {
     static constexpr size_t kScratchFloats = size_t(Cfg::kWarps) * (Cfg::kKPW + 1) * 4;  // GT<=4
     static constexpr size_t kBytes = Cfg::kStages * kStageBytes + kRedFloats * 4 +
                                      kScratchFloats * 4 + Cfg::kWarps * 4 * 2 * 4 /* m,l */ +
-                                     Cfg::kStages * sizeof(StageHdr) + 2 * Cfg::kStages * 8 /* barriers */ +
+                                     Cfg::kStages * sizeof(typename HdrOf<EXT>::type) + 2 * Cfg::kStages * 8 /* barriers */ +
                                      32 /* flags */;
 };
 
@@ -172,7 +183,10 @@ struct DecodeSmem {
 //                  counter in `sync`), so no second kernel is needed.
 // EXACT: rows are exactly NV float4 long (nv_arg == NV), which turns every bound check on the
 // row length into a compile-time constant.
-template <int NV, int GT, bool EXACT>
+// EXT: the raw scores (scaled by 1/sqrt(D)) and the log-sum-exp of every row go to ReqDev::scores
+// and ReqDev::lse as well: 4 bytes per query head and position next to the 8 D / GT bytes of K and
+// V that the head's share of the read costs.
+template <int NV, int GT, bool EXACT, bool EXT = false>
 __global__ void __launch_bounds__(DecodeCfg<NV>::kThreads, 1)
 attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
                     const ItemDev* __restrict__ items, const int* __restrict__ chunk_item_begin,
@@ -184,7 +198,8 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     int* __restrict__ status, const __grid_constant__ ReqPatchTable patch) {
     const int nv = EXACT ? NV : nv_arg;
     using Cfg = DecodeCfg<NV>;
-    using Sm = DecodeSmem<NV, GT>;
+    using Sm = DecodeSmem<NV, GT, EXT>;
+    using Hdr = typename HdrOf<EXT>::type;
     constexpr int W = Cfg::kWarps, LPK = Cfg::kLPK, KPI = Cfg::kKPI, TPS = Cfg::kTPS;
     constexpr int KPW = Cfg::kKPW, ITERS = Cfg::kIters, ST = Cfg::kStages;
     constexpr int SQ = Cfg::kSlotsQ, SV = Cfg::kSlotsV;
@@ -198,7 +213,7 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
     float* scratch = red + Sm::kRedFloats;
     float* sm_m = scratch + Sm::kScratchFloats;  // [W][4]
     float* sm_l = sm_m + W * 4;                  // [W][4]
-    StageHdr* hdr = reinterpret_cast<StageHdr*>(sm_l + W * 4);
+    Hdr* hdr = reinterpret_cast<Hdr*>(sm_l + W * 4);
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(hdr + ST);
     uint64_t* empty_bar = full_bar + ST;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(empty_bar + ST);
@@ -241,6 +256,9 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                 const float* v_new = nullptr;
                 int fused = 0;                 // bit 0 fused append, bit 1 rotate, bit 2 this unit stores
                 int pos = 0;
+                float* sc_ptr = nullptr;       // EXT: scores and log-sum-exp of the unit's first head
+                float* lse_ptr = nullptr;
+                long long sc_hs = 0, lse_hs = 0;
                 if (my_it < it_hi) {
                     item = items[my_it];
                     u = units[item.unit];
@@ -262,7 +280,13 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                         k_new = rk + size_t(u.kv_head) * r.kv_hs;
                         v_new = rv + size_t(u.kv_head) * r.kv_hs;
                         fused = 1 | ((r.flags & 1u) ? 2 : 0) | (u.store_new ? 4 : 0);
-                        pos = r.index_pos;
+                        pos = r.index_pos + r.rope_off;
+                    }
+                    if constexpr (EXT) {
+                        sc_ptr = r.scores + size_t(u.head0) * r.sc_hs + size_t(u.t_q) * r.sc_ts;
+                        lse_ptr = r.lse + size_t(u.head0) * r.lse_hs + u.t_q;
+                        sc_hs = r.sc_hs;
+                        lse_hs = r.lse_hs;
                     }
                 }
                 const int n_here = min(32, it_hi - base);
@@ -275,7 +299,14 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     const unsigned long long pages_k =
                         __shfl_sync(kFull, reinterpret_cast<unsigned long long>(pages), k);
                     const unsigned long long lbase_k = __shfl_sync(kFull, (unsigned long long)layer_base, k);
-                    StageHdr h;
+                    Hdr h;
+                    float* sc_k = nullptr;
+                    if constexpr (EXT) {
+                        sc_k = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(sc_ptr), k));
+                        h.lse = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(lse_ptr), k));
+                        h.sc_hs = __shfl_sync(kFull, sc_hs, k);
+                        h.lse_hs = __shfl_sync(kFull, lse_hs, k);
+                    }
                     h.q = reinterpret_cast<const float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(q_ptr), k));
                     h.out = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(o_ptr), k));
                     h.q_hs = __shfl_sync(kFull, q_hs, k);
@@ -337,6 +368,7 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                                     h.new_key = has_new ? ntok - 1 : -1;
                                     h.k_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(k_pool) + src + size_t(ntok - 1) * dp : nullptr;
                                     h.v_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(v_pool) + src + size_t(ntok - 1) * dp : nullptr;
+                                    if constexpr (EXT) h.scores = sc_k + tok0;
                                     hdr[s] = h;
                                     float* dst = stage_ptr(s);
                                     const uint32_t q_bytes = (first && stage_q) ? uint32_t(h.nheads) * row_bytes : 0u;
@@ -381,7 +413,7 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     report_status(status, kDevWaitEmpty);
                     *abort_flag = 1;
                 } else {
-                    StageHdr h = {};
+                    Hdr h = {};
                     h.flags = kHdrEnd;
                     hdr[s] = h;
                     mbar_arrive(&full_bar[s]);
@@ -423,7 +455,7 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
         }
         // (the abort flag is deliberately not polled here: every consumer warp must leave at the
         // same tile, or the block-wide barriers of the merge below would lose a participant)
-        const StageHdr h = hdr[s];
+        const Hdr h = hdr[s];
         if (h.flags & kHdrEnd) break;
         const float4* Ks = reinterpret_cast<const float4*>(stage_ptr(s));
         const float4* Vs = Ks + TPS * NV;
@@ -549,6 +581,9 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                 float dot = group_reduce<GT, LPK>(part, sub);
                 // invalid keys hold stale shared memory: discard whatever came out
                 sc[i] = (key < ntok) ? dot * scale : -INFINITY;
+                if constexpr (EXT) {
+                    if (canon && key < ntok && hown < h.nheads) h.scores[size_t(hown) * h.sc_hs + key] = sc[i];
+                }
                 bm = fmaxf(bm, sc[i]);
             }
 #pragma unroll
@@ -679,6 +714,9 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     L += sm_l[w * 4 + hh] * ((mw == -INFINITY) ? 0.f : expf(mw - M));
                 }
                 const float4 sum = esum[slot];
+                if constexpr (EXT) {
+                    if (h.part < 0 && idx == 0) h.lse[size_t(hh) * h.lse_hs] = M + logf(L);
+                }
                 if (h.part < 0) {
                     float* orow = h.out + size_t(hh) * h.o_hs;
                     const float inv = 1.0f / L;
@@ -736,6 +774,9 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     sum.y = fmaf(wgt, a.y, sum.y);
                     sum.z = fmaf(wgt, a.z, sum.z);
                     sum.w = fmaf(wgt, a.w, sum.w);
+                }
+                if constexpr (EXT) {
+                    if (idx == 0) h.lse[size_t(hh) * h.lse_hs] = M + logf(L);
                 }
                 const float inv = 1.0f / L;
                 float* orow = h.out + size_t(hh) * h.o_hs;

@@ -106,8 +106,8 @@ rope_append_u8_kernel(const ReqDev* __restrict__ reqs, const int* __restrict__ p
             }
         }
         const bool rotate = rope && kind != 2;
-        const float* c = cos_t + size_t(pos) * half;
-        const float* s = sin_t + size_t(pos) * half;
+        const float* c = cos_t + size_t(pos + r.rope_off) * half;
+        const float* s = sin_t + size_t(pos + r.rope_off) * half;
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -477,8 +477,8 @@ attn_splitkv_u8_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restric
             if constexpr (LPK >= 2) {
                 if (fused_rope) {
                     const int half = head_dim / 2;
-                    const float* cs = cos_t + size_t(r.index_pos) * half;
-                    const float* sn = sin_t + size_t(r.index_pos) * half;
+                    const float* cs = cos_t + size_t(r.index_pos + r.rope_off) * half;
+                    const float* sn = sin_t + size_t(r.index_pos + r.rope_off) * half;
 #pragma unroll
                     for (int hh = 0; hh < GT; ++hh) {
                         float x[EPL];
@@ -706,8 +706,8 @@ attn_splitkv_u8_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restric
                 if constexpr (LPK >= 2) {
                     if (fused_rope) {
                         const int half = head_dim / 2;
-                        rope_group<LPK, EPL>(kx, cos_t + size_t(r.index_pos) * half,
-                                             sin_t + size_t(r.index_pos) * half, sub);
+                        rope_group<LPK, EPL>(kx, cos_t + size_t(r.index_pos + r.rope_off) * half,
+                                             sin_t + size_t(r.index_pos + r.rope_off) * half, sub);
                     }
                 }
                 quantize_group<LPK, EPL>(kx, cur[0].k, cur[0].ks);

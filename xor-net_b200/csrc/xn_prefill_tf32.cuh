@@ -53,6 +53,7 @@ struct PrefillArgs {
     int group;            // query heads per KV head
     int seq_len;          // S
     int index_pos;        // P
+    int rope_off;         // table row of a position = position + rope_off
     int head_dim;         // D (multiple of 4, 16..128)
     float scale_log2;     // (1/sqrt(D)) * log2(e)
     int* status;
@@ -475,7 +476,7 @@ prefill_tf32_kernel(const __grid_constant__ CUtensorMap k_map,
                     sv[i] = lo[i];
                     if (i < n_steps && tt < a.seq_len) {
                         const float* qrow = qbase + size_t(tt) * a.q_ts + pch * 4;
-                        const size_t trow = size_t(a.index_pos + tt) * size_t(half) + size_t(pch) * 4;
+                        const size_t trow = size_t(a.index_pos + a.rope_off + tt) * size_t(half) + size_t(pch) * 4;
                         lo[i] = ldg_keep(qrow);
                         hi[i] = ldg_keep(qrow + half);
                         cv[i] = ldg_keep(a.cos_t + trow);

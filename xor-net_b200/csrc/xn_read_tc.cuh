@@ -1,0 +1,1012 @@
+// Attention of many query rows over a cached prefix on the 5th-generation tensor cores (tcgen05),
+// with f32-grade results: the read that does not append (cross attention), its causal form, and
+// the account of attention weight of its rows.  sm_100a only.
+//
+//     S = Q K^T / sqrt(D),  P = softmax(S),  O = P V,  a[j] = sum over rows and group heads of P[.][j]
+//
+// Arithmetic.  Every f32 operand x is scaled by a power of two (per query row, per 64-token page of
+// K and of V, so that the largest magnitude lies in [2^13, 2^14)) and split into two f16 values,
+// x = hi + lo with hi = f16(x) and lo = f16(x - hi): 22 significand bits, and an absolute floor of
+// 2^-39 of the page's (or row's) largest value for elements far below it.  A product takes three
+// MMAs, lo*hi + hi*lo + hi*hi, with f32 accumulators; the lo*lo term (2^-22 relative) is left out.
+// kind::f16 runs at twice the rate of kind::tf32, whose hi/lo split has as many bits, and its
+// operands are half as large.  P is split the same way (scaled by 2^14).  Sums over more than 128
+// positions are not left to the tensor cores' accumulator: every 128-position tile of O starts from
+// zero there and is added up in f32 registers; so are the softmax sums.
+//
+// Passes: (1) page_images_kernel writes K, V and Q once as hi/lo images in the shared-memory layout
+// (128-byte swizzle) that the MMAs read, so that no later block converts anything; (2)
+// read_tc_kernel, one block per (KV head, 128 packed query rows, range of pages), packed row =
+// row * group + head of the group, so that the heads of a group share every K and V tile; (3)
+// read_merge_kernel when a range was split; (4) account_tc_kernel for the attention weights.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "xn_common.cuh"
+#include "xn_prefill_tf32.cuh"
+#include "xn_read.cuh"
+
+namespace xn {
+
+// One request of a launch.
+struct TcReq {
+    const float* q;
+    float* out;
+    long long q_hs, q_ts, o_hs, o_ts;
+    int rows;
+    int kv_len;
+    int causal;        // row t sees positions up to kv_len - rows + t; else all
+    int page_off;
+    int layer;
+    int n_pages;       // pages of the prefix
+    int n_qt;          // 128-row tiles of packed query rows per KV head
+    long long img0;    // page image (page, head) = img0 + page * num_kv_heads + head
+    long long qimg0;   // query image (head, tile) = qimg0 + head * n_qt + tile
+    AccountDev acct;   // the account kernel's destination
+};
+
+// A block of read_tc_kernel: 128 packed rows of one KV head over pages [page_begin, page_end).
+struct TcItem {
+    int req, head, qt;
+    int page_begin, page_end;
+    int part;          // partial record, or -1: the block writes the output itself
+};
+// A row tile that was split over several items: its partial records are consecutive.
+struct TcMerge {
+    int req, head, qt;
+    int part_begin, part_count;
+    int pad;
+};
+// A block of account_tc_kernel: 128 positions of one KV head.
+struct TcKeyTile {
+    int req, head, tile, qt_begin;
+};
+
+// What the softmax needs to know about a page: factors that undo the scaling of K and V, and the
+// rows that hold an infinity or a NaN (their images are zero; they are added exactly on the side).
+struct __align__(16) PageMeta {
+    float fk, fv;
+    unsigned long long bad_k, bad_v;
+    unsigned long long pad;
+};
+
+// Where the cache rows are, for the rare exact path and the image kernel.
+struct CacheView {
+    const float* k;
+    const float* v;
+    const uint8_t* u8;
+    long long pool_pages;
+    int num_kv_heads, head_dim, nv, dq;
+};
+
+namespace rt {
+
+constexpr int kBM = 128;
+constexpr int kPage = 64;
+constexpr int kSub = kPage * 128;        // one column block (64 halves) of one page
+constexpr int kRowsSub = kBM * 128;      // one column block of 128 rows
+constexpr float kPScale = 16384.0f;      // 2^14: P is split at this scale
+constexpr int kThreads = 320;            // copy warp, MMA warp, two softmax warpgroups
+constexpr int kVStages = 3;
+constexpr int kQBytes = 4 * kRowsSub;    // 64 KB: hi and lo, two column blocks
+constexpr int kKBytes = 4 * kRowsSub;
+constexpr int kVBytes = 4 * kSub;        // 32 KB
+constexpr int kSmemData = kQBytes + kKBytes + kVStages * kVBytes;
+constexpr int kSmemBytes = kSmemData + 3072;   // 227 KB, all there is: the block's window starts 1024-byte aligned
+static_assert(kSmemBytes <= 232448, "shared memory of a block");
+constexpr int kTmemS = 0;                // 2 x 128 columns
+constexpr int kTmemO = 256;              // 2 x 128 columns
+
+constexpr int kAcctQStages = 2;
+constexpr int kAcctSmemData = kKBytes + kAcctQStages * kQBytes;
+constexpr int kAcctSmemBytes = kAcctSmemData + 1024 + 4096;
+
+__host__ __device__ inline int blocks_of(int head_dim) { return head_dim > 64 ? 2 : 1; }
+__host__ __device__ inline size_t page_image_bytes(int head_dim) { return size_t(4) * blocks_of(head_dim) * kSub; }
+__host__ __device__ inline size_t q_image_bytes(int head_dim) { return size_t(2) * blocks_of(head_dim) * kRowsSub; }
+// a partial record: O [128][dp], then m [128], l [128]
+__host__ __device__ inline size_t part_floats(int dp) { return size_t(kBM) * dp + 2 * kBM; }
+
+// Instruction descriptor, kind::f16 with f16 operands and f32 accumulators.
+__host__ __device__ constexpr uint32_t make_idesc16(int m, int n, int b_mn_major) {
+    return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// Power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Magnitudes
+// below 2^-60 stay smaller than that, so that the product of two inverse factors never vanishes
+// (masked scores are -inf times that product); nothing but zeros: as for 1.
+__device__ __forceinline__ void scale_of(float m, float& up, float& down) {
+    int e = int((__float_as_uint(m) >> 23) & 255u) - 127;
+    e = m == 0.f ? 0 : max(e, -60);
+    up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
+    down = __uint_as_float(uint32_t(127 - 13 + e) << 23);
+}
+
+__device__ __forceinline__ bool finite4(const float4& x) {
+    // x - x is 0 for finite x and NaN otherwise
+    return (x.x - x.x) + (x.y - x.y) + (x.z - x.z) + (x.w - x.w) == 0.f;
+}
+__device__ __forceinline__ float max4(const float4& x) {
+    return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (hi, lo) f16 pairs of two f32 values; lo is 0 behind an infinite or NaN hi
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack2(a - back.x, b - back.y);
+}
+
+// Four scaled values of a lane (columns 4 * lane ..) into the hi and lo images of a row: column block
+// lane / 16, 16-byte chunk (lane % 16) / 2 at chunk position chunk ^ (row & 7).
+__device__ __forceinline__ void store_row_image(unsigned char* hi_img, unsigned char* lo_img, size_t block_stride,
+                                                int row, int lane, int nb, float4 x, bool safe) {
+    if ((lane >> 4) >= nb) return;
+    uint2 hi, lo;
+    split2(x.x, x.y, hi.x, lo.x);
+    split2(x.z, x.w, hi.y, lo.y);
+    if (!safe) lo = make_uint2(0u, 0u);   // a query row with an infinity: inf - inf must not become NaN
+    const size_t at = size_t(lane >> 4) * block_stride + size_t(row) * 128 +
+                      size_t((((lane & 15) >> 1) ^ (row & 7)) * 16 + (lane & 1) * 8);
+    *reinterpret_cast<uint2*>(hi_img + at) = hi;
+    *reinterpret_cast<uint2*>(lo_img + at) = lo;
+}
+
+// One element of a cached row, whatever the format (rare paths only).
+__device__ __forceinline__ float cache_elem(const CacheView& c, const int* pages, int layer, int head, int key, int d, bool v) {
+    const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
+    const int tk = key % kPage;
+    if (c.u8) {
+        const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
+        const float sc = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq)[(v ? kPage : 0) + tk];
+        return (float(b[size_t((v ? kPage : 0) + tk) * c.dq + d]) - 128.0f) * sc;
+    }
+    return (v ? c.v : c.k)[(blk * kPage + tk) * size_t(c.nv) * 4 + d];
+}
+
+}  // namespace rt
+
+// Pass 1.  Blocks [0, n_page_blocks): one page of one KV head each (K and V); the rest: one 128-row
+// query tile each.  A warp handles a row per step, 4 columns per lane.  Bound by memory: 4 bytes
+// read and 4 written per element.
+__global__ void __launch_bounds__(256)
+page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_blocks,
+                   const int* __restrict__ page_ids, CacheView c, unsigned char* __restrict__ images,
+                   PageMeta* __restrict__ meta, unsigned char* __restrict__ q_images,
+                   float2* __restrict__ row_meta, float scale_log2, int group) {
+    using namespace rt;
+    pdl_launch_dependents();
+    __shared__ float s_max[2][8];
+    __shared__ unsigned s_bad[2][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = c.head_dim, nb = blocks_of(D);
+    pdl_wait();
+    if ((long long)blockIdx.x < n_page_blocks) {
+        const long long id = blockIdx.x;
+        int rq = 0;
+        while (rq + 1 < n_reqs && id >= reqs[rq + 1].img0) ++rq;
+        const TcReq& r = reqs[rq];
+        const long long local = id - r.img0;
+        const int page = int(local / c.num_kv_heads), h = int(local % c.num_kv_heads);
+        const int ntok = min(kPage, r.kv_len - page * kPage);
+        const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_ids[r.page_off + page])) * c.num_kv_heads + h;
+        float4 x[2][8];
+        if (c.u8) {
+            const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
+            const float* sc = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int tk = warp * 8 + i;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    x[kv][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (tk < ntok && lane * 4 < c.dq) {
+                        const uchar4 u = *reinterpret_cast<const uchar4*>(b + size_t(kv * kPage + tk) * c.dq + lane * 4);
+                        const float s = sc[kv * kPage + tk];
+                        // (bytes past head_dim hold 128, but 0 * s is NaN for an infinite scale)
+                        if (lane * 4 + 0 < D) x[kv][i].x = (float(u.x) - 128.0f) * s;
+                        if (lane * 4 + 1 < D) x[kv][i].y = (float(u.y) - 128.0f) * s;
+                        if (lane * 4 + 2 < D) x[kv][i].z = (float(u.z) - 128.0f) * s;
+                        if (lane * 4 + 3 < D) x[kv][i].w = (float(u.w) - 128.0f) * s;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int tk = warp * 8 + i;
+                x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (tk < ntok && lane < c.nv) {   // rows are padded with zeros to whole float4
+                    const size_t at = (blk * kPage + tk) * size_t(c.nv) * 4 + size_t(lane) * 4;
+                    x[0][i] = *reinterpret_cast<const float4*>(c.k + at);
+                    x[1][i] = *reinterpret_cast<const float4*>(c.v + at);
+                }
+            }
+        }
+        float mx[2] = {0.f, 0.f};
+        unsigned bad[2] = {0u, 0u};
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!__all_sync(0xffffffffu, finite4(x[kv][i]))) {
+                    bad[kv] |= 1u << i;
+                    x[kv][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                mx[kv] = fmaxf(mx[kv], max4(x[kv][i]));
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+        }
+        if (lane == 0) {
+            s_max[0][warp] = mx[0];
+            s_max[1][warp] = mx[1];
+            s_bad[0][warp] = bad[0];
+            s_bad[1][warp] = bad[1];
+        }
+        __syncthreads();
+        float up[2], down[2];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            float m = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) m = fmaxf(m, s_max[kv][w]);
+            scale_of(m, up[kv], down[kv]);
+        }
+        if (threadIdx.x == 0) {
+            PageMeta pm = {};
+            pm.fk = down[0];
+            pm.fv = down[1];
+            for (int w = 0; w < 8; ++w) {
+                pm.bad_k |= (unsigned long long)(s_bad[0][w]) << (8 * w);
+                pm.bad_v |= (unsigned long long)(s_bad[1][w]) << (8 * w);
+            }
+            meta[id] = pm;
+        }
+        unsigned char* img = images + size_t(id) * page_image_bytes(D);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 y = make_float4(x[kv][i].x * up[kv], x[kv][i].y * up[kv], x[kv][i].z * up[kv], x[kv][i].w * up[kv]);
+                unsigned char* hi = img + size_t(kv) * 2 * nb * kSub;
+                store_row_image(hi, hi + size_t(nb) * kSub, kSub, warp * 8 + i, lane, nb, y, true);
+            }
+    } else {
+        const long long qid = (long long)blockIdx.x - n_page_blocks;
+        int rq = 0;
+        while (rq + 1 < n_reqs && qid >= reqs[rq + 1].qimg0) ++rq;
+        const TcReq& r = reqs[rq];
+        const int local = int(qid - r.qimg0);
+        const int h = local / r.n_qt, qt = local % r.n_qt;
+        const int n_packed = r.rows * group;
+        const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
+        unsigned char* img = q_images + size_t(qid) * q_image_bytes(D);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int pr = qt * kBM + half * 64 + warp * 8 + i;
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (pr < n_packed) {
+                    const float* row = r.q + size_t(h * group + pr % group) * r.q_hs + size_t(pr / group) * r.q_ts;
+                    const int d = lane * 4;
+                    if (vec) {
+                        if (d < D) x[i] = *reinterpret_cast<const float4*>(row + d);
+                    } else {
+                        if (d + 0 < D) x[i].x = row[d + 0];
+                        if (d + 1 < D) x[i].y = row[d + 1];
+                        if (d + 2 < D) x[i].z = row[d + 2];
+                        if (d + 3 < D) x[i].w = row[d + 3];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int rr = half * 64 + warp * 8 + i;
+                const bool ok = __all_sync(0xffffffffu, finite4(x[i]));
+                float m = max4(x[i]);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                float up, down;
+                scale_of(ok ? m : 1.f, up, down);
+                const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+                store_row_image(img, img + size_t(nb) * kRowsSub, kRowsSub, rr, lane, nb, y, ok);
+                // y: the log-sum-exp of the row, written by the attention kernel; rows past the end
+                // (and rows that see nothing) keep +inf, which gives them no weight anywhere
+                if (lane == 0) row_meta[size_t(qid) * kBM + rr] = make_float2(down * scale_log2, INFINITY);
+            }
+        }
+    }
+}
+
+// Pass 2.  Shared memory: Q images 64 KB | K tile (two pages) 64 KB | three V pages of 32 KB.  Tensor
+// memory: two S / P buffers and two O tiles of 128 columns.  Roles (320 threads): warp 0 copies
+// images (1-D bulk copies), warp 1 issues the MMAs -- the S of tile j + 1 before the O of tile j, so
+// that the softmax of a tile runs beside them -- and warps 2..9 are two softmax warpgroups: thread
+// r of each owns packed row r; warpgroup w takes page w of every tile and columns [64 w, 64 w + 64)
+// of O.  S is read from tensor memory, P goes back over it as hi (32 columns) and lo (32 columns).
+// Every wait is bounded; on expiry the kernel records a status code, drains and returns.
+__global__ void __launch_bounds__(rt::kThreads, 1)
+read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items, const int* __restrict__ page_ids,
+               CacheView c, const unsigned char* __restrict__ images, const PageMeta* __restrict__ meta,
+               const unsigned char* __restrict__ q_images, float2* __restrict__ row_meta,
+               float* __restrict__ partials, float scale_log2, int group, int want_lse, int* __restrict__ status) {
+    using namespace rt;
+    using pf::fence_after_sync;
+    using pf::fence_before_sync;
+    using pf::mma_commit;
+    using pf::smem_desc;
+    using pf::tmem_ld32;
+    using pf::tmem_st32;
+    using pf::tmem_wait_ld;
+    using pf::tmem_wait_st;
+    extern __shared__ __align__(1024) unsigned char read_smem[];
+    unsigned char* smem = read_smem;
+    if (smem_u32(smem) & 1023u) {   // (the swizzled images need it; never seen otherwise)
+        if (threadIdx.x == 0) report_status(status, kDevBadIndex);
+        return;
+    }
+    unsigned char* q_s = smem;
+    unsigned char* k_s = q_s + kQBytes;
+    unsigned char* v_s = k_s + kKBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemData);
+    uint64_t* q_full = bars + 0;
+    uint64_t* k_full = bars + 1;
+    uint64_t* k_empty = bars + 2;
+    uint64_t* v_full = bars + 3;               // [3]
+    uint64_t* v_empty = v_full + kVStages;     // [3]
+    uint64_t* s_full = v_empty + kVStages;     // [2]
+    uint64_t* p_full = s_full + 2;             // [2]
+    uint64_t* o_full = p_full + 2;             // [2]
+    uint64_t* o_empty = o_full + 2;            // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    // by tile parity: a fast warp of the next tile must not be seen by a slow one of this tile
+    volatile int* sm_dead = abort_flag + 1;              // [2]
+    float* xchg = reinterpret_cast<float*>(bars + 32);   // [2 tiles][2 warpgroups][128 rows]
+
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const TcItem it = items[blockIdx.x];
+    const TcReq& r = reqs[it.req];
+    const int D = c.head_dim, nb = blocks_of(D);
+    const int n_pages = it.page_end - it.page_begin;
+    const int n_tiles = (n_pages + 1) / 2;
+    const int k_steps = (D + 15) / 16;
+    const int n_pv = (D + 15) / 16 * 16;
+    const long long qid = r.qimg0 + (long long)it.head * r.n_qt + it.qt;
+    const long long img0 = r.img0 + (long long)it.page_begin * c.num_kv_heads + it.head;
+
+    if (tid == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(k_full, 1);
+        mbar_init(k_empty, 1);
+        for (int s = 0; s < kVStages; ++s) {
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 256);
+            mbar_init(&o_full[s], 1);
+            mbar_init(&o_empty[s], 256);
+        }
+        *abort_flag = 0;
+        sm_dead[0] = sm_dead[1] = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();   // the images come from the kernel before this one
+
+    if (warp == 0) {
+        // =============================== image copies ===============================
+        if (lane == 0) {
+            const size_t img_bytes = page_image_bytes(D);
+            const size_t step = size_t(c.num_kv_heads) * img_bytes;   // next page of the same head
+            const unsigned char* base = images + size_t(img0) * img_bytes;
+            mbar_arrive_expect_tx(q_full, uint32_t(q_image_bytes(D)));
+            bulk_g2s(q_s, q_images + size_t(qid) * q_image_bytes(D), uint32_t(q_image_bytes(D)), q_full);
+            auto load_k = [&](int j) -> bool {
+                if (j > 0 && !mbar_spin_bounded(k_empty, uint32_t((j - 1) & 1))) return false;
+                const int np = min(2, n_pages - 2 * j);
+                mbar_arrive_expect_tx(k_full, uint32_t(np * 2 * nb) * kSub);
+                for (int p = 0; p < np; ++p)
+                    for (int b = 0; b < 2 * nb; ++b)   // hi blocks, then lo blocks
+                        bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
+                                 base + size_t(2 * j + p) * step + size_t(b) * kSub, kSub, k_full);
+                return true;
+            };
+            auto load_v = [&](int pg) -> bool {
+                const int st = pg % kVStages;
+                if (pg >= kVStages && !mbar_spin_bounded(&v_empty[st], uint32_t((pg / kVStages - 1) & 1))) return false;
+                const uint32_t bytes = uint32_t(2 * nb) * kSub;
+                mbar_arrive_expect_tx(&v_full[st], bytes);
+                bulk_g2s(v_s + size_t(st) * kVBytes, base + size_t(pg) * step + size_t(2 * nb) * kSub, bytes, &v_full[st]);
+                return true;
+            };
+            bool ok = load_k(0);
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                if (j + 1 < n_tiles) ok = load_k(j + 1);
+                for (int p = 2 * j; p < min(2 * j + 2, n_pages) && ok; ++p) ok = load_v(p);
+                if (*abort_flag) break;
+            }
+            if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
+        }
+    } else if (warp == 1) {
+        // =============================== MMA issuer ===============================
+        if (lane == 0) {
+            const uint32_t id_qk = make_idesc16(kBM, kBM, 0);
+            const uint32_t id_pv = make_idesc16(kBM, n_pv, 1);
+            const uint64_t qd = smem_desc(smem_u32(q_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t kd = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t vd0 = smem_desc(smem_u32(v_s), kSub, 1024, pf::kLayoutSw128);
+            const uint64_t lo_rows = uint64_t(nb) * kRowsSub >> 4;   // hi image -> lo image, 128 rows
+            const uint64_t lo_page = uint64_t(nb) * kSub >> 4;       // ... of a page
+            bool ok = mbar_spin_bounded(q_full, 0);
+            if (!ok) { report_status(status, kDevWaitFull); *abort_flag = 1; }
+            int v_st = 0, v_ph = 0;
+            auto issue_qk = [&](int j) -> bool {
+                if (!mbar_spin_bounded(k_full, uint32_t(j & 1))) return false;
+                fence_after_sync();
+                const uint32_t d = tmem + kTmemS + (j & 1) * 128;
+                // the small products first: they meet a small accumulator
+#pragma unroll
+                for (int term = 0; term < 3; ++term) {
+                    const uint64_t a0 = qd + (term == 0 ? lo_rows : 0), b0 = kd + (term == 1 ? lo_rows : 0);
+                    for (int ks = 0; ks < k_steps; ++ks) {
+                        const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
+                        mma16_ss(d, a0 + o, b0 + o, id_qk, (term > 0 || ks > 0) ? 1u : 0u);
+                    }
+                }
+                mma_commit(k_empty);
+                mma_commit(&s_full[j & 1]);
+                return true;
+            };
+            auto issue_pv = [&](int j) -> bool {
+                if (!mbar_spin_bounded(&p_full[j & 1], uint32_t((j >> 1) & 1))) return false;
+                if (j >= 2 && !mbar_spin_bounded(&o_empty[j & 1], uint32_t(((j >> 1) - 1) & 1))) return false;
+                const int np = min(2, n_pages - 2 * j);
+                const uint32_t d = tmem + kTmemO + (j & 1) * 128;
+                for (int p = 0; p < np; ++p) {
+                    if (!mbar_spin_bounded(&v_full[v_st], uint32_t(v_ph))) return false;
+                    fence_after_sync();
+                    const uint64_t vd = vd0 + uint64_t(v_st) * (kVBytes >> 4);
+                    const uint32_t pa = tmem + kTmemS + (j & 1) * 128 + p * 64;
+#pragma unroll
+                    for (int term = 0; term < 3; ++term) {
+                        const uint32_t a0 = pa + (term == 0 ? 32 : 0);
+                        const uint64_t b0 = vd + (term == 1 ? lo_page : 0);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma16_ts(d, a0 + ks * 8, b0 + ks * 128, id_pv, (p > 0 || term > 0 || ks > 0) ? 1u : 0u);
+                    }
+                    mma_commit(&v_empty[v_st]);
+                    if (++v_st == kVStages) { v_st = 0; v_ph ^= 1; }
+                }
+                mma_commit(&o_full[j & 1]);
+                return true;
+            };
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                if (!issue_qk(j)) { ok = false; break; }
+                if (j >= 1 && !issue_pv(j - 1)) { ok = false; break; }
+            }
+            if (ok && !issue_pv(n_tiles - 1)) ok = false;
+            if (!ok) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+        }
+    } else {
+        // =============================== softmax + epilogue ===============================
+        constexpr unsigned kFull = 0xffffffffu;
+        const int wg = (warp - 2) >> 2;
+        const int quarter = warp & 3;
+        const int rr = quarter * 32 + lane;               // row of the tile
+        const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+        const int pr = it.qt * kBM + rr;                  // packed row
+        const int n_packed = r.rows * group;
+        const int t = pr / group;
+        const int col0 = wg * 64;
+        // positions below `limit` are visible
+        const int limit = pr >= n_packed ? 0 : (r.causal ? r.kv_len - r.rows + t + 1 : r.kv_len);
+        const int limit_first = r.causal ? r.kv_len - r.rows + (it.qt * kBM) / group + 1 : r.kv_len;
+        const int* pages = page_ids + r.page_off;
+        auto wg_barrier = [&]() { named_bar_sync(1, 256); };
+        const float cq = __ldcg(&row_meta[size_t(qid) * kBM + rr]).x;
+        const bool my_cols = col0 < n_pv;                 // head_dim <= 64: the second half has none
+
+        float o[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) o[i] = 0.f;
+        float m_ref = -INFINITY, l_sum = 0.f;
+        float alpha_prev = 1.f, f_prev = 0.f;             // pending accumulation of tile j - 1
+        bool dead = false;
+        // O += (tile j of tensor memory) * f, after O *= alpha
+        auto add_tile = [&](int j, float alpha, float f) -> bool {
+            if (!warp_spin_bounded(&o_full[j & 1], uint32_t((j >> 1) & 1), lane)) return false;
+            fence_after_sync();
+            if (my_cols) {
+                uint32_t a[32];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    tmem_ld32(tmem + kTmemO + (j & 1) * 128 + lane_base + col0 + hf * 32, a);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[hf * 32 + i] = fmaf(__uint_as_float(a[i]), f, o[hf * 32 + i] * alpha);
+                }
+            }
+            fence_before_sync();
+            mbar_arrive(&o_empty[j & 1]);
+            return true;
+        };
+        const PageMeta* pm = meta + img0;
+        for (int j = 0; j < n_tiles; ++j) {
+            const int sb = j & 1;
+            const bool two = 2 * j + 1 < n_pages;
+            const bool have = wg == 0 || two;
+            // both pages' factors (uniform over the block)
+            const PageMeta pm0 = pm[size_t(2 * j) * c.num_kv_heads];
+            const PageMeta pm1 = two ? pm[size_t(2 * j + 1) * c.num_kv_heads] : pm0;
+            const PageMeta& own = wg ? pm1 : pm0;
+            const float fv = fmaxf(pm0.fv, pm1.fv);
+            if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
+            if (lane == 0 && dead) { sm_dead[sb] = 1; *abort_flag = 1; }
+            fence_after_sync();
+            uint32_t x0[32], x1[32];
+            const uint32_t s_addr = tmem + kTmemS + lane_base + sb * 128 + col0;
+            const int key0 = (it.page_begin + 2 * j + wg) * kPage;
+            const float cm = cq * own.fk;
+            float mx = -INFINITY;
+            if (!dead && have) {
+                tmem_ld32(s_addr, x0);
+                tmem_ld32(s_addr + 32, x1);
+                tmem_wait_ld();
+                if (own.bad_k) {
+                    // rows of K with an infinity or a NaN: their scores one by one, in f32
+                    unsigned long long b = own.bad_k;
+                    while (b) {
+                        const int cidx = __ffsll((long long)b) - 1;
+                        b &= b - 1;
+                        float dot = 0.f;
+                        if (pr < n_packed)
+                            for (int d = 0; d < D; ++d)
+                                dot = fmaf(r.q[size_t(it.head * group + pr % group) * r.q_hs + size_t(t) * r.q_ts + d],
+                                           cache_elem(c, pages, r.layer, it.head, key0 + cidx, d, false), dot);
+                        const uint32_t bits = __float_as_uint(dot * scale_log2 / cm);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i == cidx) x0[i] = bits;
+                            if (i + 32 == cidx) x1[i] = bits;
+                        }
+                    }
+                }
+                if (key0 + kPage > limit_first) {    // some row masks some position here
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (key0 + i >= limit) x0[i] = 0xff800000u;
+                        if (key0 + 32 + i >= limit) x1[i] = 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x0[i]), __uint_as_float(x1[i])));
+                mx *= cm;
+            }
+            float* xc = xchg + sb * 256;
+            xc[wg * 128 + rr] = mx;
+            wg_barrier();
+            dead = __any_sync(kFull, sm_dead[sb] != 0);
+            if (dead) break;   // taken by all eight warps: the flag was set before the barrier
+            mx = fmaxf(mx, xc[(wg ^ 1) * 128 + rr]);
+            const float m_new = fmaxf(m_ref, mx);
+            const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+            float alpha = m_new == -INFINITY ? 1.f : pf::ex2(m_ref - m_new);
+            m_ref = m_new;
+            l_sum *= alpha;
+            if (have) {
+                const float pscale = kPScale * (own.fv / fv);   // powers of two: exact
+                float ps0 = 0.f, ps1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float a = pf::ex2(fmaf(__uint_as_float(x0[i]), cm, neg_m));
+                    const float b = pf::ex2(fmaf(__uint_as_float(x0[i + 1]), cm, neg_m));
+                    ps0 += a;
+                    ps1 += b;
+                    uint32_t hi, lo;
+                    split2(a * pscale, b * pscale, hi, lo);
+                    x0[i] = hi;
+                    x0[i + 1] = lo;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float a = pf::ex2(fmaf(__uint_as_float(x1[i]), cm, neg_m));
+                    const float b = pf::ex2(fmaf(__uint_as_float(x1[i + 1]), cm, neg_m));
+                    ps0 += a;
+                    ps1 += b;
+                    uint32_t hi, lo;
+                    split2(a * pscale, b * pscale, hi, lo);
+                    x1[i] = hi;
+                    x1[i + 1] = lo;
+                }
+                l_sum += ps0 + ps1;
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { w[i] = x0[2 * i]; w[16 + i] = x1[2 * i]; }
+                tmem_st32(s_addr, w);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { w[i] = x0[2 * i + 1]; w[16 + i] = x1[2 * i + 1]; }
+                tmem_st32(s_addr + 32, w);
+                tmem_wait_st();
+            }
+            const unsigned long long bad0 = pm0.bad_v, bad1 = two ? pm1.bad_v : 0ull;
+            if (bad0 | bad1) {
+                // rows of V with an infinity or a NaN (uniform over the block): bring O up to date, then
+                // add p * v for the rows that see them; P of both pages is read back from tensor memory
+                if (j > 0) {
+                    if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+                }
+#pragma unroll
+                for (int i = 0; i < 64; ++i) o[i] *= alpha;
+                alpha = 1.f;
+                fence_before_sync();
+                wg_barrier();
+                fence_after_sync();
+                for (int p = 0; p < 2; ++p) {
+                    unsigned long long b = p ? bad1 : bad0;
+                    const float unscale = fv / (kPScale * (p ? pm1.fv : pm0.fv));
+                    while (b) {
+                        const int cidx = __ffsll((long long)b) - 1;
+                        b &= b - 1;
+                        uint32_t hi[32], lo[32];
+                        tmem_ld32(tmem + kTmemS + lane_base + sb * 128 + p * 64, hi);
+                        tmem_ld32(tmem + kTmemS + lane_base + sb * 128 + p * 64 + 32, lo);
+                        tmem_wait_ld();
+                        uint32_t hw = 0, lw = 0;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i == cidx / 2) { hw = hi[i]; lw = lo[i]; }
+                        const float2 h2 = __half22float2(*reinterpret_cast<__half2*>(&hw));
+                        const float2 l2 = __half22float2(*reinterpret_cast<__half2*>(&lw));
+                        const float pv = ((cidx & 1) ? h2.y + l2.y : h2.x + l2.x) * unscale;
+                        const int key = (it.page_begin + 2 * j + p) * kPage + cidx;
+                        if (key < limit) {   // (a weight of zero times an infinity is a NaN, as in a plain sum)
+#pragma unroll 1
+                            for (int d = 0; d < 64; ++d) {
+                                if (col0 + d >= D) break;
+                                const float add = pv * cache_elem(c, pages, r.layer, it.head, key, col0 + d, true);
+#pragma unroll
+                                for (int i = 0; i < 64; ++i)
+                                    if (i == d) o[i] += add;
+                            }
+                        }
+                    }
+                }
+                fence_before_sync();
+                wg_barrier();
+            } else if (j > 0) {
+                fence_before_sync();
+                mbar_arrive(&p_full[sb]);
+                if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+                alpha_prev = alpha;
+                f_prev = fv * (1.0f / kPScale);
+                continue;
+            }
+            alpha_prev = alpha;
+            f_prev = fv * (1.0f / kPScale);
+            fence_before_sync();
+            mbar_arrive(&p_full[sb]);
+        }
+        if (dead && lane == 0) report_status(status, kDevWaitFull);
+        if (!dead) {
+            if (!add_tile(n_tiles - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+            // (the exchange area of the tile before the last one: every thread has read the last one's
+            // only behind the barrier below)
+            float* xc = xchg + (n_tiles & 1) * 256;
+            xc[wg * 128 + rr] = l_sum;
+            wg_barrier();
+            const float l_tot = l_sum + xc[(wg ^ 1) * 128 + rr];
+            const bool whole = it.part < 0;
+            const float inv = whole ? (l_tot == 0.f ? 0.f : 1.0f / l_tot) : 1.0f;
+            if (wg == 0) {
+                if (!whole) {
+                    float* rec = partials + size_t(it.part) * part_floats(c.nv * 4) + size_t(kBM) * c.nv * 4;
+                    rec[rr] = m_ref;
+                    rec[kBM + rr] = l_tot;
+                } else if (want_lse && pr < n_packed && l_tot != 0.f) {
+                    row_meta[size_t(qid) * kBM + rr].y = m_ref + log2f(l_tot);
+                }
+            }
+            // through shared memory (the K tile is idle) so that whole rows leave in one instruction
+            float4* tile = reinterpret_cast<float4*>(k_s);   // [128 rows][32 chunks]
+            if (my_cols) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 4) {
+                    const int chunk = (col0 + i) >> 2;
+                    tile[rr * 32 + (chunk ^ (rr & 31))] = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                }
+            }
+            wg_barrier();
+            const int w8 = warp - 2;
+            const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.out) | uintptr_t(r.o_hs * 4) | uintptr_t(r.o_ts * 4)) & 15) == 0;
+            for (int i = w8 * 16; i < w8 * 16 + 16; ++i) {
+                const int p = it.qt * kBM + i;
+                if (p >= n_packed || lane >= c.nv) continue;
+                const float4 x = tile[i * 32 + (lane ^ (i & 31))];
+                if (!whole) {
+                    *reinterpret_cast<float4*>(partials + size_t(it.part) * part_floats(c.nv * 4) + size_t(i) * c.nv * 4 + lane * 4) = x;
+                    continue;
+                }
+                float* row = r.out + size_t(it.head * group + p % group) * r.o_hs + size_t(p / group) * r.o_ts + lane * 4;
+                if (vec) {
+                    *reinterpret_cast<float4*>(row) = x;
+                } else {
+                    row[0] = x.x;
+                    if (lane * 4 + 1 < D) row[1] = x.y;
+                    if (lane * 4 + 2 < D) row[2] = x.z;
+                    if (lane * 4 + 3 < D) row[3] = x.w;
+                }
+            }
+        }
+    }
+
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Pass 3.  The partial records of a split row tile, combined with their log-sum-exp weights: one warp
+// per row, the tile's rows over blockIdx.y.
+__global__ void __launch_bounds__(256)
+read_merge_kernel(const TcReq* __restrict__ reqs, const TcMerge* __restrict__ merges,
+                  const float* __restrict__ partials, float2* __restrict__ row_meta, int group, int head_dim,
+                  int nv, int want_lse) {
+    using namespace rt;
+    pdl_launch_dependents();
+    const TcMerge mg = merges[blockIdx.x];
+    const TcReq& r = reqs[mg.req];
+    const int lane = threadIdx.x & 31;
+    const int i = int(blockIdx.y) * 8 + int(threadIdx.x >> 5);
+    const int p = mg.qt * kBM + i;
+    if (p >= r.rows * group) return;
+    pdl_wait();
+    const size_t stride = part_floats(nv * 4);
+    const float* rec = partials + size_t(mg.part_begin) * stride;
+    const float* ml = rec + size_t(kBM) * nv * 4;
+    float m = -INFINITY;
+    for (int k = 0; k < mg.part_count; ++k) m = fmaxf(m, ml[size_t(k) * stride + i]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < mg.part_count; ++k) {
+        const float mk = ml[size_t(k) * stride + i];
+        const float w = mk == -INFINITY ? 0.f : pf::ex2(mk - m);
+        l = fmaf(ml[size_t(k) * stride + kBM + i], w, l);
+        if (lane < nv) {
+            const float4 x = *reinterpret_cast<const float4*>(rec + size_t(k) * stride + size_t(i) * nv * 4 + lane * 4);
+            o.x = fmaf(w, x.x, o.x);
+            o.y = fmaf(w, x.y, o.y);
+            o.z = fmaf(w, x.z, o.z);
+            o.w = fmaf(w, x.w, o.w);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    float* row = r.out + size_t(mg.head * group + p % group) * r.o_hs + size_t(p / group) * r.o_ts;
+    const int d = lane * 4;
+    if (d + 0 < head_dim) row[d + 0] = o.x * inv;
+    if (d + 1 < head_dim) row[d + 1] = o.y * inv;
+    if (d + 2 < head_dim) row[d + 2] = o.z * inv;
+    if (d + 3 < head_dim) row[d + 3] = o.w * inv;
+    if (want_lse && lane == 0 && l != 0.f)
+        row_meta[size_t(r.qimg0 + (long long)mg.head * r.n_qt + mg.qt) * kBM + i].y = m + log2f(l);
+}
+
+// Pass 4.  The account: S^T = K Q^T for 128 positions of one KV head against every tile of 128 packed
+// query rows that sees them, p = 2^(s - lse), summed over the rows in f32.  Positions are the rows of
+// the accumulator, so a thread owns a position and the sum needs no exchange and no atomics (its
+// order is fixed).  Half the MMAs of the attention itself.  Roles as above; the K tile stays, the
+// query images stream through two stages.
+__global__ void __launch_bounds__(rt::kThreads, 1)
+account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ tiles, const int* __restrict__ page_ids,
+                  CacheView c, const unsigned char* __restrict__ images, const PageMeta* __restrict__ meta,
+                  const unsigned char* __restrict__ q_images, const float2* __restrict__ row_meta,
+                  float* __restrict__ pool, float scale_log2, int group, int* __restrict__ status) {
+    using namespace rt;
+    using pf::fence_after_sync;
+    using pf::fence_before_sync;
+    using pf::mma_commit;
+    using pf::smem_desc;
+    using pf::tmem_ld32;
+    using pf::tmem_wait_ld;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    unsigned char* k_s = smem;
+    unsigned char* q_s = k_s + kKBytes;                       // [2] query images
+    float2* rm_s = reinterpret_cast<float2*>(smem + kAcctSmemData);   // [2][128]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kAcctSmemData + 2 * kBM * 8);
+    uint64_t* k_full = bars + 0;
+    uint64_t* q_full = bars + 1;     // [2]
+    uint64_t* q_empty = bars + 3;    // [2]: one commit + 256 readers of the row factors
+    uint64_t* s_full = bars + 5;     // [2]
+    uint64_t* s_empty = bars + 7;    // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    float* xchg = reinterpret_cast<float*>(bars + 16);        // [128]
+
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const TcKeyTile kt = tiles[blockIdx.x];
+    const TcReq& r = reqs[kt.req];
+    const int D = c.head_dim, nb = blocks_of(D);
+    const int k_steps = (D + 15) / 16;
+    const int np = min(2, r.n_pages - 2 * kt.tile);
+    const int n_q = r.n_qt - kt.qt_begin;
+    const long long img0 = r.img0 + (long long)(2 * kt.tile) * c.num_kv_heads + kt.head;
+    const long long qid0 = r.qimg0 + (long long)kt.head * r.n_qt + kt.qt_begin;
+    if (tid == 0) {
+        mbar_init(k_full, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], 257);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&s_empty[s], 256);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(256u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const size_t img_bytes = page_image_bytes(D);
+            mbar_arrive_expect_tx(k_full, uint32_t(np * 2 * nb) * kSub);
+            for (int p = 0; p < np; ++p)
+                for (int b = 0; b < 2 * nb; ++b)
+                    bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
+                             images + (size_t(img0) + size_t(p) * c.num_kv_heads) * img_bytes + size_t(b) * kSub, kSub, k_full);
+            bool ok = true;
+            for (int j = 0; j < n_q && ok; ++j) {
+                const int s = j & 1;
+                if (j >= 2 && !mbar_spin_bounded(&q_empty[s], uint32_t(((j >> 1) - 1) & 1))) { ok = false; break; }
+                const uint32_t bytes = uint32_t(q_image_bytes(D));
+                mbar_arrive_expect_tx(&q_full[s], bytes + kBM * 8);
+                bulk_g2s(q_s + size_t(s) * kQBytes, q_images + size_t(qid0 + j) * bytes, bytes, &q_full[s]);
+                bulk_g2s(rm_s + s * kBM, row_meta + size_t(qid0 + j) * kBM, kBM * 8, &q_full[s]);
+                if (*abort_flag) break;
+            }
+            if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = make_idesc16(kBM, kBM, 0);
+            const uint64_t kd = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t qd0 = smem_desc(smem_u32(q_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t lo_rows = uint64_t(nb) * kRowsSub >> 4;
+            bool ok = mbar_spin_bounded(k_full, 0);
+            for (int j = 0; j < n_q && ok; ++j) {
+                const int s = j & 1;
+                if (!mbar_spin_bounded(&q_full[s], uint32_t((j >> 1) & 1))) { ok = false; break; }
+                if (j >= 2 && !mbar_spin_bounded(&s_empty[s], uint32_t(((j >> 1) - 1) & 1))) { ok = false; break; }
+                fence_after_sync();
+                const uint64_t qd = qd0 + uint64_t(s) * (kQBytes >> 4);
+                const uint32_t d = tmem + s * 128;
+#pragma unroll
+                for (int term = 0; term < 3; ++term) {
+                    const uint64_t a0 = kd + (term == 0 ? lo_rows : 0), b0 = qd + (term == 1 ? lo_rows : 0);
+                    for (int ks = 0; ks < k_steps; ++ks) {
+                        const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
+                        mma16_ss(d, a0 + o, b0 + o, idesc, (term > 0 || ks > 0) ? 1u : 0u);
+                    }
+                }
+                mma_commit(&q_empty[s]);
+                mma_commit(&s_full[s]);
+            }
+            if (!ok) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+        }
+    } else {
+        const int wg = (warp - 2) >> 2;
+        const int quarter = warp & 3;
+        const int rr = quarter * 32 + lane;
+        const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+        const int key = kt.tile * 128 + rr;
+        const bool in = key < r.kv_len;
+        const int* pages = page_ids + r.page_off;
+        const PageMeta pm = meta[img0 + (rr >= kPage && np > 1 ? c.num_kv_heads : 0)];
+        const bool bad = in && ((pm.bad_k >> (rr & 63)) & 1);
+        // packed rows from `first_row` on see the position
+        const int first_row = r.causal ? max(0, (key - (r.kv_len - r.rows)) * group) : 0;
+        float sum = 0.f;
+        bool dead = false;
+        for (int j = 0; j < n_q; ++j) {
+            const int s = j & 1;
+            if (!warp_spin_bounded(&s_full[s], uint32_t((j >> 1) & 1), lane)) { dead = true; break; }
+            fence_after_sync();
+            const int row0 = (kt.qt_begin + j) * kBM + wg * 64;
+            const float2* rm = rm_s + s * kBM + wg * 64;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                uint32_t x[32];
+                tmem_ld32(tmem + lane_base + s * 128 + wg * 64 + hf * 32, x);
+                tmem_wait_ld();
+                if (bad) {
+#pragma unroll 1
+                    for (int i = 0; i < 32; ++i) {
+                        const int p = row0 + hf * 32 + i;
+                        if (p < first_row || p >= r.rows * group) continue;
+                        float dot = 0.f;
+                        for (int d = 0; d < D; ++d)
+                            dot = fmaf(r.q[size_t(kt.head * group + p % group) * r.q_hs + size_t(p / group) * r.q_ts + d],
+                                       cache_elem(c, pages, r.layer, kt.head, key, d, false), dot);
+                        sum += pf::ex2(dot * scale_log2 - rm[hf * 32 + i].y);
+                    }
+                } else {
+                    const int from = first_row - (row0 + hf * 32);   // columns before this one do not count
+                    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
+                        const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * pm.fk, f.x, -f.y));
+                        const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * pm.fk, f.z, -f.w));
+                        s0 += i >= from ? a : 0.f;
+                        s1 += i + 1 >= from ? b : 0.f;
+                    }
+                    sum += s0 + s1;
+                }
+            }
+            fence_before_sync();
+            mbar_arrive(&q_empty[s]);
+            mbar_arrive(&s_empty[s]);
+        }
+        if (dead) { if (lane == 0) { report_status(status, kDevWaitFull); *abort_flag = 1; } }
+        if (wg == 1) xchg[rr] = sum;
+        named_bar_sync(1, 256);
+        if (wg == 0 && in && !dead) account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum + xchg[rr]);
+    }
+
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+    }
+}
+
+}  // namespace xn
