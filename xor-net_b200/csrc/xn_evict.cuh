@@ -26,9 +26,10 @@ struct EvictDev {
 
 namespace ev {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRun = 32;        // candidates a thread can hold
 
 // Floats in the order of unsigned integers; NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -45,45 +46,62 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t peer_ld(const void* smem, uint32_t rank) {
-    uint32_t a, v;
+__device__ __forceinline__ uint32_t peer_addr(const void* smem, uint32_t rank) {
+    uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(smem)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return a;
+}
+__device__ __forceinline__ uint32_t peer_ld(const void* smem, uint32_t rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(smem, rank)) : "memory");
     return v;
 }
 
-// Sum over the block; every thread gets it.
-__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t* scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Exclusive prefix of v over the block in thread order, and the block's total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* scratch, uint32_t& total) {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) scratch[w] = v;
-    __syncthreads();
-    uint32_t t = lane < kThreads / 32 ? scratch[lane] : 0u;
+    uint32_t inc = v;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+    }
+    if (lane == 31) scratch[w] = inc;
     __syncthreads();
-    return t;
+    const uint32_t mine = scratch[lane];   // 32 warps
+    uint32_t winc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, winc, o);
+        if (lane >= o) winc += up;
+    }
+    total = __shfl_sync(0xffffffffu, winc, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, winc - mine, w);
+    __syncthreads();
+    return before + inc - v;
 }
 
 }  // namespace ev
 
-// One cluster of 1, 2, 4 or 8 blocks per (layer, KV head); block r of it owns a contiguous slice of
-// the candidates and keeps their keys in shared memory when they fit (`slice_cap` of them), so the
-// account is read from memory once.  Radix selection: the threshold key is found 11, 11 and 10 bits
-// at a time from histograms that the blocks add up through each other's shared memory; then every
-// block counts what it keeps, learns from its peers where its positions start, and writes them in
-// order.  Bound by the latency of its passes (a few microseconds each), not by bandwidth.
-__global__ void __launch_bounds__(ev::kThreads)
+// One cluster of 1, 2, 4 or 8 blocks per (layer, KV head).  Thread t of block r owns the RUN
+// candidates from (r * 1024 + t) * RUN on, a quarter of a page or so, and keeps their keys in
+// registers (RUN > 0): the account is read from memory once, 16 bytes per load, and thread order is
+// position order.  Radix selection: the threshold key is found 11, 11 and 10 bits at a time from
+// shared-memory histograms that the blocks read from one another; then one scan of the (above,
+// equal) counts gives every thread the place of its first kept position, ties included, and it
+// writes its run.  Bound by the latency of these steps, about 2 microseconds each, not by bandwidth:
+// [8 heads x 131072 positions: 12 us against 93 us for a loop over the slice in shared memory with a
+// ballot and four barriers per 512 positions.]
+// RUN = 0: streams too long for that; the keys are read again in every pass.
+template <int RUN>
+__global__ void __launch_bounds__(ev::kThreads, 1)
 evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __restrict__ page_ids,
                     const float* __restrict__ pool, long long pool_pages, int num_kv_heads, int cluster,
-                    int slice_cap, const int* __restrict__ acc_len) {
+                    const int* __restrict__ acc_len) {
     using namespace ev;
     pdl_launch_dependents();
-    extern __shared__ uint32_t keys_s[];            // [slice_cap]
-    __shared__ uint32_t hist[kBins];
-    __shared__ uint32_t total[kBins];
-    __shared__ uint32_t scratch[kThreads / 32];
+    __shared__ uint32_t hist[2][kBins];             // by pass parity: peers may still read the other one
+    __shared__ uint32_t scratch[32];
     __shared__ uint32_t counts[2];                  // this block's candidates above / at the threshold
     __shared__ uint32_t found[2];
     const int row = int(blockIdx.x) / cluster;
@@ -93,11 +111,13 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
     const EvictDev r = reqs[rq];
     const int local = row - r.head0;
     const int l = r.layer0 + local / num_kv_heads, h = local % num_kv_heads;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
     const int n_cand = r.len - r.recent;
     const int m = r.keep - r.recent;                // candidates to keep, 0 <= m <= n_cand
-    const int per = (n_cand + cluster - 1) / cluster;
-    const int lo = min(n_cand, int(rank) * per), hi = min(n_cand, lo + per);
+    // positions [lo, hi) are this thread's; without RUN a run that covers the stream
+    const int run = RUN > 0 ? RUN : (((n_cand + cluster * kThreads - 1) / (cluster * kThreads)) + 3) / 4 * 4;
+    const long long lo_ll = (long long)(int(rank) * kThreads + tid) * run;
+    const int lo = int(lo_ll < n_cand ? lo_ll : n_cand), hi = min(n_cand, lo + run);
     const int* pages = page_ids + r.page_off;
     const int valid = acc_len[row];                 // positions behind it have an account of zero
     const size_t base = (size_t(l) * size_t(pool_pages)) * num_kv_heads * kPageTokens + size_t(h) * kPageTokens;
@@ -105,75 +125,95 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
     auto load = [&](int j) -> float {
         return j < valid ? pool[base + size_t(pages[j / kPageTokens]) * pstep + size_t(j % kPageTokens)] : 0.f;
     };
-    const bool fits = hi - lo <= slice_cap;
+    // four positions from a multiple of four on: they never leave a page
+    auto load4 = [&](int j) -> float4 {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < valid && j < n_cand) {
+            x = *reinterpret_cast<const float4*>(pool + base + size_t(pages[j / kPageTokens]) * pstep + size_t(j % kPageTokens));
+            if (j + 1 >= valid) x.y = 0.f;
+            if (j + 2 >= valid) x.z = 0.f;
+            if (j + 3 >= valid) x.w = 0.f;
+        }
+        return x;
+    };
+    constexpr int R = RUN > 0 ? RUN : 4;
+    uint32_t keys[R];
     pdl_wait();
-    if (fits) {
-#pragma unroll 4
-        for (int j = lo + tid; j < hi; j += kThreads) keys_s[j - lo] = order_key(load(j));
-        __syncthreads();
+    if (RUN > 0) {
+        float4 x[R / 4];
+#pragma unroll
+        for (int i = 0; i < R / 4; ++i) x[i] = load4(lo + 4 * i);
+#pragma unroll
+        for (int i = 0; i < R / 4; ++i) {
+            keys[4 * i] = order_key(x[i].x);
+            keys[4 * i + 1] = order_key(x[i].y);
+            keys[4 * i + 2] = order_key(x[i].z);
+            keys[4 * i + 3] = order_key(x[i].w);
+        }
     }
-    auto key_at = [&](int j) -> uint32_t { return fits ? keys_s[j - lo] : order_key(load(j)); };
+    // f(j, key) for every candidate of the thread in order, all lanes of a warp together
+    auto each = [&](auto&& f) {
+        if (RUN > 0) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) f(lo + i, keys[i], lo + i < hi);
+        } else {
+            for (int i = 0; i < run; ++i) {
+                const int j = lo + i;
+                const bool in = j < hi;
+                f(j, in ? order_key(load(j)) : 0u, in);
+            }
+        }
+    };
 
     uint32_t prefix = 0, mask = 0, left = uint32_t(m);   // the threshold is the left-th largest with this prefix
-    if (m > 0 && m < n_cand) {
+    const bool all = m == n_cand, none = m == 0;
+    if (!all && !none) {
         for (int pass = 0; pass < 3; ++pass) {
             const int bits = pass < 2 ? 11 : 10;
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
             const uint32_t bins = 1u << bits;
-            for (int b = tid; b < kBins; b += kThreads) hist[b] = 0;
+            uint32_t* hs = hist[pass & 1];
+            hs[tid] = 0;
+            hs[tid + kThreads] = 0;
             __syncthreads();
-            for (int j0 = lo; j0 < hi; j0 += kThreads) {   // whole warps: lanes past the end vote nothing
-                const int j = j0 + tid;
-                uint32_t k = j < hi ? key_at(j) : 0u;
-                const bool in = j < hi && (k & mask) == prefix;
+            each([&](int, uint32_t k, bool in_run) {
+                const bool in = in_run && (k & mask) == prefix;
                 const uint32_t bin = (k >> shift) & (bins - 1);
-                // equal accounts are common (positions never looked at): one atomic per warp and bin
+                // equal accounts are common (positions never looked at): a warp that agrees adds once
                 const uint32_t act = __ballot_sync(0xffffffffu, in);
-                if (in) {
-                    const uint32_t same = __match_any_sync(act, bin);
-                    if (lane == __ffs(same) - 1) atomicAdd(&hist[bin], uint32_t(__popc(same)));
+                if (act == 0) return;
+                const int lead = __ffs(act) - 1;
+                const uint32_t b0 = __shfl_sync(0xffffffffu, bin, lead);
+                if (__all_sync(0xffffffffu, !in || bin == b0)) {
+                    if (lane == lead) atomicAdd(&hs[b0], uint32_t(__popc(act)));
+                } else if (in) {
+                    atomicAdd(&hs[bin], 1u);
                 }
-            }
-            __syncthreads();
+            });
+            // the bin, counted from the top, that holds the left-th largest: a thread sums two bins (one
+            // in the last pass) over the cluster, the highest on the lowest threads
+            const int per = int(bins) / kThreads;
+            const int top = int(bins) - 1 - tid * per;
+            uint32_t a = 0, b = 0;
             if (cluster > 1) {
                 cluster_sync_all();
-                for (int b = tid; b < int(bins); b += kThreads) {
-                    uint32_t t = 0;
-                    for (int p = 0; p < cluster; ++p) t += peer_ld(&hist[b], uint32_t(p));
-                    total[b] = t;
-                }
-                cluster_sync_all();
-            } else {
-                for (int b = tid; b < int(bins); b += kThreads) total[b] = hist[b];
-            }
-            __syncthreads();
-            // the bin, counted from the top, that holds the left-th largest: thread t sums a run of
-            // bins (the highest runs on the lowest threads), an exclusive scan places the runs
-            const int run = int(bins) / kThreads;   // 4 or 2
-            uint32_t mine = 0;
-            const int top = int(bins) - 1 - tid * run;
-            for (int i = 0; i < run; ++i) mine += total[top - i];
-            uint32_t inc = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += up;
-            }
-            if (lane == 31) scratch[warp] = inc;
-            __syncthreads();
-            uint32_t before = inc - mine;
-            for (int w = 0; w < warp; ++w) before += scratch[w];
-            if (before < left && left <= before + mine) {   // exactly one thread
-                uint32_t cum = before;
-                for (int i = 0; i < run; ++i) {
-                    const uint32_t t = total[top - i];
-                    if (cum + t >= left) {
-                        found[0] = uint32_t(top - i);
-                        found[1] = left - cum;
-                        break;
+                for (int p = 0; p < kMaxCluster; ++p)
+                    if (p < cluster) {
+                        a += peer_ld(&hs[top], uint32_t(p));
+                        if (per == 2) b += peer_ld(&hs[top - 1], uint32_t(p));
                     }
-                    cum += t;
-                }
+            } else {
+                __syncthreads();
+                a = hs[top];
+                if (per == 2) b = hs[top - 1];
+            }
+            uint32_t total;
+            const uint32_t before = block_scan(a + b, scratch, total);
+            if (before < left && left <= before + a + b) {   // exactly one thread
+                const bool first = left <= before + a;
+                found[0] = uint32_t(first ? top : top - 1);
+                found[1] = left - before - (first ? 0u : a);
             }
             __syncthreads();
             prefix |= found[0] << shift;
@@ -183,32 +223,29 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
         }
     }
     // m == 0 keeps no candidate, m == n_cand keeps all
-    const bool all = m == n_cand, none = m == 0;
     uint32_t gt = 0, eq = 0;
-    if (!all && !none)
-        for (int j = lo + tid; j < hi; j += kThreads) {
-            const uint32_t k = key_at(j);
-            gt += k > prefix;
-            eq += k == prefix;
-        }
-    gt = block_sum(gt, scratch);
-    eq = block_sum(eq, scratch);
-    if (tid == 0) {
-        counts[0] = all ? uint32_t(hi - lo) : gt;
-        counts[1] = eq;
-    }
-    __syncthreads();
-    uint32_t pos = 0, eq_before = 0;
+    if (all) gt = uint32_t(hi - lo);
+    else if (!none)
+        each([&](int, uint32_t k, bool in) {
+            gt += in && k > prefix;
+            eq += in && k == prefix;
+        });
+    uint32_t gt_all, eq_all;
+    const uint32_t gt_at = block_scan(gt, scratch, gt_all);
+    const uint32_t eq_at = block_scan(eq, scratch, eq_all);
+    uint32_t gt_before = 0, eq_before = 0;
     if (cluster > 1) {
+        if (tid == 0) {
+            counts[0] = gt_all;
+            counts[1] = eq_all;
+        }
+        __syncthreads();
         cluster_sync_all();
         for (uint32_t p = 0; p < rank; ++p) {
-            const uint32_t pe = peer_ld(&counts[1], p);
-            // of the equal ones the first `left` stay
-            const uint32_t pe_kept = (all || none) ? 0u : min(pe, left > eq_before ? left - eq_before : 0u);
-            pos += peer_ld(&counts[0], p) + pe_kept;
-            eq_before += pe;
+            gt_before += peer_ld(&counts[0], p);
+            eq_before += peer_ld(&counts[1], p);
         }
-        cluster_sync_all();   // no block leaves while another still reads its counts
+        cluster_sync_all();   // no block leaves while another still reads its counts (or histograms)
     }
     int* kept = r.kept_ws + size_t(local) * r.keep;
     int* kept_user = r.kept ? r.kept + size_t(local) * r.keep : nullptr;
@@ -218,38 +255,16 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
         if (kept_user) kept_user[at] = j;
         if (w_user) w_user[at] = load(j);
     };
-    if (!none)
-        for (int j0 = lo; j0 < hi; j0 += kThreads) {
-            const int j = j0 + tid;
-            const bool in = j < hi;
-            const uint32_t k = in && !all ? key_at(j) : 0u;
-            const bool is_eq = in && !all && k == prefix;
-            // the equal ones' ranks, then the kept ones' places, both in position order
-            const uint32_t eq_vote = __ballot_sync(0xffffffffu, is_eq);
-            if (lane == 0) scratch[warp] = uint32_t(__popc(eq_vote));
-            __syncthreads();
-            uint32_t er = eq_before + uint32_t(__popc(eq_vote & ((1u << lane) - 1)));
-            uint32_t eq_all = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) er += scratch[w];
-                eq_all += scratch[w];
-            }
-            const bool keep_it = in && (all || k > prefix || (is_eq && er < left));
-            const uint32_t vote = __ballot_sync(0xffffffffu, keep_it);
-            __syncthreads();
-            if (lane == 0) scratch[warp] = uint32_t(__popc(vote));
-            __syncthreads();
-            uint32_t at = pos + uint32_t(__popc(vote & ((1u << lane) - 1)));
-            uint32_t kept_all = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) at += scratch[w];
-                kept_all += scratch[w];
-            }
-            if (keep_it) emit(at, j);
-            pos += kept_all;
-            eq_before += eq_all;
-            __syncthreads();
-        }
+    if (!none) {
+        // of the equal ones the first `left` (in position order over the whole row) stay
+        uint32_t er = eq_before + eq_at;
+        uint32_t at = gt_before + gt_at + min(er, left);
+        each([&](int j, uint32_t k, bool in) {
+            const bool is_eq = !all && in && k == prefix;
+            if (in && (all || k > prefix || (is_eq && er < left))) emit(at++, j);
+            er += is_eq;
+        });
+    }
     // the last `recent` positions, shared out over the cluster
     for (int i = int(rank) * kThreads + tid; i < r.recent; i += cluster * kThreads) emit(uint32_t(m + i), n_cand + i);
 }

@@ -294,7 +294,6 @@ int32_t ready_read_kernels(xn_ctx* c) {
     }
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(account_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kAcctSmemBytes));
-    XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 200 << 10));
     c->read_funcs_ready = true;
     return XN_OK;
 }
@@ -548,10 +547,14 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     if (!merges.empty())
         XN_CUDA(c, launch_pdl(c, read_merge_kernel, dim3(unsigned(merges.size()), rt::kBM / 8), 256, 0, true, 0, reqs_d,
                               reinterpret_cast<const TcMerge*>(slot->dev + o_merge), parts, row_meta, G, D, c->nv, want ? 1 : 0));
+    // a cluster of blocks per key tile while that still adds SMs and leaves each block two row tiles
+    int cluster = 1, most_qt = 0;
+    for (const TcReq& r : reqs) most_qt = std::max(most_qt, r.n_qt);
+    while (cluster < ev::kMaxCluster && (long long)key_tiles.size() * cluster < 2 * c->sm_count && most_qt >= 4 * cluster) cluster *= 2;
     if (want)
-        XN_CUDA(c, launch_pdl(c, account_tc_kernel, dim3(unsigned(key_tiles.size())), rt::kThreads, size_t(rt::kAcctSmemBytes), true,
-                              0, reqs_d, reinterpret_cast<const TcKeyTile*>(slot->dev + o_key), pages_d, view, img, meta, qimg,
-                              row_meta, c->acct_pool, scale_log2, G, c->status_d));
+        XN_CUDA(c, launch_pdl(c, account_tc_kernel, dim3(unsigned(key_tiles.size() * cluster)), rt::kThreads,
+                              size_t(rt::kAcctSmemBytes), true, unsigned(cluster), reqs_d, reinterpret_cast<const TcKeyTile*>(slot->dev + o_key), pages_d, view, img, meta, qimg,
+                              row_meta, c->acct_pool, scale_log2, G, cluster, c->status_d));
     if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
     c->stats.prefill_launches += 1;
     return finish_slot(c, slot);
@@ -884,13 +887,15 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
     const EvictDev* ev_d = reinterpret_cast<const EvictDev*>(slot->dev + o_ev);
     const int* pages_d = reinterpret_cast<const int*>(slot->dev + o_page);
     const int* acc_d = reinterpret_cast<const int*>(slot->dev + o_acc);
-    // blocks per (layer, head): slices of about 8192 candidates, so that the passes over a long
-    // stream run on several SMs; a slice's keys stay in shared memory up to 40960 of them
-    int cluster = 1;
-    while (cluster < ev::kMaxCluster && longest > cluster * 8192) cluster *= 2;
-    const int slice_cap = std::min((longest + cluster - 1) / cluster, 40960);
-    XN_CUDA(c, launch_pdl(c, evict_select_kernel, dim3(unsigned(head0 * cluster)), ev::kThreads, size_t(slice_cap) * 4, true,
-                          unsigned(cluster), ev_d, int(ev.size()), pages_d, c->acct_pool, c->pool_pages, Hkv, cluster, slice_cap, acc_d));
+    // blocks per (layer, head): 4096 candidates each (a run of 4 per thread) up to 8 blocks, longer
+    // runs beyond that
+    int cluster = 1, run = 4;
+    while (cluster < ev::kMaxCluster && longest > cluster * ev::kThreads * run) cluster *= 2;
+    while (run <= ev::kMaxRun && longest > cluster * ev::kThreads * run) run *= 2;
+    auto select = run == 4 ? evict_select_kernel<4> : run == 8 ? evict_select_kernel<8> : run == 16 ? evict_select_kernel<16>
+                : run == 32 ? evict_select_kernel<32> : evict_select_kernel<0>;
+    XN_CUDA(c, launch_pdl(c, select, dim3(unsigned(head0 * cluster)), ev::kThreads, 0, true, unsigned(cluster), ev_d,
+                          int(ev.size()), pages_d, c->acct_pool, c->pool_pages, Hkv, cluster, acc_d));
     const EvictPools pools = {c->k_pool, c->v_pool, c->pool8, c->acct_pool, c->pool_pages, Hkv, D, c->nv, c->dq};
     if (any_copy)
         XN_CUDA(c, launch_pdl(c, evict_copy_kernel<4>, dim3(unsigned(head0), unsigned(std::min<int64_t>((keep_most + 31) / 32, 65535))),

@@ -23,6 +23,7 @@
 #include <cuda_fp16.h>
 
 #include "xn_common.cuh"
+#include "xn_evict.cuh"
 #include "xn_prefill_tf32.cuh"
 #include "xn_read.cuh"
 
@@ -66,8 +67,9 @@ struct TcKeyTile {
 // rows that hold an infinity or a NaN (their images are zero; they are added exactly on the side).
 struct __align__(16) PageMeta {
     float fk, fv;
+    unsigned bad;      // bit 0: bad_k is not empty, bit 1: bad_v
+    unsigned pad;
     unsigned long long bad_k, bad_v;
-    unsigned long long pad;
 };
 
 // Where the cache rows are, for the rare exact path and the image kernel.
@@ -133,6 +135,16 @@ __device__ __forceinline__ void scale_of(float m, float& up, float& down) {
     e = m == 0.f ? 0 : max(e, -60);
     up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
     down = __uint_as_float(uint32_t(127 - 13 + e) << 23);
+}
+
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+    return r;
+}
+
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ bool finite4(const float4& x) {
@@ -281,6 +293,7 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
                 pm.bad_k |= (unsigned long long)(s_bad[0][w]) << (8 * w);
                 pm.bad_v |= (unsigned long long)(s_bad[1][w]) << (8 * w);
             }
+            pm.bad = (pm.bad_k ? 1u : 0u) | (pm.bad_v ? 2u : 0u);
             meta[id] = pm;
         }
         unsigned char* img = images + size_t(id) * page_image_bytes(D);
@@ -573,25 +586,24 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             const bool two = 2 * j + 1 < n_pages;
             const bool have = wg == 0 || two;
             // both pages' factors (uniform over the block)
-            const PageMeta pm0 = pm[size_t(2 * j) * c.num_kv_heads];
-            const PageMeta pm1 = two ? pm[size_t(2 * j + 1) * c.num_kv_heads] : pm0;
-            const PageMeta& own = wg ? pm1 : pm0;
-            const float fv = fmaxf(pm0.fv, pm1.fv);
+            const PageMeta* pm0 = pm + size_t(2 * j) * c.num_kv_heads;
+            const PageMeta* pm1 = two ? pm0 + c.num_kv_heads : pm0;
+            const float fv0 = pm0->fv, fv1 = pm1->fv;
+            const float cm = cq * (wg ? pm1 : pm0)->fk;
+            const unsigned bad = pm0->bad | pm1->bad;
+            const float fv = fmaxf(fv0, fv1);
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
             if (lane == 0 && dead) { sm_dead[sb] = 1; *abort_flag = 1; }
             fence_after_sync();
-            uint32_t x0[32], x1[32];
             const uint32_t s_addr = tmem + kTmemS + lane_base + sb * 128 + col0;
             const int key0 = (it.page_begin + 2 * j + wg) * kPage;
-            const float cm = cq * own.fk;
+            const bool some_masked = key0 + kPage > limit_first;
             float mx = -INFINITY;
             if (!dead && have) {
-                tmem_ld32(s_addr, x0);
-                tmem_ld32(s_addr + 32, x1);
-                tmem_wait_ld();
-                if (own.bad_k) {
-                    // rows of K with an infinity or a NaN: their scores one by one, in f32
-                    unsigned long long b = own.bad_k;
+                if (bad & 1u) {
+                    // rows of K with an infinity or a NaN: their scores one by one, in f32, put where the
+                    // MMA left zeros
+                    unsigned long long b = (wg ? pm1 : pm0)->bad_k;
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
                         b &= b - 1;
@@ -600,23 +612,24 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                             for (int d = 0; d < D; ++d)
                                 dot = fmaf(r.q[size_t(it.head * group + pr % group) * r.q_hs + size_t(t) * r.q_ts + d],
                                            cache_elem(c, pages, r.layer, it.head, key0 + cidx, d, false), dot);
-                        const uint32_t bits = __float_as_uint(dot * scale_log2 / cm);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (i == cidx) x0[i] = bits;
-                            if (i + 32 == cidx) x1[i] = bits;
-                        }
+                        __syncwarp();
+                        tmem_st1(s_addr + cidx, __float_as_uint(dot * scale_log2 / cm));
                     }
                 }
-                if (key0 + kPage > limit_first) {    // some row masks some position here
+                // the scores are read twice, 32 at a time: all 64 beside O's 64 registers would spill
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (key0 + i >= limit) x0[i] = 0xff800000u;
-                        if (key0 + 32 + i >= limit) x1[i] = 0xff800000u;
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t x[32];
+                    tmem_ld32(s_addr + hf * 32, x);
+                    tmem_wait_ld();
+                    if (some_masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (key0 + hf * 32 + i >= limit) x[i] = 0xff800000u;
                     }
-                }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x0[i]), __uint_as_float(x1[i])));
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+                }
                 mx *= cm;
             }
             float* xc = xchg + sb * 256;
@@ -631,42 +644,34 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             m_ref = m_new;
             l_sum *= alpha;
             if (have) {
-                const float pscale = kPScale * (own.fv / fv);   // powers of two: exact
+                const float pscale = kPScale * ((wg ? fv1 : fv0) / fv);   // powers of two: exact
                 float ps0 = 0.f, ps1 = 0.f;
+                uint32_t hi[32], lo[32];
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float a = pf::ex2(fmaf(__uint_as_float(x0[i]), cm, neg_m));
-                    const float b = pf::ex2(fmaf(__uint_as_float(x0[i + 1]), cm, neg_m));
-                    ps0 += a;
-                    ps1 += b;
-                    uint32_t hi, lo;
-                    split2(a * pscale, b * pscale, hi, lo);
-                    x0[i] = hi;
-                    x0[i + 1] = lo;
-                }
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t x[32];
+                    tmem_ld32(s_addr + hf * 32, x);
+                    tmem_wait_ld();
+                    if (some_masked) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float a = pf::ex2(fmaf(__uint_as_float(x1[i]), cm, neg_m));
-                    const float b = pf::ex2(fmaf(__uint_as_float(x1[i + 1]), cm, neg_m));
-                    ps0 += a;
-                    ps1 += b;
-                    uint32_t hi, lo;
-                    split2(a * pscale, b * pscale, hi, lo);
-                    x1[i] = hi;
-                    x1[i + 1] = lo;
+                        for (int i = 0; i < 32; ++i)
+                            if (key0 + hf * 32 + i >= limit) x[i] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float a = pf::ex2(fmaf(__uint_as_float(x[2 * i]), cm, neg_m));
+                        const float b = pf::ex2(fmaf(__uint_as_float(x[2 * i + 1]), cm, neg_m));
+                        ps0 += a;
+                        ps1 += b;
+                        split2(a * pscale, b * pscale, hi[hf * 16 + i], lo[hf * 16 + i]);
+                    }
                 }
                 l_sum += ps0 + ps1;
-                uint32_t w[32];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) { w[i] = x0[2 * i]; w[16 + i] = x1[2 * i]; }
-                tmem_st32(s_addr, w);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) { w[i] = x0[2 * i + 1]; w[16 + i] = x1[2 * i + 1]; }
-                tmem_st32(s_addr + 32, w);
+                tmem_st32(s_addr, hi);
+                tmem_st32(s_addr + 32, lo);
                 tmem_wait_st();
             }
-            const unsigned long long bad0 = pm0.bad_v, bad1 = two ? pm1.bad_v : 0ull;
-            if (bad0 | bad1) {
+            if (bad & 2u) {
                 // rows of V with an infinity or a NaN (uniform over the block): bring O up to date, then
                 // add p * v for the rows that see them; P of both pages is read back from tensor memory
                 if (j > 0) {
@@ -679,33 +684,27 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 wg_barrier();
                 fence_after_sync();
                 for (int p = 0; p < 2; ++p) {
-                    unsigned long long b = p ? bad1 : bad0;
-                    const float unscale = fv / (kPScale * (p ? pm1.fv : pm0.fv));
+                    unsigned long long b = p == 0 ? pm0->bad_v : (two ? pm1->bad_v : 0ull);
+                    const float unscale = fv / (kPScale * (p ? fv1 : fv0));
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
                         b &= b - 1;
-                        uint32_t hi[32], lo[32];
-                        tmem_ld32(tmem + kTmemS + lane_base + sb * 128 + p * 64, hi);
-                        tmem_ld32(tmem + kTmemS + lane_base + sb * 128 + p * 64 + 32, lo);
-                        tmem_wait_ld();
-                        uint32_t hw = 0, lw = 0;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i == cidx / 2) { hw = hi[i]; lw = lo[i]; }
+                        uint32_t hw = tmem_ld1(tmem + kTmemS + lane_base + sb * 128 + p * 64 + cidx / 2);
+                        uint32_t lw = tmem_ld1(tmem + kTmemS + lane_base + sb * 128 + p * 64 + 32 + cidx / 2);
                         const float2 h2 = __half22float2(*reinterpret_cast<__half2*>(&hw));
                         const float2 l2 = __half22float2(*reinterpret_cast<__half2*>(&lw));
                         const float pv = ((cidx & 1) ? h2.y + l2.y : h2.x + l2.x) * unscale;
                         const int key = (it.page_begin + 2 * j + p) * kPage + cidx;
+                        // the row of V through the exchange area of the tile before (nobody reads that now)
+                        float* vrow = xchg + (sb ^ 1) * 256;
+                        const int e = tid - 64;
+                        if (e < 128) vrow[e] = e < D ? cache_elem(c, pages, r.layer, it.head, key, e, true) : 0.f;
+                        wg_barrier();
                         if (key < limit) {   // (a weight of zero times an infinity is a NaN, as in a plain sum)
-#pragma unroll 1
-                            for (int d = 0; d < 64; ++d) {
-                                if (col0 + d >= D) break;
-                                const float add = pv * cache_elem(c, pages, r.layer, it.head, key, col0 + d, true);
 #pragma unroll
-                                for (int i = 0; i < 64; ++i)
-                                    if (i == d) o[i] += add;
-                            }
+                            for (int i = 0; i < 64; ++i) o[i] = fmaf(pv, vrow[col0 + i], o[i]);
                         }
+                        wg_barrier();
                     }
                 }
                 fence_before_sync();
@@ -833,12 +832,13 @@ read_merge_kernel(const TcReq* __restrict__ reqs, const TcMerge* __restrict__ me
 // query rows that sees them, p = 2^(s - lse), summed over the rows in f32.  Positions are the rows of
 // the accumulator, so a thread owns a position and the sum needs no exchange and no atomics (its
 // order is fixed).  Half the MMAs of the attention itself.  Roles as above; the K tile stays, the
-// query images stream through two stages.
+// query images stream through two stages.  With few positions and many rows the row tiles are dealt
+// out to a cluster of blocks, whose first block adds up the sums through the others' shared memory.
 __global__ void __launch_bounds__(rt::kThreads, 1)
 account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ tiles, const int* __restrict__ page_ids,
                   CacheView c, const unsigned char* __restrict__ images, const PageMeta* __restrict__ meta,
                   const unsigned char* __restrict__ q_images, const float2* __restrict__ row_meta,
-                  float* __restrict__ pool, float scale_log2, int group, int* __restrict__ status) {
+                  float* __restrict__ pool, float scale_log2, int group, int cluster, int* __restrict__ status) {
     using namespace rt;
     using pf::fence_after_sync;
     using pf::fence_before_sync;
@@ -863,14 +863,16 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const TcKeyTile kt = tiles[blockIdx.x];
+    const int rank = int(ev::cluster_rank());
+    const TcKeyTile kt = tiles[int(blockIdx.x) / cluster];
     const TcReq& r = reqs[kt.req];
     const int D = c.head_dim, nb = blocks_of(D);
     const int k_steps = (D + 15) / 16;
     const int np = min(2, r.n_pages - 2 * kt.tile);
-    const int n_q = r.n_qt - kt.qt_begin;
+    const int n_all = r.n_qt - kt.qt_begin;
+    const int n_q = n_all > rank ? (n_all - rank - 1) / cluster + 1 : 0;   // row tiles rank, rank + cluster, ...
     const long long img0 = r.img0 + (long long)(2 * kt.tile) * c.num_kv_heads + kt.head;
-    const long long qid0 = r.qimg0 + (long long)kt.head * r.n_qt + kt.qt_begin;
+    const long long qid0 = r.qimg0 + (long long)kt.head * r.n_qt + kt.qt_begin + rank;
     if (tid == 0) {
         mbar_init(k_full, 1);
         for (int s = 0; s < 2; ++s) {
@@ -908,8 +910,8 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
                 if (j >= 2 && !mbar_spin_bounded(&q_empty[s], uint32_t(((j >> 1) - 1) & 1))) { ok = false; break; }
                 const uint32_t bytes = uint32_t(q_image_bytes(D));
                 mbar_arrive_expect_tx(&q_full[s], bytes + kBM * 8);
-                bulk_g2s(q_s + size_t(s) * kQBytes, q_images + size_t(qid0 + j) * bytes, bytes, &q_full[s]);
-                bulk_g2s(rm_s + s * kBM, row_meta + size_t(qid0 + j) * kBM, kBM * 8, &q_full[s]);
+                bulk_g2s(q_s + size_t(s) * kQBytes, q_images + size_t(qid0 + j * cluster) * bytes, bytes, &q_full[s]);
+                bulk_g2s(rm_s + s * kBM, row_meta + size_t(qid0 + j * cluster) * kBM, kBM * 8, &q_full[s]);
                 if (*abort_flag) break;
             }
             if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
@@ -959,7 +961,7 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
             const int s = j & 1;
             if (!warp_spin_bounded(&s_full[s], uint32_t((j >> 1) & 1), lane)) { dead = true; break; }
             fence_after_sync();
-            const int row0 = (kt.qt_begin + j) * kBM + wg * 64;
+            const int row0 = (kt.qt_begin + rank + j * cluster) * kBM + wg * 64;
             const float2* rm = rm_s + s * kBM + wg * 64;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
@@ -995,17 +997,32 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
             mbar_arrive(&q_empty[s]);
             mbar_arrive(&s_empty[s]);
         }
-        if (dead) { if (lane == 0) { report_status(status, kDevWaitFull); *abort_flag = 1; } }
+        if (dead && lane == 0) { report_status(status, kDevWaitFull); *abort_flag = 1; }
         if (wg == 1) xchg[rr] = sum;
         named_bar_sync(1, 256);
-        if (wg == 0 && in && !dead) account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum + xchg[rr]);
+        if (wg == 0) xchg[rr] += sum;
     }
+    __syncwarp();
 
     fence_before_sync();
     __syncthreads();
     if (warp == 1) {
         fence_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+    }
+    if (cluster > 1) {
+        __syncwarp();
+        ev::cluster_sync_all();
+    }
+    const int key = kt.tile * kBM + tid;
+    if (rank == 0 && tid < kBM && key < r.kv_len) {
+        float sum = xchg[tid];
+        for (int p = 1; p < cluster; ++p) sum += __uint_as_float(ev::peer_ld(&xchg[tid], uint32_t(p)));
+        account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum);
+    }
+    if (cluster > 1) {
+        __syncwarp();
+        ev::cluster_sync_all();   // no block leaves while its sums are read
     }
 }
 
