@@ -93,11 +93,14 @@ constexpr int kVStages = 3;
 constexpr int kQBytes = 4 * kRowsSub;    // 64 KB: hi and lo, two column blocks
 constexpr int kKBytes = 4 * kRowsSub;
 constexpr int kVBytes = 4 * kSub;        // 32 KB
-constexpr int kSmemData = kQBytes + kKBytes + kVStages * kVBytes;
+constexpr int kKStages = 2;
+constexpr int kSmemData = kKStages * kKBytes + kVStages * kVBytes;
+static_assert(kQBytes <= 2 * kVBytes, "the query images pass through V stages 1 and 2");
 constexpr int kSmemBytes = kSmemData + 3072;   // 227 KB, all there is: the block's window starts 1024-byte aligned
 static_assert(kSmemBytes <= 232448, "shared memory of a block");
-constexpr int kTmemS = 0;                // 2 x 128 columns
-constexpr int kTmemO = 256;              // 2 x 128 columns
+constexpr int kTmemQ = 0;                // hi 64 columns, lo 64 columns (two halves each)
+constexpr int kTmemS = 128;              // 2 x 128 columns
+constexpr int kTmemO = 384;              // 128 columns
 
 constexpr int kAcctQStages = 2;
 constexpr int kAcctSmemData = kKBytes + kAcctQStages * kQBytes;
@@ -354,8 +357,10 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
     }
 }
 
-// Pass 2.  Shared memory: Q images 64 KB | K tile (two pages) 64 KB | three V pages of 32 KB.  Tensor
-// memory: two S / P buffers and two O tiles of 128 columns.  Roles (320 threads): warp 0 copies
+// Pass 2.  Shared memory: two K tiles (two pages each) of 64 KB | three V pages of 32 KB.  Tensor
+// memory: Q hi and lo (128 columns), two S / P buffers and one O tile of 128 columns each.  (Q in
+// shared memory left room for one K tile only, whose reload then sat between two tiles' MMAs:
+// 4.3 us a tile.)  Roles (320 threads): warp 0 copies
 // images (1-D bulk copies), warp 1 issues the MMAs -- the S of tile j + 1 before the O of tile j, so
 // that the softmax of a tile runs beside them -- and warps 2..9 are two softmax warpgroups: thread
 // r of each owns packed row r; warpgroup w takes page w of every tile and columns [64 w, 64 w + 64)
@@ -381,20 +386,21 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         if (threadIdx.x == 0) report_status(status, kDevBadIndex);
         return;
     }
-    unsigned char* q_s = smem;
-    unsigned char* k_s = q_s + kQBytes;
-    unsigned char* v_s = k_s + kKBytes;
+    unsigned char* k_s = smem;
+    unsigned char* v_s = k_s + kKStages * kKBytes;
+    unsigned char* q_s = v_s + kVBytes;        // until the query rows are in tensor memory
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemData);
     uint64_t* q_full = bars + 0;
-    uint64_t* k_full = bars + 1;
-    uint64_t* k_empty = bars + 2;
-    uint64_t* v_full = bars + 3;               // [3]
+    uint64_t* q_ready = bars + 1;
+    uint64_t* k_full = bars + 2;               // [2]
+    uint64_t* k_empty = k_full + kKStages;     // [2]
+    uint64_t* v_full = k_empty + kKStages;     // [3]
     uint64_t* v_empty = v_full + kVStages;     // [3]
     uint64_t* s_full = v_empty + kVStages;     // [2]
     uint64_t* p_full = s_full + 2;             // [2]
-    uint64_t* o_full = p_full + 2;             // [2]
-    uint64_t* o_empty = o_full + 2;            // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+    uint64_t* o_full = p_full + 2;
+    uint64_t* o_empty = o_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
     // by tile parity: a fast warp of the next tile must not be seen by a slow one of this tile
     volatile int* sm_dead = abort_flag + 1;              // [2]
@@ -414,8 +420,13 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
 
     if (tid == 0) {
         mbar_init(q_full, 1);
-        mbar_init(k_full, 1);
-        mbar_init(k_empty, 1);
+        mbar_init(q_ready, 256);
+        mbar_init(o_full, 1);
+        mbar_init(o_empty, 256);
+        for (int s = 0; s < kKStages; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+        }
         for (int s = 0; s < kVStages; ++s) {
             mbar_init(&v_full[s], 1);
             mbar_init(&v_empty[s], 1);
@@ -423,8 +434,6 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 256);
-            mbar_init(&o_full[s], 1);
-            mbar_init(&o_empty[s], 256);
         }
         *abort_flag = 0;
         sm_dead[0] = sm_dead[1] = 0;
@@ -451,17 +460,19 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             mbar_arrive_expect_tx(q_full, uint32_t(q_image_bytes(D)));
             bulk_g2s(q_s, q_images + size_t(qid) * q_image_bytes(D), uint32_t(q_image_bytes(D)), q_full);
             auto load_k = [&](int j) -> bool {
-                if (j > 0 && !mbar_spin_bounded(k_empty, uint32_t((j - 1) & 1))) return false;
+                const int st = j & 1;
+                if (j >= kKStages && !mbar_spin_bounded(&k_empty[st], uint32_t(((j >> 1) - 1) & 1))) return false;
                 const int np = min(2, n_pages - 2 * j);
-                mbar_arrive_expect_tx(k_full, uint32_t(np * 2 * nb) * kSub);
+                mbar_arrive_expect_tx(&k_full[st], uint32_t(np * 2 * nb) * kSub);
                 for (int p = 0; p < np; ++p)
                     for (int b = 0; b < 2 * nb; ++b)   // hi blocks, then lo blocks
-                        bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
-                                 base + size_t(2 * j + p) * step + size_t(b) * kSub, kSub, k_full);
+                        bulk_g2s(k_s + size_t(st) * kKBytes + size_t(b) * kRowsSub + size_t(p) * kSub,
+                                 base + size_t(2 * j + p) * step + size_t(b) * kSub, kSub, &k_full[st]);
                 return true;
             };
             auto load_v = [&](int pg) -> bool {
                 const int st = pg % kVStages;
+                if (pg == 1 && !mbar_spin_bounded(q_ready, 0)) return false;   // the query images sat there
                 if (pg >= kVStages && !mbar_spin_bounded(&v_empty[st], uint32_t((pg / kVStages - 1) & 1))) return false;
                 const uint32_t bytes = uint32_t(2 * nb) * kSub;
                 mbar_arrive_expect_tx(&v_full[st], bytes);
@@ -481,36 +492,42 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         if (lane == 0) {
             const uint32_t id_qk = make_idesc16(kBM, kBM, 0);
             const uint32_t id_pv = make_idesc16(kBM, n_pv, 1);
-            const uint64_t qd = smem_desc(smem_u32(q_s), 0, 1024, pf::kLayoutSw128);
-            const uint64_t kd = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t kd0 = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
             const uint64_t vd0 = smem_desc(smem_u32(v_s), kSub, 1024, pf::kLayoutSw128);
             const uint64_t lo_rows = uint64_t(nb) * kRowsSub >> 4;   // hi image -> lo image, 128 rows
             const uint64_t lo_page = uint64_t(nb) * kSub >> 4;       // ... of a page
-            bool ok = mbar_spin_bounded(q_full, 0);
+            bool ok = mbar_spin_bounded(q_ready, 0);
             if (!ok) { report_status(status, kDevWaitFull); *abort_flag = 1; }
             int v_st = 0, v_ph = 0;
             auto issue_qk = [&](int j) -> bool {
-                if (!mbar_spin_bounded(k_full, uint32_t(j & 1))) return false;
+                if (!mbar_spin_bounded(&k_full[j & 1], uint32_t((j >> 1) & 1))) return false;
                 fence_after_sync();
                 const uint32_t d = tmem + kTmemS + (j & 1) * 128;
+                const uint64_t kd = kd0 + uint64_t(j & 1) * (kKBytes >> 4);
                 // the small products first: they meet a small accumulator
+                auto terms = [&](int steps) {
 #pragma unroll
-                for (int term = 0; term < 3; ++term) {
-                    const uint64_t a0 = qd + (term == 0 ? lo_rows : 0), b0 = kd + (term == 1 ? lo_rows : 0);
-                    for (int ks = 0; ks < k_steps; ++ks) {
-                        const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
-                        mma16_ss(d, a0 + o, b0 + o, id_qk, (term > 0 || ks > 0) ? 1u : 0u);
+                    for (int term = 0; term < 3; ++term) {
+                        const uint32_t a0 = tmem + kTmemQ + (term == 0 ? 64 : 0);
+                        const uint64_t b0 = kd + (term == 1 ? lo_rows : 0);
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            if (ks < steps)
+                                mma16_ts(d, a0 + ks * 8, b0 + uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2, id_qk,
+                                         (term > 0 || ks > 0) ? 1u : 0u);
                     }
-                }
-                mma_commit(k_empty);
+                };
+                if (k_steps == 8) terms(8);
+                else terms(k_steps);
+                mma_commit(&k_empty[j & 1]);
                 mma_commit(&s_full[j & 1]);
                 return true;
             };
             auto issue_pv = [&](int j) -> bool {
                 if (!mbar_spin_bounded(&p_full[j & 1], uint32_t((j >> 1) & 1))) return false;
-                if (j >= 2 && !mbar_spin_bounded(&o_empty[j & 1], uint32_t(((j >> 1) - 1) & 1))) return false;
+                if (j >= 1 && !mbar_spin_bounded(o_empty, uint32_t((j - 1) & 1))) return false;
                 const int np = min(2, n_pages - 2 * j);
-                const uint32_t d = tmem + kTmemO + (j & 1) * 128;
+                const uint32_t d = tmem + kTmemO;
                 for (int p = 0; p < np; ++p) {
                     if (!mbar_spin_bounded(&v_full[v_st], uint32_t(v_ph))) return false;
                     fence_after_sync();
@@ -527,7 +544,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                     mma_commit(&v_empty[v_st]);
                     if (++v_st == kVStages) { v_st = 0; v_ph ^= 1; }
                 }
-                mma_commit(&o_full[j & 1]);
+                mma_commit(o_full);
                 return true;
             };
             for (int j = 0; j < n_tiles && ok; ++j) {
@@ -556,6 +573,25 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         const float cq = __ldcg(&row_meta[size_t(qid) * kBM + rr]).x;
         const bool my_cols = col0 < n_pv;                 // head_dim <= 64: the second half has none
 
+        // query rows: shared-memory images -> tensor memory, warpgroup 0 the hi halves, 1 the lo halves
+        if (!warp_spin_bounded(q_full, 0, lane)) { report_status(status, kDevWaitFull); *abort_flag = 1; }
+        for (int b = 0; b < nb; ++b) {
+            const uint4* row = reinterpret_cast<const uint4*>(q_s + size_t(wg * nb + b) * kRowsSub + size_t(rr) * 128);
+            uint32_t x[32];
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch) {
+                const uint4 v = row[ch ^ (rr & 7)];
+                x[4 * ch] = v.x;
+                x[4 * ch + 1] = v.y;
+                x[4 * ch + 2] = v.z;
+                x[4 * ch + 3] = v.w;
+            }
+            tmem_st32(tmem + kTmemQ + lane_base + wg * 64 + b * 32, x);
+        }
+        tmem_wait_st();
+        fence_before_sync();
+        mbar_arrive(q_ready);
+
         float o[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) o[i] = 0.f;
@@ -564,20 +600,20 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         bool dead = false;
         // O += (tile j of tensor memory) * f, after O *= alpha
         auto add_tile = [&](int j, float alpha, float f) -> bool {
-            if (!warp_spin_bounded(&o_full[j & 1], uint32_t((j >> 1) & 1), lane)) return false;
+            if (!warp_spin_bounded(o_full, uint32_t(j & 1), lane)) return false;
             fence_after_sync();
             if (my_cols) {
                 uint32_t a[32];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    tmem_ld32(tmem + kTmemO + (j & 1) * 128 + lane_base + col0 + hf * 32, a);
+                    tmem_ld32(tmem + kTmemO + lane_base + col0 + hf * 32, a);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[hf * 32 + i] = fmaf(__uint_as_float(a[i]), f, o[hf * 32 + i] * alpha);
                 }
             }
             fence_before_sync();
-            mbar_arrive(&o_empty[j & 1]);
+            mbar_arrive(o_empty);
             return true;
         };
         const PageMeta* pm = meta + img0;
