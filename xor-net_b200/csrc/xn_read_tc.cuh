@@ -93,14 +93,12 @@ constexpr int kVStages = 3;
 constexpr int kQBytes = 4 * kRowsSub;    // 64 KB: hi and lo, two column blocks
 constexpr int kKBytes = 4 * kRowsSub;
 constexpr int kVBytes = 4 * kSub;        // 32 KB
-constexpr int kKStages = 2;
-constexpr int kSmemData = kKStages * kKBytes + kVStages * kVBytes;
-static_assert(kQBytes <= 2 * kVBytes, "the query images pass through V stages 1 and 2");
+constexpr int kSmemData = kQBytes + kKBytes + kVStages * kVBytes;
 constexpr int kSmemBytes = kSmemData + 3072;   // 227 KB, all there is: the block's window starts 1024-byte aligned
 static_assert(kSmemBytes <= 232448, "shared memory of a block");
-constexpr int kTmemQ = 0;                // hi 64 columns, lo 64 columns (two halves each)
-constexpr int kTmemS = 128;              // 2 x 128 columns
-constexpr int kTmemO = 384;              // 128 columns
+constexpr int kTmemS = 0;                // 2 x 128 columns
+constexpr int kTmemO = 256;              // P_hi V_hi, then P_hi V_lo + P_lo V_hi: up to 128 columns each
+constexpr int kSoftWarps = 8;
 
 constexpr int kAcctQStages = 2;
 constexpr int kAcctSmemData = kKBytes + kAcctQStages * kQBytes;
@@ -162,12 +160,21 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// (hi, lo) f16 pairs of two f32 values; lo is 0 behind an infinite or NaN hi
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
+// (hi, lo) f16 pairs of two f32 values
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __float22half2_rn(x);
     const float2 back = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack2(a - back.x, b - back.y);
+    const float2 rest = __fadd2_rn(x, make_float2(-back.x, -back.y));
+    lo = pack2(rest.x, rest.y);
+}
+
+// One arrival per warp: every lane's tensor-memory work is complete (wait::ld / wait::st) and ordered
+// before it.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+    pf::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
 }
 
 // Four scaled values of a lane (columns 4 * lane ..) into the hi and lo images of a row: column block
@@ -176,8 +183,8 @@ __device__ __forceinline__ void store_row_image(unsigned char* hi_img, unsigned 
                                                 int row, int lane, int nb, float4 x, bool safe) {
     if ((lane >> 4) >= nb) return;
     uint2 hi, lo;
-    split2(x.x, x.y, hi.x, lo.x);
-    split2(x.z, x.w, hi.y, lo.y);
+    split2(make_float2(x.x, x.y), hi.x, lo.x);
+    split2(make_float2(x.z, x.w), hi.y, lo.y);
     if (!safe) lo = make_uint2(0u, 0u);   // a query row with an infinity: inf - inf must not become NaN
     const size_t at = size_t(lane >> 4) * block_stride + size_t(row) * 128 +
                       size_t((((lane & 15) >> 1) ^ (row & 7)) * 16 + (lane & 1) * 8);
@@ -357,14 +364,18 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
     }
 }
 
-// Pass 2.  Shared memory: two K tiles (two pages each) of 64 KB | three V pages of 32 KB.  Tensor
-// memory: Q hi and lo (128 columns), two S / P buffers and one O tile of 128 columns each.  (Q in
-// shared memory left room for one K tile only, whose reload then sat between two tiles' MMAs:
-// 4.3 us a tile.)  Roles (320 threads): warp 0 copies
-// images (1-D bulk copies), warp 1 issues the MMAs -- the S of tile j + 1 before the O of tile j, so
-// that the softmax of a tile runs beside them -- and warps 2..9 are two softmax warpgroups: thread
-// r of each owns packed row r; warpgroup w takes page w of every tile and columns [64 w, 64 w + 64)
-// of O.  S is read from tensor memory, P goes back over it as hi (32 columns) and lo (32 columns).
+// Pass 2.  Shared memory: Q images 64 KB | K tile (two pages) 64 KB | three V pages of 32 KB.  Tensor
+// memory: two S / P buffers of 128 columns, one O tile of 2 x 128.  What the MMAs cost decides the
+// forms: one with A in tensor memory takes about 115 cycles for N = 128 and hardly more for N = 256
+// (64 would be the arithmetic's time), so S = Q K^T reads both operands from shared memory and
+// P_hi meets [V_hi | V_lo] as one N = 256 operand.  (With Q in tensor memory and three N = 128
+// products: 5900 cycles per tile of 128 positions, all of them MMA time.)  K has one buffer, whose
+// lo half is used first and refilled while the hi half is still read.  Roles (320 threads): warp 0
+// copies images (1-D bulk copies), warp 1 issues the MMAs -- the S of tile j + 1 before the O of
+// tile j, so that the softmax of a tile runs beside them -- and warps 2..9 are two softmax
+// warpgroups: thread r of each owns packed row r; warpgroup w takes page w of every tile and columns
+// [64 w, 64 w + 64) of O.  S is read from tensor memory, P goes back over it as hi (32 columns) and
+// lo (32 columns).
 // Every wait is bounded; on expiry the kernel records a status code, drains and returns.
 __global__ void __launch_bounds__(rt::kThreads, 1)
 read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items, const int* __restrict__ page_ids,
@@ -386,15 +397,14 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         if (threadIdx.x == 0) report_status(status, kDevBadIndex);
         return;
     }
-    unsigned char* k_s = smem;
-    unsigned char* v_s = k_s + kKStages * kKBytes;
-    unsigned char* q_s = v_s + kVBytes;        // until the query rows are in tensor memory
+    unsigned char* q_s = smem;
+    unsigned char* k_s = q_s + kQBytes;
+    unsigned char* v_s = k_s + kKBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemData);
     uint64_t* q_full = bars + 0;
-    uint64_t* q_ready = bars + 1;
-    uint64_t* k_full = bars + 2;               // [2]
-    uint64_t* k_empty = k_full + kKStages;     // [2]
-    uint64_t* v_full = k_empty + kKStages;     // [3]
+    uint64_t* k_full = bars + 1;               // [2]: lo, hi
+    uint64_t* k_empty = k_full + 2;            // [2]
+    uint64_t* v_full = k_empty + 2;            // [3]
     uint64_t* v_empty = v_full + kVStages;     // [3]
     uint64_t* s_full = v_empty + kVStages;     // [2]
     uint64_t* p_full = s_full + 2;             // [2]
@@ -420,10 +430,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
 
     if (tid == 0) {
         mbar_init(q_full, 1);
-        mbar_init(q_ready, 256);
         mbar_init(o_full, 1);
-        mbar_init(o_empty, 256);
-        for (int s = 0; s < kKStages; ++s) {
+        mbar_init(o_empty, kSoftWarps);
+        for (int s = 0; s < 2; ++s) {
             mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
         }
@@ -433,7 +442,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 256);
+            mbar_init(&p_full[s], kSoftWarps);
         }
         *abort_flag = 0;
         sm_dead[0] = sm_dead[1] = 0;
@@ -459,29 +468,27 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             const unsigned char* base = images + size_t(img0) * img_bytes;
             mbar_arrive_expect_tx(q_full, uint32_t(q_image_bytes(D)));
             bulk_g2s(q_s, q_images + size_t(qid) * q_image_bytes(D), uint32_t(q_image_bytes(D)), q_full);
-            auto load_k = [&](int j) -> bool {
-                const int st = j & 1;
-                if (j >= kKStages && !mbar_spin_bounded(&k_empty[st], uint32_t(((j >> 1) - 1) & 1))) return false;
-                const int np = min(2, n_pages - 2 * j);
-                mbar_arrive_expect_tx(&k_full[st], uint32_t(np * 2 * nb) * kSub);
+            auto load_k = [&](int j, int part) -> bool {   // part 0: lo, 1: hi
+                if (j > 0 && !mbar_spin_bounded(&k_empty[part], uint32_t((j - 1) & 1))) return false;
+                const int np = min(2, n_pages - 2 * j), b0 = part ? 0 : nb;
+                mbar_arrive_expect_tx(&k_full[part], uint32_t(np * nb) * kSub);
                 for (int p = 0; p < np; ++p)
-                    for (int b = 0; b < 2 * nb; ++b)   // hi blocks, then lo blocks
-                        bulk_g2s(k_s + size_t(st) * kKBytes + size_t(b) * kRowsSub + size_t(p) * kSub,
-                                 base + size_t(2 * j + p) * step + size_t(b) * kSub, kSub, &k_full[st]);
+                    for (int b = b0; b < b0 + nb; ++b)
+                        bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
+                                 base + size_t(2 * j + p) * step + size_t(b) * kSub, kSub, &k_full[part]);
                 return true;
             };
             auto load_v = [&](int pg) -> bool {
                 const int st = pg % kVStages;
-                if (pg == 1 && !mbar_spin_bounded(q_ready, 0)) return false;   // the query images sat there
                 if (pg >= kVStages && !mbar_spin_bounded(&v_empty[st], uint32_t((pg / kVStages - 1) & 1))) return false;
                 const uint32_t bytes = uint32_t(2 * nb) * kSub;
                 mbar_arrive_expect_tx(&v_full[st], bytes);
                 bulk_g2s(v_s + size_t(st) * kVBytes, base + size_t(pg) * step + size_t(2 * nb) * kSub, bytes, &v_full[st]);
                 return true;
             };
-            bool ok = load_k(0);
+            bool ok = load_k(0, 0) && load_k(0, 1);
             for (int j = 0; j < n_tiles && ok; ++j) {
-                if (j + 1 < n_tiles) ok = load_k(j + 1);
+                if (j + 1 < n_tiles) ok = load_k(j + 1, 0) && load_k(j + 1, 1);
                 for (int p = 2 * j; p < min(2 * j + 2, n_pages) && ok; ++p) ok = load_v(p);
                 if (*abort_flag) break;
             }
@@ -491,35 +498,41 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         // =============================== MMA issuer ===============================
         if (lane == 0) {
             const uint32_t id_qk = make_idesc16(kBM, kBM, 0);
-            const uint32_t id_pv = make_idesc16(kBM, n_pv, 1);
-            const uint64_t kd0 = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
+            const uint32_t id_pv = make_idesc16(kBM, nb * 64, 1);        // P_lo V_hi
+            const uint32_t id_pv2 = make_idesc16(kBM, nb * 128, 1);      // P_hi [V_hi | V_lo]
+            const uint64_t qd = smem_desc(smem_u32(q_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t kd = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
             const uint64_t vd0 = smem_desc(smem_u32(v_s), kSub, 1024, pf::kLayoutSw128);
             const uint64_t lo_rows = uint64_t(nb) * kRowsSub >> 4;   // hi image -> lo image, 128 rows
-            const uint64_t lo_page = uint64_t(nb) * kSub >> 4;       // ... of a page
-            bool ok = mbar_spin_bounded(q_ready, 0);
+            bool ok = mbar_spin_bounded(q_full, 0);
             if (!ok) { report_status(status, kDevWaitFull); *abort_flag = 1; }
             int v_st = 0, v_ph = 0;
             auto issue_qk = [&](int j) -> bool {
-                if (!mbar_spin_bounded(&k_full[j & 1], uint32_t((j >> 1) & 1))) return false;
+                if (!mbar_spin_bounded(&k_full[0], uint32_t(j & 1))) return false;
                 fence_after_sync();
                 const uint32_t d = tmem + kTmemS + (j & 1) * 128;
-                const uint64_t kd = kd0 + uint64_t(j & 1) * (kKBytes >> 4);
-                // the small products first: they meet a small accumulator
-                auto terms = [&](int steps) {
+                auto term = [&](uint64_t a0, uint64_t b0, uint32_t acc) {
+                    if (k_steps == 8) {
 #pragma unroll
-                    for (int term = 0; term < 3; ++term) {
-                        const uint32_t a0 = tmem + kTmemQ + (term == 0 ? 64 : 0);
-                        const uint64_t b0 = kd + (term == 1 ? lo_rows : 0);
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)
-                            if (ks < steps)
-                                mma16_ts(d, a0 + ks * 8, b0 + uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2, id_qk,
-                                         (term > 0 || ks > 0) ? 1u : 0u);
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
+                            mma16_ss(d, a0 + o, b0 + o, id_qk, ks > 0 ? 1u : acc);
+                        }
+                    } else {
+                        for (int ks = 0; ks < k_steps; ++ks) {
+                            const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
+                            mma16_ss(d, a0 + o, b0 + o, id_qk, ks > 0 ? 1u : acc);
+                        }
                     }
                 };
-                if (k_steps == 8) terms(8);
-                else terms(k_steps);
-                mma_commit(&k_empty[j & 1]);
+                // the small products first: they meet a small accumulator
+                term(qd, kd + lo_rows, 0u);
+                mma_commit(&k_empty[0]);
+                if (!mbar_spin_bounded(&k_full[1], uint32_t(j & 1))) return false;
+                fence_after_sync();
+                term(qd + lo_rows, kd, 1u);
+                term(qd, kd, 1u);
+                mma_commit(&k_empty[1]);
                 mma_commit(&s_full[j & 1]);
                 return true;
             };
@@ -534,13 +547,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                     const uint64_t vd = vd0 + uint64_t(v_st) * (kVBytes >> 4);
                     const uint32_t pa = tmem + kTmemS + (j & 1) * 128 + p * 64;
 #pragma unroll
-                    for (int term = 0; term < 3; ++term) {
-                        const uint32_t a0 = pa + (term == 0 ? 32 : 0);
-                        const uint64_t b0 = vd + (term == 1 ? lo_page : 0);
+                    for (int ks = 0; ks < 4; ++ks) mma16_ts(d, pa + ks * 8, vd + ks * 128, id_pv2, (p > 0 || ks > 0) ? 1u : 0u);
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            mma16_ts(d, a0 + ks * 8, b0 + ks * 128, id_pv, (p > 0 || term > 0 || ks > 0) ? 1u : 0u);
-                    }
+                    for (int ks = 0; ks < 4; ++ks) mma16_ts(d + nb * 64, pa + 32 + ks * 8, vd + ks * 128, id_pv, 1u);
                     mma_commit(&v_empty[v_st]);
                     if (++v_st == kVStages) { v_st = 0; v_ph ^= 1; }
                 }
@@ -573,47 +582,41 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         const float cq = __ldcg(&row_meta[size_t(qid) * kBM + rr]).x;
         const bool my_cols = col0 < n_pv;                 // head_dim <= 64: the second half has none
 
-        // query rows: shared-memory images -> tensor memory, warpgroup 0 the hi halves, 1 the lo halves
-        if (!warp_spin_bounded(q_full, 0, lane)) { report_status(status, kDevWaitFull); *abort_flag = 1; }
-        for (int b = 0; b < nb; ++b) {
-            const uint4* row = reinterpret_cast<const uint4*>(q_s + size_t(wg * nb + b) * kRowsSub + size_t(rr) * 128);
-            uint32_t x[32];
+        float2 o[32];
 #pragma unroll
-            for (int ch = 0; ch < 8; ++ch) {
-                const uint4 v = row[ch ^ (rr & 7)];
-                x[4 * ch] = v.x;
-                x[4 * ch + 1] = v.y;
-                x[4 * ch + 2] = v.z;
-                x[4 * ch + 3] = v.w;
-            }
-            tmem_st32(tmem + kTmemQ + lane_base + wg * 64 + b * 32, x);
-        }
-        tmem_wait_st();
-        fence_before_sync();
-        mbar_arrive(q_ready);
-
-        float o[64];
-#pragma unroll
-        for (int i = 0; i < 64; ++i) o[i] = 0.f;
+        for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
         float m_ref = -INFINITY, l_sum = 0.f;
         float alpha_prev = 1.f, f_prev = 0.f;             // pending accumulation of tile j - 1
         bool dead = false;
-        // O += (tile j of tensor memory) * f, after O *= alpha
+        auto scale_o = [&](float alpha) {                 // the maximum seldom moves after the first tiles
+            if (!__any_sync(kFull, alpha != 1.f)) return;
+            const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __fmul2_rn(o[i], a2);
+        };
+        // O = O * alpha + (tile j of tensor memory) * f
         auto add_tile = [&](int j, float alpha, float f) -> bool {
+            scale_o(alpha);
             if (!warp_spin_bounded(o_full, uint32_t(j & 1), lane)) return false;
             fence_after_sync();
             if (my_cols) {
-                uint32_t a[32];
+                const float2 f2 = make_float2(f, f);
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t a[32];
+                    tmem_ld32(tmem + kTmemO + nb * 64 + lane_base + col0 + hf * 32, a);   // the small products
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[hf * 16 + i] = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), f2, o[hf * 16 + i]);
                     tmem_ld32(tmem + kTmemO + lane_base + col0 + hf * 32, a);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[hf * 32 + i] = fmaf(__uint_as_float(a[i]), f, o[hf * 32 + i] * alpha);
+                    for (int i = 0; i < 16; ++i)
+                        o[hf * 16 + i] = __ffma2_rn(make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])), f2, o[hf * 16 + i]);
                 }
             }
-            fence_before_sync();
-            mbar_arrive(o_empty);
+            warp_arrive(o_empty, lane);
             return true;
         };
         const PageMeta* pm = meta + img0;
@@ -676,12 +679,13 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             mx = fmaxf(mx, xc[(wg ^ 1) * 128 + rr]);
             const float m_new = fmaxf(m_ref, mx);
             const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
-            float alpha = m_new == -INFINITY ? 1.f : pf::ex2(m_ref - m_new);
+            float alpha = m_new == m_ref ? 1.f : pf::ex2(m_ref - m_new);
             m_ref = m_new;
             l_sum *= alpha;
             if (have) {
                 const float pscale = kPScale * ((wg ? fv1 : fv0) / fv);   // powers of two: exact
-                float ps0 = 0.f, ps1 = 0.f;
+                float2 ps = make_float2(0.f, 0.f);
+                const float2 cm2 = make_float2(cm, cm), nm2 = make_float2(neg_m, neg_m), sc2 = make_float2(pscale, pscale);
                 uint32_t hi[32], lo[32];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
@@ -695,14 +699,14 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float a = pf::ex2(fmaf(__uint_as_float(x[2 * i]), cm, neg_m));
-                        const float b = pf::ex2(fmaf(__uint_as_float(x[2 * i + 1]), cm, neg_m));
-                        ps0 += a;
-                        ps1 += b;
-                        split2(a * pscale, b * pscale, hi[hf * 16 + i], lo[hf * 16 + i]);
+                        float2 p = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), cm2, nm2);
+                        p.x = pf::ex2(p.x);
+                        p.y = pf::ex2(p.y);
+                        ps = __fadd2_rn(ps, p);
+                        split2(__fmul2_rn(p, sc2), hi[hf * 16 + i], lo[hf * 16 + i]);
                     }
                 }
-                l_sum += ps0 + ps1;
+                l_sum += ps.x + ps.y;
                 tmem_st32(s_addr, hi);
                 tmem_st32(s_addr + 32, lo);
                 tmem_wait_st();
@@ -713,8 +717,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 if (j > 0) {
                     if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
                 }
-#pragma unroll
-                for (int i = 0; i < 64; ++i) o[i] *= alpha;
+                scale_o(alpha);
                 alpha = 1.f;
                 fence_before_sync();
                 wg_barrier();
@@ -738,7 +741,10 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                         wg_barrier();
                         if (key < limit) {   // (a weight of zero times an infinity is a NaN, as in a plain sum)
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) o[i] = fmaf(pv, vrow[col0 + i], o[i]);
+                            for (int i = 0; i < 32; ++i) {
+                                o[i].x = fmaf(pv, vrow[col0 + 2 * i], o[i].x);
+                                o[i].y = fmaf(pv, vrow[col0 + 2 * i + 1], o[i].y);
+                            }
                         }
                         wg_barrier();
                     }
@@ -746,8 +752,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 fence_before_sync();
                 wg_barrier();
             } else if (j > 0) {
-                fence_before_sync();
-                mbar_arrive(&p_full[sb]);
+                warp_arrive(&p_full[sb], lane);
                 if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
                 alpha_prev = alpha;
                 f_prev = fv * (1.0f / kPScale);
@@ -755,8 +760,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             }
             alpha_prev = alpha;
             f_prev = fv * (1.0f / kPScale);
-            fence_before_sync();
-            mbar_arrive(&p_full[sb]);
+            warp_arrive(&p_full[sb], lane);
         }
         if (dead && lane == 0) report_status(status, kDevWaitFull);
         if (!dead) {
@@ -782,9 +786,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             float4* tile = reinterpret_cast<float4*>(k_s);   // [128 rows][32 chunks]
             if (my_cols) {
 #pragma unroll
-                for (int i = 0; i < 64; i += 4) {
-                    const int chunk = (col0 + i) >> 2;
-                    tile[rr * 32 + (chunk ^ (rr & 31))] = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                for (int i = 0; i < 32; i += 2) {
+                    const int chunk = (col0 >> 2) + (i >> 1);
+                    tile[rr * 32 + (chunk ^ (rr & 31))] = make_float4(o[i].x * inv, o[i].y * inv, o[i + 1].x * inv, o[i + 1].y * inv);
                 }
             }
             wg_barrier();
