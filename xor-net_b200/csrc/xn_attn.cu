@@ -139,6 +139,10 @@ struct xn_stream {
     // with the other callers, and the kernels read and write the buffer over PCIe directly.
     unsigned char* call_buf = nullptr;
     size_t call_cap = 0;
+    // The page table on the device, for reads that do not append: its first `pages_d_valid` entries
+    // are up to date (uploaded on the context's stream when a read needs more).
+    int* pages_d = nullptr;
+    size_t pages_d_cap = 0, pages_d_valid = 0;
 };
 
 // One context per GPU of a box behind one handle; streams are placed on the least-loaded one.
@@ -231,6 +235,7 @@ struct xn_ctx {
                                                            // (allocated by the first call that keeps one)
     int read_tc_min_rows = 24;    // packed rows (rows x heads of a group) from which the tensor cores take a read
     bool read_funcs_ready = false;
+    ReadTable read_table;         // the launch parameter of a read, filled in place
     // attention output block (sub-norm + ternary o_proj)
     std::vector<OutProj> out_proj;                         // per layer
     std::vector<OutProj> qkv_proj;                         // per layer: q, k, v rows stacked, no norm
@@ -360,35 +365,47 @@ struct SplitKernel {
     int tile_tokens;
 };
 
-template <int NV, int GT, bool EXACT, bool EXT>
-SplitKernel make_split() {
-    return {attn_splitkv_kernel<NV, GT, EXACT, EXT>, DecodeSmem<NV, GT, EXT>::kBytes, DecodeCfg<NV>::kThreads,
-            DecodeCfg<NV>::kTPS};
+using ReadFn = void (*)(const ReadTable, const float*, const float*, float*, int*, long long, int, int, int, float, int*);
+struct ReadKernel {
+    ReadFn fn;
+    size_t smem;
+    int threads;
+};
+
+// What a dispatch hands out: the decode kernel, its variant with scores, the read kernel without and
+// with scores.
+struct SplitKernels {
+    SplitKernel decode, scores;
+    ReadKernel read[2];
+};
+
+template <int NV, int GT, bool EXACT>
+SplitKernels make_split() {
+    using Cfg = DecodeCfg<NV>;
+    return {{attn_splitkv_kernel<NV, GT, EXACT>, DecodeSmem<NV, GT>::kBytes, Cfg::kThreads, Cfg::kTPS},
+            {attn_splitkv_scores_kernel<NV, GT, EXACT>, DecodeSmem<NV, GT, true>::kBytes, Cfg::kThreads, Cfg::kTPS},
+            {{attn_read_kernel<NV, GT, EXACT, false>, DecodeSmem<NV, GT>::kBytes, Cfg::kThreads},
+             {attn_read_kernel<NV, GT, EXACT, true>, DecodeSmem<NV, GT, true>::kBytes, Cfg::kThreads}}};
 }
 
 template <int NV, bool EXACT>
-SplitKernel pick_gt(int gt, bool ext) {
-    if (ext) {
-        if (gt == 4) return make_split<NV, 4, EXACT, true>();
-        if (gt == 2) return make_split<NV, 2, EXACT, true>();
-        return make_split<NV, 1, EXACT, true>();
-    }
-    if (gt == 4) return make_split<NV, 4, EXACT, false>();
-    if (gt == 2) return make_split<NV, 2, EXACT, false>();
-    return make_split<NV, 1, EXACT, false>();
+SplitKernels pick_gt(int gt) {
+    if (gt == 4) return make_split<NV, 4, EXACT>();
+    if (gt == 2) return make_split<NV, 2, EXACT>();
+    return make_split<NV, 1, EXACT>();
 }
 
 // Exact instantiations exist for the row lengths of head_dim 64, 100, 128 and 256.
-// ext: the variant that also writes the scores and the log-sum-exps (reads that keep an account).
-SplitKernel pick_split(int nv_class, int gt, bool exact, bool ext = false) {
+SplitKernels pick_splits(int nv_class, int gt, bool exact) {
     switch (nv_class) {
-        case 8: return pick_gt<8, false>(gt, ext);
-        case 16: return exact ? pick_gt<16, true>(gt, ext) : pick_gt<16, false>(gt, ext);
-        case 25: return pick_gt<25, true>(gt, ext);
-        case 32: return exact ? pick_gt<32, true>(gt, ext) : pick_gt<32, false>(gt, ext);
-        default: return exact ? pick_gt<64, true>(gt, ext) : pick_gt<64, false>(gt, ext);
+        case 8: return pick_gt<8, false>(gt);
+        case 16: return exact ? pick_gt<16, true>(gt) : pick_gt<16, false>(gt);
+        case 25: return pick_gt<25, true>(gt);
+        case 32: return exact ? pick_gt<32, true>(gt) : pick_gt<32, false>(gt);
+        default: return exact ? pick_gt<64, true>(gt) : pick_gt<64, false>(gt);
     }
 }
+SplitKernel pick_split(int nv_class, int gt, bool exact) { return pick_splits(nv_class, gt, exact).decode; }
 
 using Split8Fn = void (*)(const ReqDev*, const UnitDev*, const ItemDev*, const int*, int, const int*,
                           const uint8_t*, float*, int*, long long, int, int, float, const float*,
@@ -573,6 +590,7 @@ void release_pages(xn_ctx* c, xn_stream* s) {
     c->pcache.valid = false;   // the kept plan may name this stream's pages
     for (auto it = s->pages.rbegin(); it != s->pages.rend(); ++it) c->free_pages.push_back(*it);
     s->pages.clear();
+    s->pages_d_valid = 0;
     std::fill(s->hw.begin(), s->hw.end(), 0);
     std::fill(s->acc_len.begin(), s->acc_len.end(), 0);
     std::fill(s->shift.begin(), s->shift.end(), 0);
@@ -801,6 +819,7 @@ struct StreamRollback {
                 c->free_pages.push_back(s->pages.back());
                 s->pages.pop_back();
             }
+            s->pages_d_valid = std::min(s->pages_d_valid, s->pages.size());
             s->hw[size_t(it->layer)] = it->hw;
         }
     }
@@ -1997,6 +2016,7 @@ int32_t xn_ctx_destroy(xn_ctx* c) {
     if (c->stream) cudaStreamSynchronize(c->stream);
     for (xn_stream* s : c->streams) {
         free_call_buffer(s);
+        guarded_free(c, s->pages_d);
         s->magic = 0;
         delete s;
     }
@@ -2150,6 +2170,7 @@ int32_t xn_stream_destroy(xn_ctx* c, xn_stream* s) {
         c->streams.erase(s);
     }
     free_call_buffer(s);
+    guarded_free(c, s->pages_d);
     s->magic = 0;
     delete s;
     return XN_OK;

@@ -78,6 +78,36 @@ struct ReqPatchTable {
     ReqPatch e[kPatchReqs];
 };
 
+// A read that does not append, as a kernel parameter: nothing has to be planned or uploaded for it.
+// The tiles of all (request, KV head, head subgroup, row) units are numbered through, request by
+// request; every unit of a request has `n_tiles` of them and block b of G takes tiles
+// [T b / G, T (b + 1) / G).
+constexpr int kReadEntries = 64;
+struct ReadEntry {
+    const float* q;
+    float* out;
+    const int* pages;         // the stream's page table on the device
+    float* scores;            // with weights: as in ReqDev
+    float* lse;
+    float* user;              // the caller's copy of the account, or nullptr
+    long long user_hs;
+    long long q_hs, q_ts, o_hs, o_ts;
+    long long sc_hs, sc_ts, lse_hs;
+    long long tile0;          // first tile of the request
+    int n_tiles;              // of one unit
+    int rows, kv_len, layer;
+    int old_from, old_len, store;   // of the account: see AccountDev
+    int pad;
+};
+struct ReadTable {
+    int n;
+    int subs, gt, group;      // head subgroups per KV head, heads per subgroup, heads per KV head
+    int n_blocks;             // G
+    int pad;
+    long long n_tiles;        // T
+    ReadEntry e[kReadEntries];
+};
+
 // A (request, KV head, query-head subgroup, query row) to attend over kv_len cached tokens.
 struct UnitDev {
     int req;

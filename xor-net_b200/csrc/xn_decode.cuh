@@ -186,16 +186,18 @@ struct DecodeSmem {
 // EXT: the raw scores (scaled by 1/sqrt(D)) and the log-sum-exp of every row go to ReqDev::scores
 // and ReqDev::lse as well: 4 bytes per query head and position next to the 8 D / GT bytes of K and
 // V that the head's share of the read costs.
-template <int NV, int GT, bool EXACT, bool EXT = false>
-__global__ void __launch_bounds__(DecodeCfg<NV>::kThreads, 1)
-attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
-                    const ItemDev* __restrict__ items, const int* __restrict__ chunk_item_begin,
-                    int n_chunks, const int* __restrict__ page_ids,
-                    const float* __restrict__ k_pool, const float* __restrict__ v_pool,
-                    float* __restrict__ partials, int* __restrict__ sync, long long pool_pages,
-                    int num_kv_heads, int head_dim, int nv_arg, float scale,
-                    const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-                    int* __restrict__ status, const __grid_constant__ ReqPatchTable patch) {
+// READ: a read that does not append, described by the ReadTable parameter `tab` (the plan arrays and
+// `patch` are not used): every block works out its own tiles, units and partial slots from it.
+template <int NV, int GT, bool EXACT, bool EXT, bool READ>
+__device__ __forceinline__ void
+splitkv_body(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
+             const ItemDev* __restrict__ items, const int* __restrict__ chunk_item_begin,
+             int n_chunks, const int* __restrict__ page_ids,
+             const float* __restrict__ k_pool, const float* __restrict__ v_pool,
+             float* __restrict__ partials, int* __restrict__ sync, long long pool_pages,
+             int num_kv_heads, int head_dim, int nv_arg, float scale,
+             const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+             int* __restrict__ status, const ReqPatchTable* patch_p, const ReadTable* tab) {
     const int nv = EXACT ? NV : nv_arg;
     using Cfg = DecodeCfg<NV>;
     using Sm = DecodeSmem<NV, GT, EXT>;
@@ -239,6 +241,99 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
         // =============================== producer ===============================
         int fill = 0;
         bool ok = true;
+        if constexpr (READ) {
+            const long long T = tab->n_tiles, G = tab->n_blocks, b = blockIdx.x;
+            auto block_of = [&](long long tile) { return int(((tile + 1) * G - 1) / T); };
+            long long cur = T * b / G;
+            const long long hi = T * (b + 1) / G;
+            int rq = 0;
+            while (ok && cur < hi) {
+                while (rq + 1 < tab->n && cur >= tab->e[rq + 1].tile0) ++rq;
+                const ReadEntry& e = tab->e[rq];
+                const long long unit = (cur - e.tile0) / e.n_tiles;
+                const long long unit0 = e.tile0 + unit * e.n_tiles;   // the unit's first tile
+                const int tile_begin = int(cur - unit0);
+                const int tile_end = int(min((long long)e.n_tiles, hi - unit0));
+                const int b0 = block_of(unit0), b1 = block_of(unit0 + e.n_tiles - 1);
+                const int t = int(unit % e.rows);
+                const int hs = int(unit / e.rows);
+                const int kv_head = hs / tab->subs, sb = hs % tab->subs;
+                const int head0 = kv_head * tab->group + sb * tab->gt;
+                Hdr h;
+                h.q = e.q + size_t(head0) * e.q_hs + size_t(t) * e.q_ts;
+                h.out = e.out + size_t(head0) * e.o_hs + size_t(t) * e.o_ts;
+                h.q_hs = e.q_hs;
+                h.o_hs = e.o_hs;
+                h.nheads = min(tab->gt, tab->group - sb * tab->gt);
+                // a block has at most one unit that began before it (slot 2b) and one that goes on
+                // behind it (slot 2b + 1)
+                h.part = b1 == b0 ? -1 : (int(b) == b0 ? 2 * int(b) + 1 : 2 * int(b));
+                h.part_begin = 2 * b0 + 1;
+                h.part_count = b1 - b0 + 1;
+                h.merge_slot = b0;
+                h.new_key = -1;
+                h.k_dst = nullptr;
+                h.v_dst = nullptr;
+                if constexpr (EXT) {
+                    h.lse = e.lse + size_t(head0) * e.lse_hs + t;
+                    h.lse_hs = e.lse_hs;
+                    h.sc_hs = e.sc_hs;
+                }
+                const bool stage_q = Sm::kStageQ && (head_dim % 4 == 0) &&
+                                     ((reinterpret_cast<uintptr_t>(h.q) | uintptr_t(h.q_hs * 4)) & 15) == 0;
+                const size_t lbase = size_t(e.layer) * size_t(pool_pages);
+                for (int tb = tile_begin; tb < tile_end && ok; tb += 32) {
+                    const int my_tile = tb + lane;
+                    int my_page = 0;
+                    if (my_tile < tile_end) my_page = e.pages[(my_tile * TPS) / kPageTokens];
+                    const int n_t = min(32, tile_end - tb);
+                    for (int tt = 0; tt < n_t; ++tt, ++fill) {
+                        __syncwarp();
+                        const int page = __shfl_sync(kFull, my_page, tt);
+                        if (lane == 0) {
+                            const int tile = tb + tt;
+                            const int s = fill % ST;
+                            if (fill >= ST && !XN_DECODE_WAIT(&empty_bar[s], ((fill / ST) - 1) & 1)) {
+                                report_status(status, kDevWaitEmpty);
+                                *abort_flag = 1;
+                                ok = false;
+                            } else if (!XN_PAGE_OK(page, pool_pages)) {
+                                report_status(status, kDevBadIndex);
+                                *abort_flag = 1;
+                                ok = false;
+                            } else {
+                                const int tok0 = tile * TPS;
+                                const int ntok = min(TPS, e.kv_len - tok0);
+                                const size_t src = ((lbase + size_t(page)) * num_kv_heads + kv_head) * page_floats +
+                                                   size_t(tok0 % kPageTokens) * dp;
+                                const bool first = tile == tile_begin;
+                                const uint32_t bytes = uint32_t(ntok) * dp * 4;
+                                const uint32_t row_bytes = uint32_t(dp) * 4;
+                                h.flags = (first ? kHdrFirst : 0) | (tile == tile_end - 1 ? kHdrLast : 0) |
+                                          (first && stage_q ? kHdrQStaged : 0);
+                                h.ntok = ntok;
+                                if constexpr (EXT)
+                                    h.scores = e.scores + size_t(head0) * e.sc_hs + size_t(t) * e.sc_ts + tok0;
+                                hdr[s] = h;
+                                float* dst = stage_ptr(s);
+                                const uint32_t q_bytes = (first && stage_q) ? uint32_t(h.nheads) * row_bytes : 0u;
+                                mbar_arrive_expect_tx(&full_bar[s], 2 * bytes + q_bytes);
+                                bulk_g2s(dst, k_pool + src, bytes, &full_bar[s]);
+                                bulk_g2s(dst + TPS * NV * 4, v_pool + src, bytes, &full_bar[s]);
+                                if (q_bytes)
+                                    for (int hh = 0; hh < h.nheads; ++hh)
+                                        bulk_g2s(dst + Cfg::kStageFloats + hh * dp, h.q + size_t(hh) * h.q_hs,
+                                                 row_bytes, &full_bar[s]);
+                            }
+                        }
+                        ok = __shfl_sync(kFull, ok ? 1 : 0, 0) != 0;
+                        if (!ok) break;
+                    }
+                }
+                cur = unit0 + tile_end;
+            }
+        } else {
+        const ReqPatchTable& patch = *patch_p;
         int chunk = blockIdx.x;
         while (ok && chunk < n_chunks) {
             const int it_lo = chunk_item_begin[chunk], it_hi = chunk_item_begin[chunk + 1];
@@ -405,6 +500,7 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
             if (lane == 0) next = atomicAdd(&sync[kSyncChunk], 1) + int(gridDim.x);
             chunk = __shfl_sync(kFull, next, 0);
         }
+        }
         if (lane == 0) {
             if (ok) {
                 // end-of-work marker
@@ -424,10 +520,12 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
                     mbar_wait_bounded(&full_bar[f % ST], (f / ST) & 1);
             }
             // the last block to finish re-arms the chunk counter for the next launch
-            __threadfence();
-            if (atomicAdd(&sync[kSyncDone], 1) == int(gridDim.x) - 1) {
-                sync[kSyncChunk] = 0;
-                sync[kSyncDone] = 0;
+            if constexpr (!READ) {
+                __threadfence();
+                if (atomicAdd(&sync[kSyncDone], 1) == int(gridDim.x) - 1) {
+                    sync[kSyncChunk] = 0;
+                    sync[kSyncDone] = 0;
+                }
             }
         }
         return;
@@ -756,16 +854,21 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
         named_bar_sync(1, W * 32);
         if (*last_flag) {
             const size_t ps = part_stride_floats(nv);
+            // (a read's records: the slot behind its first block's tiles, then the slots before the others')
+            auto rec_at = [&](int i, int hh) {
+                const int slot = READ ? h.part_begin + 2 * i - (i > 0 ? 1 : 0) : h.part_begin + i;
+                return partials + (size_t(slot) * GT + hh) * ps;
+            };
             for (int e = ctid; e < GT * nv; e += W * 32) {
                 const int hh = e / nv, idx = e % nv;
                 if (hh >= h.nheads) continue;
                 float M = -INFINITY;
                 for (int i = 0; i < h.part_count; ++i)
-                    M = fmaxf(M, __ldcg(partials + (size_t(h.part_begin + i) * GT + hh) * ps));
+                    M = fmaxf(M, __ldcg(rec_at(i, hh)));
                 float L = 0.f;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int i = 0; i < h.part_count; ++i) {
-                    const float* rec = partials + (size_t(h.part_begin + i) * GT + hh) * ps;
+                    const float* rec = rec_at(i, hh);
                     const float mi = __ldcg(rec);
                     const float wgt = (mi == -INFINITY) ? 0.f : expf(mi - M);
                     L += __ldcg(rec + 1) * wgt;
@@ -790,6 +893,50 @@ attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__
         // (no barrier here: `red` and `last_flag` are next written behind the next item's barriers,
         // which no thread passes before every thread has left this point)
     }
+}
+
+template <int NV, int GT, bool EXACT>
+__global__ void __launch_bounds__(DecodeCfg<NV>::kThreads, 1)
+attn_splitkv_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
+                    const ItemDev* __restrict__ items, const int* __restrict__ chunk_item_begin,
+                    int n_chunks, const int* __restrict__ page_ids,
+                    const float* __restrict__ k_pool, const float* __restrict__ v_pool,
+                    float* __restrict__ partials, int* __restrict__ sync, long long pool_pages,
+                    int num_kv_heads, int head_dim, int nv_arg, float scale,
+                    const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+                    int* __restrict__ status, const __grid_constant__ ReqPatchTable patch) {
+    splitkv_body<NV, GT, EXACT, false, false>(reqs, units, items, chunk_item_begin, n_chunks, page_ids, k_pool, v_pool,
+                                              partials, sync, pool_pages, num_kv_heads, head_dim, nv_arg, scale, cos_t,
+                                              sin_t, status, &patch, nullptr);
+}
+
+// The same over a ReadTable; EXT also leaves the scores and the log-sum-exps.
+template <int NV, int GT, bool EXACT, bool EXT>
+__global__ void __launch_bounds__(DecodeCfg<NV>::kThreads, 1)
+attn_read_kernel(const __grid_constant__ ReadTable tab, const float* __restrict__ k_pool,
+                 const float* __restrict__ v_pool, float* __restrict__ partials, int* __restrict__ sync,
+                 long long pool_pages, int num_kv_heads, int head_dim, int nv_arg, float scale,
+                 int* __restrict__ status) {
+    splitkv_body<NV, GT, EXACT, EXT, true>(nullptr, nullptr, nullptr, nullptr, 0, nullptr, k_pool, v_pool, partials, sync,
+                                           pool_pages, num_kv_heads, head_dim, nv_arg, scale, nullptr, nullptr, status,
+                                           nullptr, &tab);
+}
+
+// ... and, with the plan arrays (prompt rows that the tensor-core read does not take: causal, or of
+// head_dim > 128), the scores too.
+template <int NV, int GT, bool EXACT>
+__global__ void __launch_bounds__(DecodeCfg<NV>::kThreads, 1)
+attn_splitkv_scores_kernel(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
+                           const ItemDev* __restrict__ items, const int* __restrict__ chunk_item_begin,
+                           int n_chunks, const int* __restrict__ page_ids,
+                           const float* __restrict__ k_pool, const float* __restrict__ v_pool,
+                           float* __restrict__ partials, int* __restrict__ sync, long long pool_pages,
+                           int num_kv_heads, int head_dim, int nv_arg, float scale,
+                           const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+                           int* __restrict__ status, const __grid_constant__ ReqPatchTable patch) {
+    splitkv_body<NV, GT, EXACT, true, false>(reqs, units, items, chunk_item_begin, n_chunks, page_ids, k_pool, v_pool,
+                                             partials, sync, pool_pages, num_kv_heads, head_dim, nv_arg, scale, cos_t,
+                                             sin_t, status, &patch, nullptr);
 }
 
 // Generic attention for requests whose positions fold around the ring (index_pos + seq_len >

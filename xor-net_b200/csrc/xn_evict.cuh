@@ -11,8 +11,9 @@
 namespace xn {
 
 struct EvictDev {
-    int page_off;
+    const int* pages;          // the stream's page table on the device
     int layer0, n_layers;      // layers [layer0, layer0 + n_layers)
+    int acc_len;               // positions behind it have an account of zero (the same in all these layers)
     int len, keep, recent;
     int head0;                 // first (layer, KV head) row of this request among the launch's rows
     int copy;                  // 1: the rows go to k_out / v_out and the stream stays as it is;
@@ -22,6 +23,14 @@ struct EvictDev {
     float* k_out;
     float* v_out;
     float* w_out;              // the kept positions' accounts for the caller, or nullptr
+};
+
+// A launch's requests, as a kernel parameter.
+constexpr int kEvictEntries = 24;
+struct EvictTable {
+    int n;
+    int pad;
+    EvictDev e[kEvictEntries];
 };
 
 namespace ev {
@@ -95,9 +104,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* scratch, ui
 // RUN = 0: streams too long for that; the keys are read again in every pass.
 template <int RUN>
 __global__ void __launch_bounds__(ev::kThreads, 1)
-evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __restrict__ page_ids,
-                    const float* __restrict__ pool, long long pool_pages, int num_kv_heads, int cluster,
-                    const int* __restrict__ acc_len) {
+evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restrict__ pool, long long pool_pages,
+                    int num_kv_heads, int cluster) {
     using namespace ev;
     pdl_launch_dependents();
     __shared__ uint32_t hist[2][kBins];             // by pass parity: peers may still read the other one
@@ -107,8 +115,8 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
     const int row = int(blockIdx.x) / cluster;
     const uint32_t rank = cluster_rank();
     int rq = 0;
-    while (rq + 1 < n_reqs && row >= reqs[rq + 1].head0) ++rq;
-    const EvictDev r = reqs[rq];
+    while (rq + 1 < tab.n && row >= tab.e[rq + 1].head0) ++rq;
+    const EvictDev& r = tab.e[rq];
     const int local = row - r.head0;
     const int l = r.layer0 + local / num_kv_heads, h = local % num_kv_heads;
     const int tid = threadIdx.x, lane = tid & 31;
@@ -118,8 +126,8 @@ evict_select_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __
     const int run = RUN > 0 ? RUN : (((n_cand + cluster * kThreads - 1) / (cluster * kThreads)) + 3) / 4 * 4;
     const long long lo_ll = (long long)(int(rank) * kThreads + tid) * run;
     const int lo = int(lo_ll < n_cand ? lo_ll : n_cand), hi = min(n_cand, lo + run);
-    const int* pages = page_ids + r.page_off;
-    const int valid = acc_len[row];                 // positions behind it have an account of zero
+    const int* pages = r.pages;
+    const int valid = r.acc_len;
     const size_t base = (size_t(l) * size_t(pool_pages)) * num_kv_heads * kPageTokens + size_t(h) * kPageTokens;
     const size_t pstep = size_t(num_kv_heads) * kPageTokens;
     auto load = [&](int j) -> float {
@@ -284,16 +292,16 @@ struct EvictPools {
 // row.  Bound by memory: each kept row is read and written once.
 template <int ROWS>
 __global__ void __launch_bounds__(256)
-evict_copy_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __restrict__ page_ids, EvictPools p) {
+evict_copy_kernel(const __grid_constant__ EvictTable tab, EvictPools p) {
     pdl_wait();
     int rq = 0;
-    while (rq + 1 < n_reqs && int(blockIdx.x) >= reqs[rq + 1].head0) ++rq;
-    const EvictDev& r = reqs[rq];
+    while (rq + 1 < tab.n && int(blockIdx.x) >= tab.e[rq + 1].head0) ++rq;
+    const EvictDev& r = tab.e[rq];
     if (r.copy != 1) return;
     const int local = int(blockIdx.x) - r.head0;
     const int l = r.layer0 + local / p.num_kv_heads, h = local % p.num_kv_heads;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int* pages = page_ids + r.page_off;
+    const int* pages = r.pages;
     const int* kept = r.kept_ws + size_t(local) * r.keep;
     const size_t lbase = size_t(l) * size_t(p.pool_pages);
     const int D = p.head_dim;
@@ -363,12 +371,11 @@ evict_copy_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __re
 constexpr int kMoveThreads = 512;
 constexpr int kMoveSlice = 128;    // bytes of a row per block
 __global__ void __launch_bounds__(kMoveThreads)
-evict_move_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __restrict__ page_ids, EvictPools p,
-                  const int* __restrict__ acc_len) {
+evict_move_kernel(const __grid_constant__ EvictTable tab, EvictPools p) {
     pdl_wait();
     int rq = 0;
-    while (rq + 1 < n_reqs && int(blockIdx.x) >= reqs[rq + 1].head0) ++rq;
-    const EvictDev& r = reqs[rq];
+    while (rq + 1 < tab.n && int(blockIdx.x) >= tab.e[rq + 1].head0) ++rq;
+    const EvictDev& r = tab.e[rq];
     if (r.copy) return;
     const int row = int(blockIdx.x);
     const int local = row - r.head0;
@@ -378,9 +385,9 @@ evict_move_kernel(const EvictDev* __restrict__ reqs, int n_reqs, const int* __re
     const int row_bytes = p.u8 ? p.dq : p.nv * 16;
     const int off = slice * kMoveSlice;
     const int bytes = min(kMoveSlice, row_bytes - off);
-    const int* pages = page_ids + r.page_off;
+    const int* pages = r.pages;
     const int* kept = r.kept_ws + size_t(local) * r.keep;
-    const int valid = acc_len[row];
+    const int valid = r.acc_len;
     const size_t lbase = size_t(l) * size_t(p.pool_pages);
     unsigned char* base;
     size_t blk_bytes;

@@ -53,6 +53,20 @@ struct FewAccount {
     int row_step;          // 1 causal, 0 otherwise
 };
 
+__device__ __forceinline__ float account_sum(const FewAccount& r, int h, int group, int key) {
+    float sum = 0.f;
+    for (int t = 0; t < r.rows; ++t) {
+        if (key >= r.row_limit0 + t * r.row_step) continue;
+#pragma unroll 4
+        for (int g = 0; g < group; ++g) {
+            const size_t head = size_t(h) * group + g;
+            const float s = r.scores[head * r.sc_hs + size_t(t) * r.sc_ts + key];
+            sum += expf(s - r.lse[head * r.lse_hs + t]);
+        }
+    }
+    return sum;
+}
+
 // One thread per cached position, blockIdx.y = KV head, blockIdx.z = request: 4 (G rows + 1..2)
 // bytes per position, read coalesced along the positions; a few per cent of what the attention
 // kernel before it reads.  The sum's order is fixed (rows, then heads): the same bits every time.
@@ -64,18 +78,20 @@ account_few_kernel(const FewAccount* __restrict__ reqs, const int* __restrict__ 
     const int key = int(blockIdx.x) * 256 + int(threadIdx.x);
     if (key >= r.a.kv_len) return;
     pdl_wait();            // scores and log-sum-exps come from the kernel before this one
-    const int h = blockIdx.y;
-    float sum = 0.f;
-    for (int t = 0; t < r.rows; ++t) {
-        if (key >= r.row_limit0 + t * r.row_step) continue;
-#pragma unroll 4
-        for (int g = 0; g < group; ++g) {
-            const size_t head = size_t(h) * group + g;
-            const float s = r.scores[head * r.sc_hs + size_t(t) * r.sc_ts + key];
-            sum += expf(s - r.lse[head * r.lse_hs + t]);
-        }
-    }
-    account_store(r.a, page_ids, pool, pool_pages, num_kv_heads, h, key, sum);
+    account_store(r.a, page_ids, pool, pool_pages, num_kv_heads, blockIdx.y, key, account_sum(r, blockIdx.y, group, key));
+}
+
+// The same for a read that came as a ReadTable.
+__global__ void __launch_bounds__(256)
+account_table_kernel(const __grid_constant__ ReadTable tab, float* __restrict__ pool, long long pool_pages, int num_kv_heads) {
+    pdl_launch_dependents();
+    const ReadEntry& e = tab.e[blockIdx.z];
+    const int key = int(blockIdx.x) * 256 + int(threadIdx.x);
+    if (key >= e.kv_len) return;
+    const FewAccount r = {{e.user, e.user_hs, e.old_from, e.old_len, e.store, e.kv_len, 0, e.layer},
+                          e.scores, e.lse, e.sc_hs, e.sc_ts, e.lse_hs, e.rows, e.kv_len, 0};
+    pdl_wait();
+    account_store(r.a, e.pages, pool, pool_pages, num_kv_heads, blockIdx.y, key, account_sum(r, blockIdx.y, tab.group, key));
 }
 
 // Rows that see no position: zeros.

@@ -289,12 +289,96 @@ CacheView cache_view(const xn_ctx* c) {
 int32_t ready_read_kernels(xn_ctx* c) {
     if (c->read_funcs_ready) return XN_OK;
     if (!c->kv_u8) {
-        const SplitKernel k = pick_split(c->nv_class, c->gt, c->nv_exact, true);
-        XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.smem)));
+        const SplitKernels k = pick_splits(c->nv_class, c->gt, c->nv_exact);
+        XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.scores.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.scores.smem)));
+        for (const ReadKernel& r : k.read)
+            XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(r.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(r.smem)));
     }
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(account_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kAcctSmemBytes));
     c->read_funcs_ready = true;
+    return XN_OK;
+}
+
+// The stream's page table on the device, at least its first n entries.
+int32_t device_pages(xn_ctx* c, xn_stream* s, size_t n, const int** out) {
+    if (n > s->pages_d_cap) {
+        XN_CUDA(c, cudaStreamSynchronize(c->stream));   // launches in flight may still read the old one
+        XN_CUDA(c, guarded_free(c, s->pages_d));
+        s->pages_d = nullptr;
+        s->pages_d_cap = s->pages_d_valid = 0;
+        const size_t want = align_up(n + n / 2, 64);
+        XN_CUDA(c, guarded_malloc(c, reinterpret_cast<void**>(&s->pages_d), want * 4, "page table"));
+        s->pages_d_cap = want;
+    }
+    if (n > s->pages_d_valid) {
+        // pageable memory: the call returns when the entries have been taken
+        const size_t to = std::min(s->pages.size(), s->pages_d_cap);
+        XN_CUDA(c, cudaMemcpyAsync(s->pages_d + s->pages_d_valid, s->pages.data() + s->pages_d_valid, (to - s->pages_d_valid) * 4,
+                                   cudaMemcpyHostToDevice, c->stream));
+        s->pages_d_valid = to;
+    }
+    *out = s->pages_d;
+    return XN_OK;
+}
+
+// Few rows that all see the same prefix, f32 cache: up to kReadEntries requests per launch, described
+// by the launch parameter alone.
+int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
+    const int Hq = c->num_heads, Hkv = c->num_kv_heads;
+    ReadTable& t = c->read_table;
+    t.n = n;
+    t.subs = c->subs;
+    t.gt = c->gt;
+    t.group = c->group;
+    t.n_tiles = 0;
+    int32_t rc;
+    size_t floats = 0;
+    int max_kv = 0;
+    for (int i = 0; i < n; ++i) {
+        const ReadSub& s = subs[i];
+        ReadEntry& e = t.e[i];
+        e.q = s.q; e.q_hs = s.q_hs; e.q_ts = s.q_ts;
+        e.out = s.out; e.o_hs = s.o_hs; e.o_ts = s.o_ts;
+        if ((rc = device_pages(c, s.stream, size_t((s.kv + kPageTokens - 1) / kPageTokens), &e.pages)) != XN_OK) return rc;
+        e.rows = s.rows; e.kv_len = s.kv; e.layer = s.layer;
+        e.n_tiles = (s.kv + c->tile_tokens - 1) / c->tile_tokens;
+        e.tile0 = t.n_tiles;
+        t.n_tiles += (long long)e.n_tiles * Hkv * c->subs * s.rows;
+        max_kv = std::max(max_kv, s.kv);
+        if (!want) continue;
+        e.user = s.acct.user; e.user_hs = s.acct.user_hs;
+        e.old_from = s.acct.old_from; e.old_len = s.acct.old_len; e.store = s.acct.store;
+        e.sc_ts = (long long)align_up(size_t(s.kv), 4);
+        e.sc_hs = e.sc_ts * s.rows;
+        e.lse_hs = s.rows;
+        floats += size_t(e.sc_hs) * Hq + align_up(size_t(s.rows) * Hq, 4);
+    }
+    if (want) {
+        if ((rc = grow_device(c, &c->read_ws, &c->read_ws_cap, floats)) != XN_OK) return rc;
+        float* at = c->read_ws;
+        for (int i = 0; i < n; ++i) {
+            ReadEntry& e = t.e[i];
+            e.scores = at;
+            at += size_t(e.sc_hs) * Hq;
+            e.lse = at;
+            at += align_up(size_t(e.rows) * Hq, 4);
+        }
+    }
+    t.n_blocks = int(std::min<long long>(t.n_tiles, c->decode_ctas));
+    if ((rc = grow_device(c, &c->partials, &c->partials_cap, size_t(2 * t.n_blocks) * c->gt * part_stride_floats(c->nv))) != XN_OK)
+        return rc;
+    const ReadKernel k = pick_splits(c->nv_class, c->gt, c->nv_exact).read[want ? 1 : 0];
+    if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
+    k.fn<<<t.n_blocks, k.threads, k.smem, c->stream>>>(t, c->k_pool, c->v_pool, c->partials, c->sync_d, c->pool_pages, Hkv,
+                                                       c->head_dim, c->nv, c->scale, c->status_d);
+    XN_CUDA(c, cudaGetLastError());
+    if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
+    c->stats.kernel_launches += 1;
+    c->stats.decode_launches += 1;
+    if (want)
+        XN_CUDA(c, launch_pdl(c, account_table_kernel, dim3(unsigned((max_kv + 255) / 256), unsigned(Hkv), unsigned(n)), 256, 0, true, 0,
+                              t, c->acct_pool, c->pool_pages, Hkv));
     return XN_OK;
 }
 
@@ -401,7 +485,8 @@ int32_t launch_read_few(xn_ctx* c, const std::vector<ReadSub>& subs, bool want) 
                 reqs_d, units_d, items_d, cta_d, sp.ctas, pages_d, c->pool8, c->partials, c->sync_d, c->pool_pages,
                 Hkv, c->head_dim, c->scale * 1.4426950408889634f, c->cos_d, c->sin_d, c->status_d);
         } else {
-            const SplitKernel k = pick_split(c->nv_class, c->gt, c->nv_exact, want);
+            const SplitKernels ks = pick_splits(c->nv_class, c->gt, c->nv_exact);
+            const SplitKernel& k = want ? ks.scores : ks.decode;
             c->pcache.table.n = 0;
             k.fn<<<std::min(sp.ctas, c->decode_ctas), k.threads, k.smem, c->stream>>>(
                 reqs_d, units_d, items_d, cta_d, sp.ctas, pages_d, c->k_pool, c->v_pool, c->partials, c->sync_d,
@@ -603,7 +688,8 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
         if ((rc = grow_io(c, io_in + io_out)) != XN_OK) return rc;
     }
     size_t in_at = 0, out_at = io_in;
-    std::vector<ReadSub> few[2], tc;   // few[1]: with weights
+    // [1]: with weights.  table: few rows that all see the whole prefix; few: the others, and the u8 format
+    std::vector<ReadSub> table[2], few[2], tc;
     struct Zero { float* out; long long o_hs, o_ts; int rows; };
     std::vector<Zero> zeros;
     for (int i = 0; i < n; ++i) {
@@ -656,7 +742,9 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
             continue;
         }
         if (s.causal && r.rows > kv) zeros.push_back({s.out, s.o_hs, s.o_ts, int(r.rows - kv)});
-        few[s.want ? 1 : 0].push_back(s);
+        const bool fits = !s.want || align_up(size_t(kv), 4) * Hq * size_t(r.rows) <= kReadScoreBudget / 4;
+        if (!c->kv_u8 && r.rows > 0 && (!s.causal || r.rows == 1) && fits) table[s.want ? 1 : 0].push_back(s);
+        else few[s.want ? 1 : 0].push_back(s);
     }
     if (host && io_in) {
         XN_CUDA(c, cudaMemcpyAsync(c->io_dev, c->io_host, io_in, cudaMemcpyHostToDevice, c->stream));
@@ -679,7 +767,19 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
         if ((rc = launch_read_tc(c, std::vector<ReadSub>(tc.begin() + long(i), tc.begin() + long(j)))) != XN_OK) return rc;
         i = j;
     }
-    // few rows: all at once without weights; with weights in portions whose scores fit, a request of
+    for (int w = 0; w < 2; ++w)
+        for (size_t i = 0; i < table[w].size();) {
+            // (a launch's scores fit the budget, or it is one request; the rows of one request are few)
+            size_t j = i, floats = 0;
+            for (; j < table[w].size() && j - i < size_t(kReadEntries); ++j) {
+                const size_t f = w ? align_up(size_t(table[w][j].kv), 4) * Hq * size_t(table[w][j].rows) : 0;
+                if (j > i && floats + f > kReadScoreBudget / 4) break;
+                floats += f;
+            }
+            if ((rc = launch_read_table(c, table[w].data() + i, int(j - i), w == 1)) != XN_OK) return rc;
+            i = j;
+        }
+    // the other few rows: all at once without weights; with weights in portions whose scores fit, a request of
     // too many rows (long prompts of head_dim > 128) in several row blocks whose weights add up
     if (!few[0].empty()) {
         std::vector<ReadSub> part;
@@ -829,30 +929,19 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
         }
         if (io && (rc = grow_io(c, io)) != XN_OK) return rc;
     }
+    // Entries of layers with one account length each; a launch takes up to kEvictEntries of them.
     std::vector<EvictDev> ev;
-    std::vector<int32_t> page_ids, acc;
     size_t kept_ws = 0, at = 0;
-    int head0 = 0, longest = 1;
-    int64_t keep_most = 1;
-    bool any_copy = false, any_move = false;
     for (int i = 0; i < n; ++i) {
         const One& o = ones[size_t(i)];
         if (o.len == 0) continue;
         const xn_evict_req& r = reqs[i];
         EvictDev e = {};
-        e.page_off = int(page_ids.size());
-        const size_t np = size_t((o.len + kPageTokens - 1) / kPageTokens);
-        page_ids.insert(page_ids.end(), r.stream->pages.begin(), r.stream->pages.begin() + long(np));
-        e.layer0 = o.l0;
-        e.n_layers = o.nl;
         e.len = int(o.len);
         e.keep = int(o.kept);
         e.recent = int(std::min(r.recent, o.kept));
-        e.head0 = head0;
         e.copy = o.copy ? 1 : (o.move ? 0 : 2);
-        e.kept_ws = reinterpret_cast<int*>(kept_ws);
-        const size_t rows = size_t(o.nl) * Hkv * size_t(o.kept);
-        kept_ws += rows;
+        const size_t per_layer = size_t(Hkv) * size_t(o.kept), rows = per_layer * o.nl;
         if (host) {
             auto take = [&](size_t bytes) { unsigned char* p = c->io_dev + at; at += align_up(bytes, 16); return p; };
             if (r.kept) e.kept = reinterpret_cast<int*>(take(rows * 4));
@@ -868,45 +957,62 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
             e.v_out = r.v_out;
         }
         if (!o.copy && !o.move && !e.kept && !e.w_out) continue;   // nothing to do, nothing to report
-        for (int l = o.l0; l < o.l0 + o.nl; ++l)
-            for (int h = 0; h < Hkv; ++h) acc.push_back(int32_t(std::min(r.stream->acc_len[size_t(l)], o.len)));
-        head0 += o.nl * Hkv;
-        longest = std::max(longest, e.len - e.recent);
-        keep_most = std::max(keep_most, o.kept);
-        any_copy |= o.copy;
-        any_move |= o.move;
-        ev.push_back(e);
+        if ((rc = device_pages(c, r.stream, size_t((o.len + kPageTokens - 1) / kPageTokens), &e.pages)) != XN_OK) return rc;
+        for (int l = o.l0; l < o.l0 + o.nl;) {
+            int m = l + 1;
+            while (m < o.l0 + o.nl && r.stream->acc_len[size_t(m)] == r.stream->acc_len[size_t(l)]) ++m;
+            EvictDev x = e;
+            x.layer0 = l;
+            x.n_layers = m - l;
+            x.acc_len = int(std::min(r.stream->acc_len[size_t(l)], o.len));
+            const size_t skip = size_t(l - o.l0) * per_layer;
+            if (x.kept) x.kept += skip;
+            if (x.w_out) x.w_out += skip;
+            if (x.k_out) x.k_out += skip * D;
+            if (x.v_out) x.v_out += skip * D;
+            x.kept_ws = reinterpret_cast<int*>(kept_ws);   // an offset until the buffer is there
+            kept_ws += size_t(x.n_layers) * per_layer;
+            ev.push_back(x);
+            l = m;
+        }
     }
     if (ev.empty()) return XN_OK;
     if ((rc = grow_device(c, &c->read_ws, &c->read_ws_cap, kept_ws)) != XN_OK) return rc;
-    for (EvictDev& e : ev) e.kept_ws = reinterpret_cast<int*>(c->read_ws) + reinterpret_cast<uintptr_t>(e.kept_ws);
-    PlanBuf b;
-    const size_t o_ev = b.put(ev), o_page = b.put(page_ids), o_acc = b.put(acc);
-    PlanSlot* slot = nullptr;
-    if ((rc = commit_plan(c, b, &slot)) != XN_OK) return rc;
-    const EvictDev* ev_d = reinterpret_cast<const EvictDev*>(slot->dev + o_ev);
-    const int* pages_d = reinterpret_cast<const int*>(slot->dev + o_page);
-    const int* acc_d = reinterpret_cast<const int*>(slot->dev + o_acc);
-    // blocks per (layer, head): 4096 candidates each (a run of 4 per thread) up to 8 blocks, longer
-    // runs beyond that
-    int cluster = 1, run = 4;
-    while (cluster < ev::kMaxCluster && longest > cluster * ev::kThreads * run) cluster *= 2;
-    while (run <= ev::kMaxRun && longest > cluster * ev::kThreads * run) run *= 2;
-    auto select = run == 4 ? evict_select_kernel<4> : run == 8 ? evict_select_kernel<8> : run == 16 ? evict_select_kernel<16>
-                : run == 32 ? evict_select_kernel<32> : evict_select_kernel<0>;
-    XN_CUDA(c, launch_pdl(c, select, dim3(unsigned(head0 * cluster)), ev::kThreads, 0, true, unsigned(cluster), ev_d,
-                          int(ev.size()), pages_d, c->acct_pool, c->pool_pages, Hkv, cluster, acc_d));
     const EvictPools pools = {c->k_pool, c->v_pool, c->pool8, c->acct_pool, c->pool_pages, Hkv, D, c->nv, c->dq};
-    if (any_copy)
-        XN_CUDA(c, launch_pdl(c, evict_copy_kernel<4>, dim3(unsigned(head0), unsigned(std::min<int64_t>((keep_most + 31) / 32, 65535))),
-                              256, 0, true, 0, ev_d, int(ev.size()), pages_d, pools));
-    if (any_move) {
-        const int row_bytes = c->kv_u8 ? c->dq : c->nv * 16;
-        const unsigned slices = unsigned((row_bytes + kMoveSlice - 1) / kMoveSlice);
-        XN_CUDA(c, launch_pdl(c, evict_move_kernel, dim3(unsigned(head0), 2 * slices), kMoveThreads, 0, true, 0, ev_d, int(ev.size()),
-                              pages_d, pools, acc_d));
+    for (size_t i0 = 0; i0 < ev.size(); i0 += kEvictEntries) {
+        EvictTable tab;
+        tab.n = int(std::min<size_t>(kEvictEntries, ev.size() - i0));
+        int head0 = 0, longest = 1, keep_most = 1;
+        bool any_copy = false, any_move = false;
+        for (int i = 0; i < tab.n; ++i) {
+            EvictDev& e = tab.e[i];
+            e = ev[i0 + size_t(i)];
+            e.kept_ws = reinterpret_cast<int*>(c->read_ws) + reinterpret_cast<uintptr_t>(e.kept_ws);
+            e.head0 = head0;
+            head0 += e.n_layers * Hkv;
+            longest = std::max(longest, e.len - e.recent);
+            keep_most = std::max(keep_most, e.keep);
+            any_copy |= e.copy == 1;
+            any_move |= e.copy == 0;
+        }
+        // blocks per (layer, head): 4096 candidates each (a run of 4 per thread) up to 8 blocks, longer
+        // runs beyond that
+        int cluster = 1, run = 4;
+        while (cluster < ev::kMaxCluster && longest > cluster * ev::kThreads * run) cluster *= 2;
+        while (run <= ev::kMaxRun && longest > cluster * ev::kThreads * run) run *= 2;
+        auto select = run == 4 ? evict_select_kernel<4> : run == 8 ? evict_select_kernel<8> : run == 16 ? evict_select_kernel<16>
+                    : run == 32 ? evict_select_kernel<32> : evict_select_kernel<0>;
+        XN_CUDA(c, launch_pdl(c, select, dim3(unsigned(head0 * cluster)), ev::kThreads, 0, true, unsigned(cluster), tab, c->acct_pool,
+                              c->pool_pages, Hkv, cluster));
+        if (any_copy)
+            XN_CUDA(c, launch_pdl(c, evict_copy_kernel<4>, dim3(unsigned(head0), unsigned(std::min((keep_most + 31) / 32, 65535))), 256, 0,
+                                  true, 0, tab, pools));
+        if (any_move) {
+            const int row_bytes = c->kv_u8 ? c->dq : c->nv * 16;
+            const unsigned slices = unsigned((row_bytes + kMoveSlice - 1) / kMoveSlice);
+            XN_CUDA(c, launch_pdl(c, evict_move_kernel, dim3(unsigned(head0), 2 * slices), kMoveThreads, 0, true, 0, tab, pools));
+        }
     }
-    if ((rc = finish_slot(c, slot)) != XN_OK) return rc;
     // the streams shrink: lengths, accounts, and the pages that no layer needs any more (their next
     // owner's launches come behind these on the context's stream)
     for (int i = 0; i < n; ++i) {
@@ -924,6 +1030,7 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
             c->free_pages.push_back(s->pages.back());
             s->pages.pop_back();
         }
+        s->pages_d_valid = std::min(s->pages_d_valid, s->pages.size());
         c->pcache.valid = false;   // the kept plan may name this stream's pages and length
     }
     if (host) {
