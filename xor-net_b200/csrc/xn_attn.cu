@@ -29,6 +29,7 @@
 #include "xn_prefill_f32.cuh"
 #include "xn_prefill_tf32.cuh"
 #include "xn_read.cuh"
+#include "xn_read_small.cuh"
 #include "xn_read_tc.cuh"
 #include "xn_static_decode.cuh"
 #include "xn_ternary.hpp"

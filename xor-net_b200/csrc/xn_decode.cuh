@@ -236,6 +236,7 @@ splitkv_body(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
         mbar_fence_init();
     }
     __syncthreads();
+    if constexpr (READ) pdl_wait();   // launched as a programmatic dependent
 
     if (warp == 0) {
         // =============================== producer ===============================

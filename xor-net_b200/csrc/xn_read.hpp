@@ -354,6 +354,22 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
         e.lse_hs = s.rows;
         floats += size_t(e.sc_hs) * Hq + align_up(size_t(s.rows) * Hq, 4);
     }
+    // Small calls: a cluster per (request, KV head), of as many blocks (of 32 positions or more) as there
+    // are SMs for, if a block's share of the positions is then small.
+    static const int small_max = getenv("XN_SMALL") ? atoi(getenv("XN_SMALL")) : 128;
+    if (c->head_dim <= 128 && n * Hkv <= c->sm_count) {
+        int cluster = 1;
+        while (cluster < ev::kMaxCluster && n * Hkv * cluster * 2 <= c->sm_count && max_kv > cluster * 32) cluster *= 2;
+        if ((max_kv + cluster - 1) / cluster <= std::min(small_max, rs::kMaxTokens)) {
+            if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
+            XN_CUDA(c, launch_pdl(c, read_small_kernel, dim3(unsigned(n * Hkv * cluster)), rs::kThreads, 0, true, unsigned(cluster), t,
+                                  c->k_pool, c->v_pool, c->acct_pool, c->pool_pages, Hkv, c->head_dim, c->nv, c->scale, cluster,
+                                  want ? 1 : 0));
+            if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
+            c->stats.decode_launches += 1;
+            return XN_OK;
+        }
+    }
     if (want) {
         if ((rc = grow_device(c, &c->read_ws, &c->read_ws_cap, floats)) != XN_OK) return rc;
         float* at = c->read_ws;
@@ -370,11 +386,9 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
         return rc;
     const ReadKernel k = pick_splits(c->nv_class, c->gt, c->nv_exact).read[want ? 1 : 0];
     if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
-    k.fn<<<t.n_blocks, k.threads, k.smem, c->stream>>>(t, c->k_pool, c->v_pool, c->partials, c->sync_d, c->pool_pages, Hkv,
-                                                       c->head_dim, c->nv, c->scale, c->status_d);
-    XN_CUDA(c, cudaGetLastError());
+    XN_CUDA(c, launch_pdl(c, k.fn, dim3(unsigned(t.n_blocks)), k.threads, k.smem, true, 0, t, c->k_pool, c->v_pool, c->partials,
+                          c->sync_d, c->pool_pages, Hkv, c->head_dim, c->nv, c->scale, c->status_d));
     if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
-    c->stats.kernel_launches += 1;
     c->stats.decode_launches += 1;
     if (want)
         XN_CUDA(c, launch_pdl(c, account_table_kernel, dim3(unsigned((max_kv + 255) / 256), unsigned(Hkv), unsigned(n)), 256, 0, true, 0,
