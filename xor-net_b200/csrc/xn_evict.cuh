@@ -38,7 +38,7 @@ namespace ev {
 constexpr int kThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxRun = 32;        // candidates a thread can hold
+constexpr int kMaxRun = 32;        // candidates of a thread whose keys are kept on chip
 
 // Floats in the order of unsigned integers; NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -64,6 +64,23 @@ __device__ __forceinline__ uint32_t peer_ld(const void* smem, uint32_t rank) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(smem, rank)) : "memory");
     return v;
+}
+
+__device__ __forceinline__ uint4 peer_ld4u(const void* smem, uint32_t rank) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(peer_addr(smem, rank))
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// The float behind a key; false where a key stands for several (NaNs, zeros).
+__device__ __forceinline__ bool key_value(uint32_t k, float& x) {
+    x = __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+    return k != 0u && k != 0x80000000u;
 }
 
 // Exclusive prefix of v over the block in thread order, and the block's total.
@@ -92,26 +109,25 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* scratch, ui
 
 }  // namespace ev
 
-// One cluster of 1, 2, 4 or 8 blocks per (layer, KV head).  Thread t of block r owns the RUN
-// candidates from (r * 1024 + t) * RUN on, a quarter of a page or so, and keeps their keys in
-// registers (RUN > 0): the account is read from memory once, 16 bytes per load, and thread order is
-// position order.  Radix selection: the threshold key is found 11, 11 and 10 bits at a time from
-// shared-memory histograms that the blocks read from one another; then one scan of the (above,
-// equal) counts gives every thread the place of its first kept position, ties included, and it
-// writes its run.  Bound by the latency of these steps, about 2 microseconds each, not by bandwidth:
-// [8 heads x 131072 positions: 12 us against 93 us for a loop over the slice in shared memory with a
-// ballot and four barriers per 512 positions.]
-// RUN = 0: streams too long for that; the keys are read again in every pass.
-template <int RUN>
+// One cluster of 1, 2, 4 or 8 blocks per (layer, KV head).  Thread t of block r owns the `run`
+// candidates from (r * 1024 + t) * run on -- run is a power of two up to 32, so they share a page --
+// and keeps their keys in its own row of shared memory: the account is read from memory once, 16
+// bytes per load, and thread order is position order.  Radix selection: the threshold key is found
+// 11, 11 and 10 bits at a time from histograms that the blocks read from one another (fewer steps when
+// a bin is kept whole); then one scan of the (above, equal) counts gives every thread the place of its
+// first kept position, ties included, and it writes its run.  Bound by the latency of these steps and
+// by fetching instructions that run once, so the loops are rolled: see the figures in the design notes.
+// Streams too long for that (run = 0) read their keys again in every pass.
 __global__ void __launch_bounds__(ev::kThreads, 1)
 evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restrict__ pool, long long pool_pages,
-                    int num_kv_heads, int cluster) {
+                    int num_kv_heads, int cluster, int run_or_0) {
     using namespace ev;
     pdl_launch_dependents();
-    __shared__ uint32_t hist[2][kBins];             // by pass parity: peers may still read the other one
+    extern __shared__ uint32_t keys_s[];            // [1024][run + 1]
+    __shared__ __align__(16) uint32_t hist[2][kBins];   // by pass parity: peers may still read the other one
     __shared__ uint32_t scratch[32];
     __shared__ uint32_t counts[2];                  // this block's candidates above / at the threshold
-    __shared__ uint32_t found[2];
+    __shared__ uint32_t found[3];
     const int row = int(blockIdx.x) / cluster;
     const uint32_t rank = cluster_rank();
     int rq = 0;
@@ -122,159 +138,164 @@ evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restr
     const int tid = threadIdx.x, lane = tid & 31;
     const int n_cand = r.len - r.recent;
     const int m = r.keep - r.recent;                // candidates to keep, 0 <= m <= n_cand
-    // positions [lo, hi) are this thread's; without RUN a run that covers the stream
-    const int run = RUN > 0 ? RUN : (((n_cand + cluster * kThreads - 1) / (cluster * kThreads)) + 3) / 4 * 4;
-    const long long lo_ll = (long long)(int(rank) * kThreads + tid) * run;
-    const int lo = int(lo_ll < n_cand ? lo_ll : n_cand), hi = min(n_cand, lo + run);
+    // positions [lo, hi) are this thread's
+    const int run = run_or_0 ? run_or_0 : (((n_cand + cluster * kThreads - 1) / (cluster * kThreads)) + 3) / 4 * 4;
+    const int lo = int(min((long long)(int(rank) * kThreads + tid) * run, (long long)n_cand)), hi = min(n_cand, lo + run);
     const int* pages = r.pages;
     const int valid = r.acc_len;
-    const size_t base = (size_t(l) * size_t(pool_pages)) * num_kv_heads * kPageTokens + size_t(h) * kPageTokens;
-    const size_t pstep = size_t(num_kv_heads) * kPageTokens;
+    const float* base = pool + (size_t(l) * size_t(pool_pages) * num_kv_heads + h) * kPageTokens;
+    const int page_step = num_kv_heads * kPageTokens;
     auto load = [&](int j) -> float {
-        return j < valid ? pool[base + size_t(pages[j / kPageTokens]) * pstep + size_t(j % kPageTokens)] : 0.f;
+        return j < valid ? base[(long long)pages[j / kPageTokens] * page_step + j % kPageTokens] : 0.f;
     };
-    // four positions from a multiple of four on: they never leave a page
-    auto load4 = [&](int j) -> float4 {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (j < valid && j < n_cand) {
-            x = *reinterpret_cast<const float4*>(pool + base + size_t(pages[j / kPageTokens]) * pstep + size_t(j % kPageTokens));
-            if (j + 1 >= valid) x.y = 0.f;
-            if (j + 2 >= valid) x.z = 0.f;
-            if (j + 3 >= valid) x.w = 0.f;
-        }
-        return x;
-    };
-    constexpr int R = RUN > 0 ? RUN : 4;
-    uint32_t keys[R];
+    uint32_t* mine = keys_s + tid * (run + 1);
     pdl_wait();
-    if (RUN > 0) {
-        float4 x[R / 4];
-#pragma unroll
-        for (int i = 0; i < R / 4; ++i) x[i] = load4(lo + 4 * i);
-#pragma unroll
-        for (int i = 0; i < R / 4; ++i) {
-            keys[4 * i] = order_key(x[i].x);
-            keys[4 * i + 1] = order_key(x[i].y);
-            keys[4 * i + 2] = order_key(x[i].z);
-            keys[4 * i + 3] = order_key(x[i].w);
+    if (run_or_0) {
+        const float* at = base;
+        if (lo < min(valid, n_cand)) at += (long long)pages[lo / kPageTokens] * page_step + lo % kPageTokens;
+#pragma unroll 1
+        for (int i = 0; i < run; i += 4) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (lo + i < min(valid, n_cand)) x = *reinterpret_cast<const float4*>(at + i);
+            mine[i] = order_key(x.x);
+            mine[i + 1] = order_key(lo + i + 1 < valid ? x.y : 0.f);
+            mine[i + 2] = order_key(lo + i + 2 < valid ? x.z : 0.f);
+            mine[i + 3] = order_key(lo + i + 3 < valid ? x.w : 0.f);
         }
     }
-    // f(j, key) for every candidate of the thread in order, all lanes of a warp together
-    auto each = [&](auto&& f) {
-        if (RUN > 0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) f(lo + i, keys[i], lo + i < hi);
-        } else {
-            for (int i = 0; i < run; ++i) {
-                const int j = lo + i;
-                const bool in = j < hi;
-                f(j, in ? order_key(load(j)) : 0u, in);
-            }
-        }
-    };
+    auto key_at = [&](int i) -> uint32_t { return run_or_0 ? mine[i] : order_key(load(lo + i)); };
 
     uint32_t prefix = 0, mask = 0, left = uint32_t(m);   // the threshold is the left-th largest with this prefix
     const bool all = m == n_cand, none = m == 0;
+    bool whole_bin = false;
     if (!all && !none) {
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass < 2 ? 11 : 10;
+#pragma unroll 1
+        for (int pass = 0; pass < 3 && !whole_bin; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-            const uint32_t bins = 1u << bits;
+            const uint32_t bins = pass < 2 ? 2048u : 1024u;
             uint32_t* hs = hist[pass & 1];
             hs[tid] = 0;
             hs[tid + kThreads] = 0;
             __syncthreads();
-            each([&](int, uint32_t k, bool in_run) {
-                const bool in = in_run && (k & mask) == prefix;
-                const uint32_t bin = (k >> shift) & (bins - 1);
+#pragma unroll 2
+            for (int i = 0; i < run; ++i) {
+                const uint32_t k = lo + i < hi ? key_at(i) : 0u;
+                const bool in = lo + i < hi && (k & mask) == prefix;
+                const uint32_t bin = in ? (k >> shift) & (bins - 1) : kBins;
                 // equal accounts are common (positions never looked at): a warp that agrees adds once
-                const uint32_t act = __ballot_sync(0xffffffffu, in);
-                if (act == 0) return;
-                const int lead = __ffs(act) - 1;
-                const uint32_t b0 = __shfl_sync(0xffffffffu, bin, lead);
-                if (__all_sync(0xffffffffu, !in || bin == b0)) {
-                    if (lane == lead) atomicAdd(&hs[b0], uint32_t(__popc(act)));
-                } else if (in) {
-                    atomicAdd(&hs[bin], 1u);
-                }
-            });
-            // the bin, counted from the top, that holds the left-th largest: a thread sums two bins (one
-            // in the last pass) over the cluster, the highest on the lowest threads
-            const int per = int(bins) / kThreads;
-            const int top = int(bins) - 1 - tid * per;
-            uint32_t a = 0, b = 0;
-            if (cluster > 1) {
-                cluster_sync_all();
+                const bool same = __all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0));
+                if (in && (!same || lane == 0)) atomicAdd(&hs[bin], same ? 32u : 1u);
+            }
+            // the bin, counted from the top, that holds the left-th largest: the first threads sum four bins
+            // each over the cluster, the highest on the lowest threads
+            const int top = int(bins) - 4 - tid * 4;
+            uint4 c = make_uint4(0u, 0u, 0u, 0u);
+            if (cluster > 1) cluster_sync_all();
+            else __syncthreads();
+            if (top >= 0) {
+                if (cluster > 1) {
+                    uint4 x[kMaxCluster];
 #pragma unroll
-                for (int p = 0; p < kMaxCluster; ++p)
-                    if (p < cluster) {
-                        a += peer_ld(&hs[top], uint32_t(p));
-                        if (per == 2) b += peer_ld(&hs[top - 1], uint32_t(p));
+                    for (int p = 0; p < kMaxCluster; ++p) x[p] = p < cluster ? peer_ld4u(&hs[top], uint32_t(p)) : c;
+#pragma unroll
+                    for (int p = 0; p < kMaxCluster; ++p) {
+                        c.x += x[p].x;
+                        c.y += x[p].y;
+                        c.z += x[p].z;
+                        c.w += x[p].w;
                     }
-            } else {
-                __syncthreads();
-                a = hs[top];
-                if (per == 2) b = hs[top - 1];
+                } else {
+                    c = *reinterpret_cast<const uint4*>(&hs[top]);
+                }
             }
             uint32_t total;
-            const uint32_t before = block_scan(a + b, scratch, total);
-            if (before < left && left <= before + a + b) {   // exactly one thread
-                const bool first = left <= before + a;
-                found[0] = uint32_t(first ? top : top - 1);
-                found[1] = left - before - (first ? 0u : a);
+            const uint32_t sum = (c.x + c.y) + (c.z + c.w);
+            const uint32_t before = block_scan(sum, scratch, total);
+            if (before < left && left <= before + sum) {     // exactly one thread
+                uint32_t rest = left - before, bin = uint32_t(top) + 3, n = c.w;
+                if (rest > n) { rest -= n; --bin; n = c.z; if (rest > n) { rest -= n; --bin; n = c.y; if (rest > n) { rest -= n; --bin; n = c.x; } } }
+                found[0] = bin;
+                found[1] = rest;
+                found[2] = rest == n;                        // the whole bin stays: no need to look into it
             }
             __syncthreads();
             prefix |= found[0] << shift;
             mask |= (bins - 1) << shift;
             left = found[1];
+            whole_bin = found[2] != 0;
             __syncthreads();
         }
     }
-    // m == 0 keeps no candidate, m == n_cand keeps all
+    // what a key is: 2 kept, 1 tied at the threshold (the first `left` of those stay), 0 out
+    auto kind = [&](uint32_t k) -> int {
+        if (all) return 2;
+        if (none) return 0;
+        const uint32_t t = k & mask;
+        return t > prefix ? 2 : (t == prefix ? (whole_bin ? 2 : 1) : 0);
+    };
     uint32_t gt = 0, eq = 0;
-    if (all) gt = uint32_t(hi - lo);
-    else if (!none)
-        each([&](int, uint32_t k, bool in) {
-            gt += in && k > prefix;
-            eq += in && k == prefix;
-        });
-    uint32_t gt_all, eq_all;
-    const uint32_t gt_at = block_scan(gt, scratch, gt_all);
-    const uint32_t eq_at = block_scan(eq, scratch, eq_all);
+#pragma unroll 1
+    for (int i = 0; i < hi - lo; ++i) {
+        const int x = kind(key_at(i));
+        gt += x == 2;
+        eq += x == 1;
+    }
+    uint32_t gt_all, eq_all, gt_at, eq_at;
+    if (run_or_0) {            // at most 1024 * 32 of either: both in one scan
+        uint32_t both;
+        const uint32_t at = block_scan(gt | eq << 16, scratch, both);
+        gt_at = at & 0xffffu;
+        eq_at = at >> 16;
+        gt_all = both & 0xffffu;
+        eq_all = both >> 16;
+    } else {
+        gt_at = block_scan(gt, scratch, gt_all);
+        eq_at = block_scan(eq, scratch, eq_all);
+    }
     uint32_t gt_before = 0, eq_before = 0;
     if (cluster > 1) {
         if (tid == 0) {
             counts[0] = gt_all;
             counts[1] = eq_all;
         }
-        __syncthreads();
         cluster_sync_all();
-        for (uint32_t p = 0; p < rank; ++p) {
-            gt_before += peer_ld(&counts[0], p);
-            eq_before += peer_ld(&counts[1], p);
+        if (lane < int(rank)) {
+            gt_before = peer_ld(&counts[0], uint32_t(lane));
+            eq_before = peer_ld(&counts[1], uint32_t(lane));
         }
-        cluster_sync_all();   // no block leaves while another still reads its counts (or histograms)
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+            gt_before += __shfl_xor_sync(0xffffffffu, gt_before, o);
+            eq_before += __shfl_xor_sync(0xffffffffu, eq_before, o);
+        }
+        gt_before = __shfl_sync(0xffffffffu, gt_before, 0);
+        eq_before = __shfl_sync(0xffffffffu, eq_before, 0);
+        cluster_arrive();      // no block leaves while another still reads its counts (or histograms): waited for below
     }
     int* kept = r.kept_ws + size_t(local) * r.keep;
     int* kept_user = r.kept ? r.kept + size_t(local) * r.keep : nullptr;
     float* w_user = r.w_out ? r.w_out + size_t(local) * r.keep : nullptr;
-    auto emit = [&](uint32_t at, int j) {
+    auto emit = [&](uint32_t at, int j, uint32_t key) {
         kept[at] = j;
         if (kept_user) kept_user[at] = j;
-        if (w_user) w_user[at] = load(j);
+        float x;
+        if (w_user) w_user[at] = key_value(key, x) ? x : load(j);
     };
-    if (!none) {
-        // of the equal ones the first `left` (in position order over the whole row) stay
-        uint32_t er = eq_before + eq_at;
-        uint32_t at = gt_before + gt_at + min(er, left);
-        each([&](int j, uint32_t k, bool in) {
-            const bool is_eq = !all && in && k == prefix;
-            if (in && (all || k > prefix || (is_eq && er < left))) emit(at++, j);
-            er += is_eq;
-        });
-    }
+    // of the tied ones the first `left` (in position order over the whole row) stay
+    uint32_t er = eq_before + eq_at;
+    uint32_t at = gt_before + gt_at + min(er, left);
+    if (gt + eq > 0)
+#pragma unroll 1
+        for (int i = 0; i < hi - lo; ++i) {
+            const uint32_t k = key_at(i);
+            const int x = kind(k);
+            if (x == 2 || (x == 1 && er < left)) emit(at++, lo + i, k);
+            er += x == 1;
+        }
     // the last `recent` positions, shared out over the cluster
-    for (int i = int(rank) * kThreads + tid; i < r.recent; i += cluster * kThreads) emit(uint32_t(m + i), n_cand + i);
+#pragma unroll 1
+    for (int i = int(rank) * kThreads + tid; i < r.recent; i += cluster * kThreads) emit(uint32_t(m + i), n_cand + i, 0u);
+    if (cluster > 1) cluster_wait();
 }
 
 // What the row kernels move: f32 rows (row_words = 4 * nv floats, K and V pools) or u8 blocks.

@@ -296,6 +296,8 @@ int32_t ready_read_kernels(xn_ctx* c) {
     }
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(account_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kAcctSmemBytes));
+    XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(ev::kThreads * (ev::kMaxRun + 1) * 4)));
     c->read_funcs_ready = true;
     return XN_OK;
 }
@@ -1014,10 +1016,9 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
         int cluster = 1, run = 4;
         while (cluster < ev::kMaxCluster && longest > cluster * ev::kThreads * run) cluster *= 2;
         while (run <= ev::kMaxRun && longest > cluster * ev::kThreads * run) run *= 2;
-        auto select = run == 4 ? evict_select_kernel<4> : run == 8 ? evict_select_kernel<8> : run == 16 ? evict_select_kernel<16>
-                    : run == 32 ? evict_select_kernel<32> : evict_select_kernel<0>;
-        XN_CUDA(c, launch_pdl(c, select, dim3(unsigned(head0 * cluster)), ev::kThreads, 0, true, unsigned(cluster), tab, c->acct_pool,
-                              c->pool_pages, Hkv, cluster));
+        if (run > ev::kMaxRun) run = 0;
+        XN_CUDA(c, launch_pdl(c, evict_select_kernel, dim3(unsigned(head0 * cluster)), ev::kThreads, size_t(ev::kThreads) * (run + 1) * 4,
+                              true, unsigned(cluster), tab, c->acct_pool, c->pool_pages, Hkv, cluster, run));
         if (any_copy)
             XN_CUDA(c, launch_pdl(c, evict_copy_kernel<4>, dim3(unsigned(head0), unsigned(std::min((keep_most + 31) / 32, 65535))), 256, 0,
                                   true, 0, tab, pools));

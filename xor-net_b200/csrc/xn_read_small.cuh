@@ -32,8 +32,6 @@ __device__ __forceinline__ void peer_st4(const void* smem, uint32_t rank, const 
                  "f"(v.z), "f"(v.w)
                  : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 }  // namespace rs
 
@@ -51,7 +49,7 @@ read_small_kernel(const __grid_constant__ ReadTable tab, const float* __restrict
     __shared__ float own[kHeads][2], share_w[kHeads][ev::kMaxCluster];
     __shared__ float acc_s[kMaxTokens];
     pdl_launch_dependents();
-    if (cluster > 1) cluster_arrive();   // waited for before the first remote store: the peers must have started
+    if (cluster > 1) ev::cluster_arrive();   // waited for before the first remote store: the peers must have started
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const int sub = lane & 15, grp = lane >> 4;                   // sixteen lanes share a key
     const int rank = int(ev::cluster_rank());
@@ -196,7 +194,7 @@ read_small_kernel(const __grid_constant__ ReadTable tab, const float* __restrict
                     own[w][1] = l;
                 }
             }
-            if (cluster > 1 && pass == 0) cluster_wait();
+            if (cluster > 1 && pass == 0) ev::cluster_wait();
             __syncthreads();
             if (tid < cluster * kHeads) {   // the softmax state to every block, this one included
                 const int p = tid / kHeads, hh = tid % kHeads;
@@ -239,8 +237,8 @@ read_small_kernel(const __grid_constant__ ReadTable tab, const float* __restrict
                 else part[par][at] = s;
             }
             if (cluster > 1) {
-                cluster_arrive();
-                cluster_wait();
+                ev::cluster_arrive();
+                ev::cluster_wait();
             } else {
                 __syncthreads();
             }
