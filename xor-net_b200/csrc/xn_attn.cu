@@ -29,6 +29,7 @@
 #include "xn_prefill_f32.cuh"
 #include "xn_prefill_tf32.cuh"
 #include "xn_read.cuh"
+#include "xn_read_mid.cuh"
 #include "xn_read_small.cuh"
 #include "xn_read_tc.cuh"
 #include "xn_static_decode.cuh"
@@ -234,7 +235,9 @@ struct xn_ctx {
     float* read_ws = nullptr; size_t read_ws_cap = 0;      // floats: operand images, scores, partial records
     float* acct_pool = nullptr;                            // account of attention weight, paged like K and V
                                                            // (allocated by the first call that keeps one)
-    int read_tc_min_rows = 24;    // packed rows (rows x heads of a group) from which the tensor cores take a read
+    int read_mid_min_rows = 5;    // packed rows (rows x heads of a group) from which the mid kernel takes a read
+    int read_tc_min_rows = 65;    // ... from which the tcgen05 passes take it
+    CUtensorMap v_map_rows;       // the V pool like k_map (128-byte swizzle of 16-byte chunks), for the mid kernel
     bool read_funcs_ready = false;
     ReadTable read_table;         // the launch parameter of a read, filled in place
     // attention output block (sub-norm + ternary o_proj)
@@ -1870,6 +1873,7 @@ int32_t xn_ctx_create(const xn_ctx_desc* d, xn_ctx** out_ctx) {
     if (const char* env = getenv("XORNET_ATTN_OUTPROJ_ROWS")) c->out_rows_kernel = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_PREFILL_PDL")) c->pf_pdl = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_READ_TC_MIN_ROWS")) c->read_tc_min_rows = std::max(1, atoi(env));
+    if (const char* env = getenv("XORNET_ATTN_READ_MID_MIN_ROWS")) c->read_mid_min_rows = std::max(1, atoi(env));
     if (const char* env = getenv("XORNET_ATTN_F32_TILED")) c->f32_tiled = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_F32_TILED_MIN_ROWS")) c->f32_tiled_min_rows = std::max(1, atoi(env));
 
@@ -1975,7 +1979,8 @@ int32_t xn_ctx_create(const xn_ctx_desc* d, xn_ctx** out_ctx) {
             c->tf32_ok = make_map_f32(&c->k_map, c->k_pool, 2, dims, str, box) &&
                          // V is consumed MN-major: 32-byte-chunk swizzle
                          make_map_f32(&c->v_map, c->v_pool, 2, dims, str, box,
-                                      CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
+                                      CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B) &&
+                         make_map_f32(&c->v_map_rows, c->v_pool, 2, dims, str, box);
             if (c->tf32_ok) {
                 XN_CREATE_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(prefill_tf32_kernel<false>),
                                                     cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -97,6 +97,8 @@ struct ReadEntry {
     int n_tiles;              // of one unit
     int rows, kv_len, layer;
     int old_from, old_len, store;   // of the account: see AccountDev
+    int causal;               // row t sees positions up to kv_len - rows + t; else all
+    int n_rt;                 // row tiles of packed query rows per KV head (read_mid_kernel only)
     int pad;
 };
 struct ReadTable {

@@ -38,6 +38,7 @@ namespace ev {
 constexpr int kThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
+constexpr int kCountMax = 512;     // candidates that are ranked by counting
 constexpr int kMaxRun = 32;        // candidates of a thread whose keys are kept on chip
 
 // Floats in the order of unsigned integers; NaN lowest, -0 equal to +0.
@@ -123,7 +124,7 @@ evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restr
                     int num_kv_heads, int cluster, int run_or_0) {
     using namespace ev;
     pdl_launch_dependents();
-    extern __shared__ uint32_t keys_s[];            // [1024][run + 1]
+    extern __shared__ __align__(16) uint32_t keys_s[];   // [1024][run + 1]
     __shared__ __align__(16) uint32_t hist[2][kBins];   // by pass parity: peers may still read the other one
     __shared__ uint32_t scratch[32];
     __shared__ uint32_t counts[2];                  // this block's candidates above / at the threshold
@@ -150,6 +151,45 @@ evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restr
     };
     uint32_t* mine = keys_s + tid * (run + 1);
     pdl_wait();
+    int* kept = r.kept_ws + size_t(local) * r.keep;
+    int* kept_user = r.kept ? r.kept + size_t(local) * r.keep : nullptr;
+    float* w_user = r.w_out ? r.w_out + size_t(local) * r.keep : nullptr;
+    auto emit = [&](uint32_t at, int j, uint32_t key) {
+        kept[at] = j;
+        if (kept_user) kept_user[at] = j;
+        float x;
+        if (w_user) w_user[at] = key_value(key, x) ? x : load(j);
+    };
+    if (n_cand <= kCountMax) {   // (one block then)
+        // Few candidates: thread j counts those that go before candidate j -- a third of the radix passes'
+        // time at 300 of them, as much at 1000.
+        if (rank != 0) return;   // (a cluster that another row's length asked for)
+        const uint32_t k = tid < n_cand ? order_key(load(tid)) : 0u;
+        if (tid < kCountMax) keys_s[tid] = k;
+        __syncthreads();
+        int before = 0;
+        if (tid < n_cand) {
+            int j = 0;
+#pragma unroll 2
+            for (; j + 4 <= tid; j += 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(&keys_s[j]);
+                before += (x.x >= k) + (x.y >= k) + (x.z >= k) + (x.w >= k);
+            }
+            for (; j < tid; ++j) before += keys_s[j] >= k;
+            for (; j < n_cand && (j & 3); ++j) before += keys_s[j] > k;
+#pragma unroll 2
+            for (; j < n_cand; j += 4) {   // (keys behind the last candidate are 0: above nothing)
+                const uint4 x = *reinterpret_cast<const uint4*>(&keys_s[j]);
+                before += (x.x > k) + (x.y > k) + (x.z > k) + (x.w > k);
+            }
+        }
+        const bool stays = tid < n_cand && before < m;
+        uint32_t total;
+        const uint32_t at = block_scan(stays ? 1u : 0u, scratch, total);
+        if (stays) emit(at, tid, k);
+        for (int i = tid; i < r.recent; i += kThreads) emit(uint32_t(m + i), n_cand + i, 0u);
+        return;
+    }
     if (run_or_0) {
         const float* at = base;
         if (lo < min(valid, n_cand)) at += (long long)pages[lo / kPageTokens] * page_step + lo % kPageTokens;
@@ -181,6 +221,7 @@ evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restr
             for (int i = 0; i < run; ++i) {
                 const uint32_t k = lo + i < hi ? key_at(i) : 0u;
                 const bool in = lo + i < hi && (k & mask) == prefix;
+                if (pass > 0 && !__any_sync(0xffffffffu, in)) continue;
                 const uint32_t bin = in ? (k >> shift) & (bins - 1) : kBins;
                 // equal accounts are common (positions never looked at): a warp that agrees adds once
                 const bool same = __all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0));
@@ -272,15 +313,6 @@ evict_select_kernel(const __grid_constant__ EvictTable tab, const float* __restr
         eq_before = __shfl_sync(0xffffffffu, eq_before, 0);
         cluster_arrive();      // no block leaves while another still reads its counts (or histograms): waited for below
     }
-    int* kept = r.kept_ws + size_t(local) * r.keep;
-    int* kept_user = r.kept ? r.kept + size_t(local) * r.keep : nullptr;
-    float* w_user = r.w_out ? r.w_out + size_t(local) * r.keep : nullptr;
-    auto emit = [&](uint32_t at, int j, uint32_t key) {
-        kept[at] = j;
-        if (kept_user) kept_user[at] = j;
-        float x;
-        if (w_user) w_user[at] = key_value(key, x) ? x : load(j);
-    };
     // of the tied ones the first `left` (in position order over the whole row) stay
     uint32_t er = eq_before + eq_at;
     uint32_t at = gt_before + gt_at + min(er, left);

@@ -89,7 +89,8 @@ account_table_kernel(const __grid_constant__ ReadTable tab, float* __restrict__ 
     const int key = int(blockIdx.x) * 256 + int(threadIdx.x);
     if (key >= e.kv_len) return;
     const FewAccount r = {{e.user, e.user_hs, e.old_from, e.old_len, e.store, e.kv_len, 0, e.layer},
-                          e.scores, e.lse, e.sc_hs, e.sc_ts, e.lse_hs, e.rows, e.kv_len, 0};
+                          e.scores, e.lse, e.sc_hs, e.sc_ts, e.lse_hs, e.rows,
+                          e.causal ? e.kv_len - e.rows + 1 : e.kv_len, e.causal};
     pdl_wait();
     account_store(r.a, e.pages, pool, pool_pages, num_kv_heads, blockIdx.y, key, account_sum(r, blockIdx.y, tab.group, key));
 }

@@ -286,11 +286,18 @@ CacheView cache_view(const xn_ctx* c) {
     return {c->k_pool, c->v_pool, c->pool8, c->pool_pages, c->num_kv_heads, c->head_dim, c->nv, c->dq};
 }
 
+using MidFn = void (*)(const ReadTable, const CUtensorMap, const CUtensorMap, float*, int*, long long, int, int, int, float, int, int*);
+MidFn pick_mid(int mt) {
+    return mt == 1 ? read_mid_kernel<1> : mt == 2 ? read_mid_kernel<2> : mt == 3 ? read_mid_kernel<3> : read_mid_kernel<4>;
+}
+
 int32_t ready_read_kernels(xn_ctx* c) {
     if (c->read_funcs_ready) return XN_OK;
     if (!c->kv_u8) {
         const SplitKernels k = pick_splits(c->nv_class, c->gt, c->nv_exact);
         XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(k.scores.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.scores.smem)));
+        for (int mt = 1; mt <= 4 && c->tf32_ok; ++mt)
+            XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(pick_mid(mt)), cudaFuncAttributeMaxDynamicSharedMemorySize, int(rm::smem_bytes(mt))));
         for (const ReadKernel& r : k.read)
             XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(r.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(r.smem)));
     }
@@ -324,9 +331,10 @@ int32_t device_pages(xn_ctx* c, xn_stream* s, size_t n, const int** out) {
     return XN_OK;
 }
 
-// Few rows that all see the same prefix, f32 cache: up to kReadEntries requests per launch, described
-// by the launch parameter alone.
-int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
+// f32 cache, up to kReadEntries requests per launch, described by the launch parameter alone.  mt = 0:
+// few rows that all see the same prefix (the small kernel, or the split-KV kernel over a table); else the
+// mid kernel with mt * 16 packed rows per unit.
+int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int mt) {
     const int Hq = c->num_heads, Hkv = c->num_kv_heads;
     ReadTable& t = c->read_table;
     t.n = n;
@@ -344,9 +352,12 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
         e.out = s.out; e.o_hs = s.o_hs; e.o_ts = s.o_ts;
         if ((rc = device_pages(c, s.stream, size_t((s.kv + kPageTokens - 1) / kPageTokens), &e.pages)) != XN_OK) return rc;
         e.rows = s.rows; e.kv_len = s.kv; e.layer = s.layer;
-        e.n_tiles = (s.kv + c->tile_tokens - 1) / c->tile_tokens;
+        const int tile = mt ? kPageTokens : c->tile_tokens;
+        e.n_tiles = (s.kv + tile - 1) / tile;
+        e.causal = s.causal && s.rows > 1 ? 1 : 0;
+        e.n_rt = mt ? (s.rows * c->group + 16 * mt - 1) / (16 * mt) : 1;
         e.tile0 = t.n_tiles;
-        t.n_tiles += (long long)e.n_tiles * Hkv * c->subs * s.rows;
+        t.n_tiles += (long long)e.n_tiles * Hkv * (mt ? e.n_rt : c->subs * s.rows);
         max_kv = std::max(max_kv, s.kv);
         if (!want) continue;
         e.user = s.acct.user; e.user_hs = s.acct.user_hs;
@@ -359,7 +370,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
     // Small calls: a cluster per (request, KV head), of as many blocks (of 32 positions or more) as there
     // are SMs for, if a block's share of the positions is then small.
     static const int small_max = getenv("XN_SMALL") ? atoi(getenv("XN_SMALL")) : 128;
-    if (c->head_dim <= 128 && n * Hkv <= c->sm_count) {
+    if (mt == 0 && c->head_dim <= 128 && n * Hkv <= c->sm_count) {
         int cluster = 1;
         while (cluster < ev::kMaxCluster && n * Hkv * cluster * 2 <= c->sm_count && max_kv > cluster * 32) cluster *= 2;
         if ((max_kv + cluster - 1) / cluster <= std::min(small_max, rs::kMaxTokens)) {
@@ -383,13 +394,19 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want) {
             at += align_up(size_t(e.rows) * Hq, 4);
         }
     }
-    t.n_blocks = int(std::min<long long>(t.n_tiles, c->decode_ctas));
-    if ((rc = grow_device(c, &c->partials, &c->partials_cap, size_t(2 * t.n_blocks) * c->gt * part_stride_floats(c->nv))) != XN_OK)
-        return rc;
-    const ReadKernel k = pick_splits(c->nv_class, c->gt, c->nv_exact).read[want ? 1 : 0];
+    t.n_blocks = int(std::min<long long>(t.n_tiles, mt ? c->sm_count : c->decode_ctas));
+    const size_t part = mt ? rm::part_floats(mt, c->nv * 4) : c->gt * part_stride_floats(c->nv);
+    if ((rc = grow_device(c, &c->partials, &c->partials_cap, size_t(2 * t.n_blocks) * part)) != XN_OK) return rc;
     if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
-    XN_CUDA(c, launch_pdl(c, k.fn, dim3(unsigned(t.n_blocks)), k.threads, k.smem, true, 0, t, c->k_pool, c->v_pool, c->partials,
-                          c->sync_d, c->pool_pages, Hkv, c->head_dim, c->nv, c->scale, c->status_d));
+    if (mt) {
+        XN_CUDA(c, launch_pdl(c, pick_mid(mt), dim3(unsigned(t.n_blocks)), rm::kThreads, rm::smem_bytes(mt), true, 0, t, c->k_map,
+                              c->v_map_rows, c->partials, c->sync_d, c->pool_pages, Hkv, c->head_dim, c->nv,
+                              c->scale * 1.4426950408889634f, want ? 1 : 0, c->status_d));
+    } else {
+        const ReadKernel k = pick_splits(c->nv_class, c->gt, c->nv_exact).read[want ? 1 : 0];
+        XN_CUDA(c, launch_pdl(c, k.fn, dim3(unsigned(t.n_blocks)), k.threads, k.smem, true, 0, t, c->k_pool, c->v_pool, c->partials,
+                              c->sync_d, c->pool_pages, Hkv, c->head_dim, c->nv, c->scale, c->status_d));
+    }
     if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
     c->stats.decode_launches += 1;
     if (want)
@@ -705,7 +722,8 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
     }
     size_t in_at = 0, out_at = io_in;
     // [1]: with weights.  table: few rows that all see the whole prefix; few: the others, and the u8 format
-    std::vector<ReadSub> table[2], few[2], tc;
+    // mid: the mid kernel's
+    std::vector<ReadSub> table[2], mid[2], few[2], tc;
     struct Zero { float* out; long long o_hs, o_ts; int rows; };
     std::vector<Zero> zeros;
     for (int i = 0; i < n; ++i) {
@@ -757,9 +775,11 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
             tc.push_back(s);
             continue;
         }
-        if (s.causal && r.rows > kv) zeros.push_back({s.out, s.o_hs, s.o_ts, int(r.rows - kv)});
         const bool fits = !s.want || align_up(size_t(kv), 4) * Hq * size_t(r.rows) <= kReadScoreBudget / 4;
-        if (!c->kv_u8 && r.rows > 0 && (!s.causal || r.rows == 1) && fits) table[s.want ? 1 : 0].push_back(s);
+        const bool use_mid = c->tf32_ok && !c->kv_u8 && r.rows > 0 && (long long)r.rows * c->group >= c->read_mid_min_rows && fits;
+        if (!use_mid && s.causal && r.rows > kv) zeros.push_back({s.out, s.o_hs, s.o_ts, int(r.rows - kv)});
+        if (use_mid) mid[s.want ? 1 : 0].push_back(s);
+        else if (!c->kv_u8 && r.rows > 0 && (!s.causal || r.rows == 1) && fits) table[s.want ? 1 : 0].push_back(s);
         else few[s.want ? 1 : 0].push_back(s);
     }
     if (host && io_in) {
@@ -783,18 +803,24 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
         if ((rc = launch_read_tc(c, std::vector<ReadSub>(tc.begin() + long(i), tc.begin() + long(j)))) != XN_OK) return rc;
         i = j;
     }
-    for (int w = 0; w < 2; ++w)
-        for (size_t i = 0; i < table[w].size();) {
-            // (a launch's scores fit the budget, or it is one request; the rows of one request are few)
+    for (int w = 0; w < 4; ++w) {
+        const std::vector<ReadSub>& list = w < 2 ? table[w] : mid[w - 2];
+        const bool want = w & 1;
+        for (size_t i = 0; i < list.size();) {
+            // (a launch's scores fit the budget, or it is one request)
             size_t j = i, floats = 0;
-            for (; j < table[w].size() && j - i < size_t(kReadEntries); ++j) {
-                const size_t f = w ? align_up(size_t(table[w][j].kv), 4) * Hq * size_t(table[w][j].rows) : 0;
+            long long most = 1;
+            for (; j < list.size() && j - i < size_t(kReadEntries); ++j) {
+                const size_t f = want ? align_up(size_t(list[j].kv), 4) * Hq * size_t(list[j].rows) : 0;
                 if (j > i && floats + f > kReadScoreBudget / 4) break;
                 floats += f;
+                most = std::max(most, (long long)list[j].rows * c->group);
             }
-            if ((rc = launch_read_table(c, table[w].data() + i, int(j - i), w == 1)) != XN_OK) return rc;
+            const int mt = w < 2 ? 0 : int(std::min<long long>(4, (most + 15) / 16));
+            if ((rc = launch_read_table(c, list.data() + i, int(j - i), want, mt)) != XN_OK) return rc;
             i = j;
         }
+    }
     // the other few rows: all at once without weights; with weights in portions whose scores fit, a request of
     // too many rows (long prompts of head_dim > 128) in several row blocks whose weights add up
     if (!few[0].empty()) {
