@@ -47,11 +47,10 @@ def plain(q, k, v, causal=False):
 
 
 def context(monkeypatch, path, *args, **kw):
-    """path: "few", "mid", "tc" and "fused" force the f32 kernels, the warp-MMA one, and the tcgen05 kernel with
-    images made before it or in it (where the shape allows them), "auto" leaves the choice."""
+    """path: "few", "mid" and "tc" force the f32 kernels, the warp-MMA one and the tcgen05 passes (where the
+    shape allows them), "auto" leaves the choice."""
     if path != "auto":
-        monkeypatch.setenv("XORNET_ATTN_READ_TC_MIN_ROWS", "1" if path in ("tc", "fused") else "1000000000")
-        monkeypatch.setenv("XORNET_ATTN_READ_FUSED_MAX_ROWS", "128" if path == "fused" else "0")
+        monkeypatch.setenv("XORNET_ATTN_READ_TC_MIN_ROWS", "1" if path == "tc" else "1000000000")
         monkeypatch.setenv("XORNET_ATTN_READ_MID_MIN_ROWS", "1" if path == "mid" else "1000000000")
     return xn.Context(*args, **kw)
 
@@ -68,7 +67,7 @@ def filled(ctx, rng, n, layer=0, cap=None):
     return st, k, v
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("Hq,Hkv,D", [(20, 5, 128), (4, 4, 64), (6, 2, 100), (5, 1, 33), (8, 2, 8), (16, 2, 80), (3, 1, 1)])
 def test_write_and_read_shapes(monkeypatch, path, Hq, Hkv, D):
     rng = np.random.default_rng(D + Hq)
@@ -104,7 +103,7 @@ def test_long_rows_of_the_cache(D):
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("n,R", [(1, 1), (64, 64), (70, 3), (129, 129), (200, 40), (40, 90), (1, 130), (300, 257)])
 def test_causal_rows_and_rows_that_see_nothing(monkeypatch, path, n, R):
     rng = np.random.default_rng(n * 1000 + R)
@@ -122,7 +121,7 @@ def test_causal_rows_and_rows_that_see_nothing(monkeypatch, path, n, R):
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_batches_share_streams_mix_lengths_and_leave_neighbours_alone(monkeypatch, path):
     import torch
 
@@ -171,7 +170,7 @@ def test_batches_share_streams_mix_lengths_and_leave_neighbours_alone(monkeypatc
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_account_adds_up_is_set_and_follows_writes(monkeypatch, path):
     rng = np.random.default_rng(8)
     Hq, Hkv, D, n = 6, 3, 64, 150
@@ -261,7 +260,7 @@ def test_u8_weights_need_a_head_dim_the_tensor_cores_take():
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_values_over_many_orders_of_magnitude(monkeypatch, path):
     """K, V and Q rows of very different sizes (a page's largest element sets its scale), zero rows."""
     rng = np.random.default_rng(17)
@@ -289,7 +288,7 @@ def test_values_over_many_orders_of_magnitude(monkeypatch, path):
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 def test_infinities_and_nan_stay_where_they_are_seen(monkeypatch, path, value):
     rng = np.random.default_rng(4)
@@ -647,7 +646,7 @@ def test_calls_are_refused_inside_a_capture_and_work_after_it():
     ctx.close()
 
 
-@pytest.mark.parametrize("path", ["few", "mid", "tc", "fused"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_same_bits_every_time_and_work_of_two_threads(monkeypatch, path):
     import threading
 

@@ -301,8 +301,7 @@ int32_t ready_read_kernels(xn_ctx* c) {
         for (const ReadKernel& r : k.read)
             XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(r.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, int(r.smem)));
     }
-    XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel<false>), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
-    XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel<true>), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
+    XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(read_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kSmemBytes));
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(account_tc_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, rt::kAcctSmemBytes));
     XN_CUDA(c, cudaFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     int(ev::kThreads * (ev::kMaxRun + 1) * 4)));
@@ -568,8 +567,7 @@ int read_piece_tiles(const std::vector<int>& tiles, int sms) {
 }
 
 // Many rows: the tensor-core passes of xn_read_tc.cuh.
-// fused: every request has one row tile per KV head, and the attention kernel converts the cache itself.
-int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs, bool fused) {
+int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     const int Hkv = c->num_kv_heads, D = c->head_dim, G = c->group;
     std::vector<TcReq> reqs(subs.size());
     std::vector<int32_t> page_ids;
@@ -638,9 +636,8 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs, bool fused) 
         return fail(c, XN_ERR_CAPACITY, "%lld pages and row tiles in one submission are too many", n_img + n_qimg);
 
     // workspace: page images | query images | page factors | row factors | partial records
-    const bool images = !fused || want;
-    const size_t img_b = images ? size_t(n_img) * rt::page_image_bytes(D) : 0, q_b = images ? size_t(n_qimg) * rt::q_image_bytes(D) : 0;
-    const size_t meta_b = images ? align_up(size_t(n_img) * sizeof(PageMeta), 256) : 0, row_b = size_t(n_qimg) * rt::kBM * sizeof(float2);
+    const size_t img_b = size_t(n_img) * rt::page_image_bytes(D), q_b = size_t(n_qimg) * rt::q_image_bytes(D);
+    const size_t meta_b = align_up(size_t(n_img) * sizeof(PageMeta), 256), row_b = size_t(n_qimg) * rt::kBM * sizeof(float2);
     const size_t part_b = size_t(n_parts) * rt::part_floats(c->nv * 4) * 4;
     int32_t rc = grow_device(c, &c->read_ws, &c->read_ws_cap, (img_b + q_b + meta_b + row_b + part_b) / 4 + 64);
     if (rc != XN_OK) return rc;
@@ -660,10 +657,9 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs, bool fused) 
     const CacheView view = cache_view(c);
     const float scale_log2 = c->scale * 1.4426950408889634f;
     if (c->profile && (rc = profile_begin(c, 1)) != XN_OK) return rc;
-    if (!fused)
     XN_CUDA(c, launch_pdl(c, page_images_kernel, dim3(unsigned(n_img + n_qimg)), 256, 0, true, 0, reqs_d, int(subs.size()), n_img,
                           pages_d, view, img, meta, qimg, row_meta, scale_log2, G));
-    XN_CUDA(c, launch_pdl(c, fused ? read_tc_kernel<true> : read_tc_kernel<false>, dim3(unsigned(items.size())), rt::kThreads, size_t(rt::kSmemBytes), true, 0, reqs_d,
+    XN_CUDA(c, launch_pdl(c, read_tc_kernel, dim3(unsigned(items.size())), rt::kThreads, size_t(rt::kSmemBytes), true, 0, reqs_d,
                           reinterpret_cast<const TcItem*>(slot->dev + o_item), pages_d, view, img, meta, qimg, row_meta,
                           parts, scale_log2, G, want ? 1 : 0, c->status_d));
     if (!merges.empty())
@@ -727,8 +723,7 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
     size_t in_at = 0, out_at = io_in;
     // [1]: with weights.  table: few rows that all see the whole prefix; few: the others, and the u8 format
     // mid: the mid kernel's
-    // mid: the mid kernel's; tc[1]: one row tile per KV head, converted in the kernel
-    std::vector<ReadSub> table[2], mid[2], few[2], tc[2];
+    std::vector<ReadSub> table[2], mid[2], few[2], tc;
     struct Zero { float* out; long long o_hs, o_ts; int rows; };
     std::vector<Zero> zeros;
     for (int i = 0; i < n; ++i) {
@@ -777,7 +772,7 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
         const bool use_tc = D <= 128 && r.rows > 0 &&
                             ((long long)r.rows * c->group >= c->read_tc_min_rows || (c->kv_u8 && s.want));
         if (use_tc) {
-            tc[(long long)r.rows * c->group <= c->read_fused_max_rows ? 1 : 0].push_back(s);
+            tc.push_back(s);
             continue;
         }
         const bool fits = !s.want || align_up(size_t(kv), 4) * Hq * size_t(r.rows) <= kReadScoreBudget / 4;
@@ -797,19 +792,16 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
             z.out, z.o_hs, z.o_ts, Hq, z.rows, D);
         c->stats.kernel_launches += 1;
     }
-    for (int f = 0; f < 2; ++f) {
-        const std::vector<ReadSub>& list = tc[f];
-        for (size_t i = 0; i < list.size();) {
-            size_t bytes = 0, j = i;
-            for (; j < list.size(); ++j) {
-                const size_t b = size_t((list[j].kv + kPageTokens - 1) / kPageTokens) * Hkv * rt::page_image_bytes(D) +
-                                 (size_t(list[j].rows) * c->group / rt::kBM + 1) * Hkv * rt::q_image_bytes(D);
-                if (j > i && bytes + b > kReadImageBudget) break;
-                bytes += b;
-            }
-            if ((rc = launch_read_tc(c, std::vector<ReadSub>(list.begin() + long(i), list.begin() + long(j)), f == 1)) != XN_OK) return rc;
-            i = j;
+    for (size_t i = 0; i < tc.size();) {
+        size_t bytes = 0, j = i;
+        for (; j < tc.size(); ++j) {
+            const size_t b = size_t((tc[j].kv + kPageTokens - 1) / kPageTokens) * Hkv * rt::page_image_bytes(D) +
+                             (size_t(tc[j].rows) * c->group / rt::kBM + 1) * Hkv * rt::q_image_bytes(D);
+            if (j > i && bytes + b > kReadImageBudget) break;
+            bytes += b;
         }
+        if ((rc = launch_read_tc(c, std::vector<ReadSub>(tc.begin() + long(i), tc.begin() + long(j)))) != XN_OK) return rc;
+        i = j;
     }
     for (int w = 0; w < 4; ++w) {
         const std::vector<ReadSub>& list = w < 2 ? table[w] : mid[w - 2];

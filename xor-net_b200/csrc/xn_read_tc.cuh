@@ -192,43 +192,6 @@ __device__ __forceinline__ void store_row_image(unsigned char* hi_img, unsigned 
     *reinterpret_cast<uint2*>(lo_img + at) = lo;
 }
 
-// Four columns (4 * lane ..) of token tk of a cache block, zeros past the row's end.
-__device__ __forceinline__ float4 cache_row4(const CacheView& c, size_t blk, int tk, int lane, bool v) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c.u8) {
-        const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
-        if (lane * 4 < c.dq) {
-            const float s = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq)[(v ? kPage : 0) + tk];
-            const uchar4 u = *reinterpret_cast<const uchar4*>(b + size_t((v ? kPage : 0) + tk) * c.dq + lane * 4);
-            // (bytes past head_dim hold 128, but 0 * s is NaN for an infinite scale)
-            if (lane * 4 + 0 < c.head_dim) x.x = (float(u.x) - 128.0f) * s;
-            if (lane * 4 + 1 < c.head_dim) x.y = (float(u.y) - 128.0f) * s;
-            if (lane * 4 + 2 < c.head_dim) x.z = (float(u.z) - 128.0f) * s;
-            if (lane * 4 + 3 < c.head_dim) x.w = (float(u.w) - 128.0f) * s;
-        }
-    } else if (lane < c.nv) {   // rows are padded with zeros to whole float4
-        x = *reinterpret_cast<const float4*>((v ? c.v : c.k) + (blk * kPage + tk) * size_t(c.nv) * 4 + size_t(lane) * 4);
-    }
-    return x;
-}
-
-// Four columns of a packed query row (row p of a KV head's group), zeros past the end.
-__device__ __forceinline__ float4 query_row4(const TcReq& r, int head, int group, int p, int lane, int D, bool vec) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int d = lane * 4;
-    if (p >= r.rows * group || d >= D) return x;
-    const float* row = r.q + (long long)(head * group + p % group) * r.q_hs + (long long)(p / group) * r.q_ts + d;
-    if (vec) return *reinterpret_cast<const float4*>(row);
-    x.x = row[0];
-    if (d + 1 < D) x.y = row[1];
-    if (d + 2 < D) x.z = row[2];
-    if (d + 3 < D) x.w = row[3];
-    return x;
-}
-__device__ __forceinline__ bool query_vec(const TcReq& r, int D) {
-    return (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
-}
-
 // One element of a cached row, whatever the format (rare paths only).
 __device__ __forceinline__ float cache_elem(const CacheView& c, const int* pages, int layer, int head, int key, int d, bool v) {
     const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
@@ -268,13 +231,36 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
         const int ntok = min(kPage, r.kv_len - page * kPage);
         const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_ids[r.page_off + page])) * c.num_kv_heads + h;
         float4 x[2][8];
+        if (c.u8) {
+            const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
+            const float* sc = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int tk = warp * 8 + i;
-            x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (tk < ntok) {
-                x[0][i] = cache_row4(c, blk, tk, lane, false);
-                x[1][i] = cache_row4(c, blk, tk, lane, true);
+            for (int i = 0; i < 8; ++i) {
+                const int tk = warp * 8 + i;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    x[kv][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (tk < ntok && lane * 4 < c.dq) {
+                        const uchar4 u = *reinterpret_cast<const uchar4*>(b + size_t(kv * kPage + tk) * c.dq + lane * 4);
+                        const float s = sc[kv * kPage + tk];
+                        // (bytes past head_dim hold 128, but 0 * s is NaN for an infinite scale)
+                        if (lane * 4 + 0 < D) x[kv][i].x = (float(u.x) - 128.0f) * s;
+                        if (lane * 4 + 1 < D) x[kv][i].y = (float(u.y) - 128.0f) * s;
+                        if (lane * 4 + 2 < D) x[kv][i].z = (float(u.z) - 128.0f) * s;
+                        if (lane * 4 + 3 < D) x[kv][i].w = (float(u.w) - 128.0f) * s;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int tk = warp * 8 + i;
+                x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (tk < ntok && lane < c.nv) {   // rows are padded with zeros to whole float4
+                    const size_t at = (blk * kPage + tk) * size_t(c.nv) * 4 + size_t(lane) * 4;
+                    x[0][i] = *reinterpret_cast<const float4*>(c.k + at);
+                    x[1][i] = *reinterpret_cast<const float4*>(c.v + at);
+                }
             }
         }
         float mx[2] = {0.f, 0.f};
@@ -336,14 +322,28 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
         const TcReq& r = reqs[rq];
         const int local = int(qid - r.qimg0);
         const int h = local / r.n_qt, qt = local % r.n_qt;
-        const bool vec = query_vec(r, D);
+        const int n_packed = r.rows * group;
+        const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
         unsigned char* img = q_images + size_t(qid) * q_image_bytes(D);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
             float4 x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = query_row4(r, h, group, qt * kBM + half * 64 + warp * 8 + i, lane, D, vec);
+                const int pr = qt * kBM + half * 64 + warp * 8 + i;
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (pr < n_packed) {
+                    const float* row = r.q + size_t(h * group + pr % group) * r.q_hs + size_t(pr / group) * r.q_ts;
+                    const int d = lane * 4;
+                    if (vec) {
+                        if (d < D) x[i] = *reinterpret_cast<const float4*>(row + d);
+                    } else {
+                        if (d + 0 < D) x[i].x = row[d + 0];
+                        if (d + 1 < D) x[i].y = row[d + 1];
+                        if (d + 2 < D) x[i].z = row[d + 2];
+                        if (d + 3 < D) x[i].w = row[d + 3];
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -376,17 +376,11 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_
 // warpgroups: thread r of each owns packed row r; warpgroup w takes page w of every tile and columns
 // [64 w, 64 w + 64) of O.  S is read from tensor memory, P goes back over it as hi (32 columns) and
 // lo (32 columns).
-// FUSED, for requests of one row tile per KV head: there is no pass 1.  Every K and V element is needed
-// by one block only, so the softmax warps convert each tile themselves, between two softmaxes, while the
-// MMAs of the tile before run; warp 0 asks for the tiles ahead of them to be brought to L2.  (Images
-// through global memory move three times the cache's bytes.)  With weights the K and query images are
-// also left in global memory for pass 4.
 // Every wait is bounded; on expiry the kernel records a status code, drains and returns.
-template <bool FUSED>
 __global__ void __launch_bounds__(rt::kThreads, 1)
 read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items, const int* __restrict__ page_ids,
-               CacheView c, unsigned char* __restrict__ images, PageMeta* __restrict__ meta,
-               unsigned char* __restrict__ q_images, float2* __restrict__ row_meta,
+               CacheView c, const unsigned char* __restrict__ images, const PageMeta* __restrict__ meta,
+               const unsigned char* __restrict__ q_images, float2* __restrict__ row_meta,
                float* __restrict__ partials, float scale_log2, int group, int want_lse, int* __restrict__ status) {
     using namespace rt;
     using pf::fence_after_sync;
@@ -421,9 +415,6 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
     // by tile parity: a fast warp of the next tile must not be seen by a slow one of this tile
     volatile int* sm_dead = abort_flag + 1;              // [2]
     float* xchg = reinterpret_cast<float*>(bars + 32);   // [2 tiles][2 warpgroups][128 rows]
-    // FUSED: largest magnitudes and bad rows of the tiles' pages by warp, [2 tiles][K, V][2 pages][8 warps]
-    float* conv_max = xchg + 512;
-    unsigned char* conv_bad = reinterpret_cast<unsigned char*>(conv_max + 64);
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -438,15 +429,15 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
     const long long img0 = r.img0 + (long long)it.page_begin * c.num_kv_heads + it.head;
 
     if (tid == 0) {
-        mbar_init(q_full, FUSED ? kSoftWarps : 1);
+        mbar_init(q_full, 1);
         mbar_init(o_full, 1);
         mbar_init(o_empty, kSoftWarps);
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&k_full[s], FUSED ? kSoftWarps : 1);
+            mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
         }
         for (int s = 0; s < kVStages; ++s) {
-            mbar_init(&v_full[s], FUSED ? kSoftWarps : 1);
+            mbar_init(&v_full[s], 1);
             mbar_init(&v_empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -471,20 +462,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
 
     if (warp == 0) {
         // =============================== image copies ===============================
-        if (FUSED) {
-            // K and V pages of this item to L2, two tiles ahead of their conversion
-            if (lane < 2) {
-                const size_t bytes = c.u8 ? size_t(kPage) * (2 * size_t(c.dq) + 8) : size_t(kPage) * c.nv * 16;
-                for (int pg = 0; pg < n_pages; ++pg) {
-                    if (pg >= 6 && !(pg & 1) && !mbar_spin_bounded(&k_empty[0], uint32_t((pg / 2 - 3) & 1))) break;
-                    const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_ids[r.page_off + it.page_begin + pg])) * c.num_kv_heads + it.head;
-                    const void* src = c.u8 ? static_cast<const void*>(c.u8 + blk * bytes)
-                                           : reinterpret_cast<const unsigned char*>(lane ? c.v : c.k) + blk * bytes;
-                    if (!c.u8 || lane == 0)
-                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(uint32_t(bytes)) : "memory");
-                }
-            }
-        } else if (lane == 0) {
+        if (lane == 0) {
             const size_t img_bytes = page_image_bytes(D);
             const size_t step = size_t(c.num_kv_heads) * img_bytes;   // next page of the same head
             const unsigned char* base = images + size_t(img0) * img_bytes;
@@ -601,142 +579,8 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
         const int limit_first = r.causal ? r.kv_len - r.rows + (it.qt * kBM) / group + 1 : r.kv_len;
         const int* pages = page_ids + r.page_off;
         auto wg_barrier = [&]() { named_bar_sync(1, 256); };
-        const int w8 = warp - 2;
+        const float cq = __ldcg(&row_meta[size_t(qid) * kBM + rr]).x;
         const bool my_cols = col0 < n_pv;                 // head_dim <= 64: the second half has none
-        auto proxy_arrive = [&](uint64_t* bar) {          // shared memory written here, read by the MMAs
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        float cq;
-        if constexpr (FUSED) {
-            const bool vec = query_vec(r, D);
-            unsigned char* img = want_lse ? q_images + size_t(qid) * q_image_bytes(D) : nullptr;
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                float4 x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[i] = query_row4(r, it.head, group, it.qt * kBM + half * 64 + w8 * 8 + i, lane, D, vec);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = half * 64 + w8 * 8 + i;
-                    const bool ok = __all_sync(kFull, finite4(x[i]));
-                    float m = max4(x[i]);
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-                    float up, down;
-                    scale_of(ok ? m : 1.f, up, down);
-                    const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
-                    store_row_image(q_s, q_s + size_t(nb) * kRowsSub, kRowsSub, row, lane, nb, y, ok);
-                    if (lane == 0) xchg[row] = down * scale_log2;
-                    if (want_lse) {
-                        store_row_image(img, img + size_t(nb) * kRowsSub, kRowsSub, row, lane, nb, y, ok);
-                        if (lane == 0) row_meta[size_t(qid) * kBM + row] = make_float2(down * scale_log2, INFINITY);
-                    }
-                }
-            }
-            proxy_arrive(q_full);
-            wg_barrier();
-            cq = xchg[rr];
-            wg_barrier();
-        } else {
-            cq = __ldcg(&row_meta[size_t(qid) * kBM + rr]).x;
-        }
-        // FUSED: K (or V) of tile j from the cache to its images.  Returns the factors that undo the two
-        // pages' scaling, and whether some row holds an infinity or a NaN.
-        auto convert = [&](int j, bool v, float& f0, float& f1) -> unsigned {
-            const int np = min(2, n_pages - 2 * j), par = j & 1;
-            float4 x[2][8];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int page = it.page_begin + 2 * j + p;
-                size_t blk = 0;
-                if (p < np) blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(pages[page])) * c.num_kv_heads + it.head;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int tk = w8 * 8 + i;
-                    x[p][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (p < np && page * kPage + tk < r.kv_len) x[p][i] = cache_row4(c, blk, tk, lane, v);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                float m = 0.f;
-                unsigned bad = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (!__all_sync(kFull, finite4(x[p][i]))) {
-                        bad |= 1u << i;
-                        x[p][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                    m = fmaxf(m, max4(x[p][i]));
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-                if (lane == 0) {
-                    conv_max[((par * 2 + v) * 2 + p) * 8 + w8] = m;
-                    conv_bad[((par * 2 + v) * 2 + p) * 8 + w8] = (unsigned char)bad;
-                }
-            }
-            wg_barrier();
-            float up[2];
-            float f[2];
-            unsigned any = 0;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const float4 a = *reinterpret_cast<const float4*>(&conv_max[((par * 2 + v) * 2 + p) * 8]);
-                const float4 b = *reinterpret_cast<const float4*>(&conv_max[((par * 2 + v) * 2 + p) * 8 + 4]);
-                const uint2 z = *reinterpret_cast<const uint2*>(&conv_bad[((par * 2 + v) * 2 + p) * 8]);
-                any |= z.x | z.y;
-                scale_of(fmaxf(max4(a), max4(b)), up[p], f[p]);
-            }
-            f0 = f[0];
-            f1 = np > 1 ? f[1] : f[0];
-            if (!v && j > 0) {
-                // QK of the tile before has read the K tile
-                if (!warp_spin_bounded(&k_empty[1], uint32_t((j - 1) & 1), lane)) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                if (p >= np) break;
-                const int pg = 2 * j + p;
-                unsigned char* hi_img = v ? v_s + size_t(pg % kVStages) * kVBytes : k_s + size_t(p) * kSub;
-                const size_t stride = v ? size_t(kSub) : size_t(kRowsSub);
-                if (v && pg >= kVStages) {
-                    if (!warp_spin_bounded(&v_empty[pg % kVStages], uint32_t((pg / kVStages - 1) & 1), lane)) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
-                }
-                unsigned char* g_img = (want_lse && !v) ? images + (size_t(img0) + size_t(pg) * c.num_kv_heads) * page_image_bytes(D) : nullptr;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 y = make_float4(x[p][i].x * up[p], x[p][i].y * up[p], x[p][i].z * up[p], x[p][i].w * up[p]);
-                    store_row_image(hi_img, hi_img + size_t(nb) * stride, stride, w8 * 8 + i, lane, nb, y, true);
-                    if (g_img) store_row_image(g_img, g_img + size_t(nb) * kSub, kSub, w8 * 8 + i, lane, nb, y, true);
-                }
-                if (g_img && w8 == 0 && lane == 0) {
-                    PageMeta pm = {};
-                    pm.fk = f[p];
-                    for (int k = 0; k < 8; ++k) pm.bad_k |= (unsigned long long)(conv_bad[(par * 4 + p) * 8 + k]) << (8 * k);
-                    meta[img0 + (long long)pg * c.num_kv_heads] = pm;
-                }
-                if (v) proxy_arrive(&v_full[pg % kVStages]);
-            }
-            if (!v) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&k_full[0]);
-                    mbar_arrive(&k_full[1]);
-                }
-            }
-            return any;
-        };
-        float nfk0 = 0.f, nfk1 = 0.f, nfv0 = 0.f, nfv1 = 0.f;   // of the tile that was converted last
-        unsigned nbad = 0;
-        if constexpr (FUSED) {
-            nbad = convert(0, false, nfk0, nfk1) ? 1u : 0u;
-            nbad |= convert(0, true, nfv0, nfv1) ? 2u : 0u;
-        }
 
         float2 o[32];
 #pragma unroll
@@ -783,14 +627,10 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             // both pages' factors (uniform over the block)
             const PageMeta* pm0 = pm + size_t(2 * j) * c.num_kv_heads;
             const PageMeta* pm1 = two ? pm0 + c.num_kv_heads : pm0;
-            const float fv0 = FUSED ? nfv0 : pm0->fv, fv1 = FUSED ? nfv1 : pm1->fv;
-            const float cm = cq * (FUSED ? (wg ? nfk1 : nfk0) : (wg ? pm1 : pm0)->fk);
-            const unsigned bad = FUSED ? nbad : pm0->bad | pm1->bad;
+            const float fv0 = pm0->fv, fv1 = pm1->fv;
+            const float cm = cq * (wg ? pm1 : pm0)->fk;
+            const unsigned bad = pm0->bad | pm1->bad;
             const float fv = fmaxf(fv0, fv1);
-            auto bad_rows = [&](bool v, int p) -> unsigned long long {
-                if (!FUSED) return v ? (p ? pm1 : pm0)->bad_v : (p ? pm1 : pm0)->bad_k;
-                return *reinterpret_cast<const unsigned long long*>(&conv_bad[((sb * 2 + v) * 2 + p) * 8]);
-            };
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
             if (lane == 0 && dead) { sm_dead[sb] = 1; *abort_flag = 1; }
             fence_after_sync();
@@ -802,7 +642,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 if (bad & 1u) {
                     // rows of K with an infinity or a NaN: their scores one by one, in f32, put where the
                     // MMA left zeros
-                    unsigned long long b = bad_rows(false, wg);
+                    unsigned long long b = (wg ? pm1 : pm0)->bad_k;
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
                         b &= b - 1;
@@ -883,7 +723,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 wg_barrier();
                 fence_after_sync();
                 for (int p = 0; p < 2; ++p) {
-                    unsigned long long b = p == 0 || two ? bad_rows(true, p) : 0ull;
+                    unsigned long long b = p == 0 ? pm0->bad_v : (two ? pm1->bad_v : 0ull);
                     const float unscale = fv / (kPScale * (p ? fv1 : fv0));
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
@@ -911,19 +751,16 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 }
                 fence_before_sync();
                 wg_barrier();
+            } else if (j > 0) {
                 warp_arrive(&p_full[sb], lane);
-            } else {
-                warp_arrive(&p_full[sb], lane);
-                if (j > 0 && !add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+                if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
+                alpha_prev = alpha;
+                f_prev = fv * (1.0f / kPScale);
+                continue;
             }
             alpha_prev = alpha;
             f_prev = fv * (1.0f / kPScale);
-            if constexpr (FUSED) {
-                if (j + 1 < n_tiles) {
-                    nbad = convert(j + 1, false, nfk0, nfk1) ? 1u : 0u;
-                    nbad |= convert(j + 1, true, nfv0, nfv1) ? 2u : 0u;
-                }
-            }
+            warp_arrive(&p_full[sb], lane);
         }
         if (dead && lane == 0) report_status(status, kDevWaitFull);
         if (!dead) {
@@ -955,6 +792,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 }
             }
             wg_barrier();
+            const int w8 = warp - 2;
             const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.out) | uintptr_t(r.o_hs * 4) | uintptr_t(r.o_ts * 4)) & 15) == 0;
             for (int i = w8 * 16; i < w8 * 16 + 16; ++i) {
                 const int p = it.qt * kBM + i;
