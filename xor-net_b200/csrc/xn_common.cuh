@@ -82,7 +82,7 @@ struct ReqPatchTable {
 // The tiles of all (request, KV head, head subgroup, row) units are numbered through, request by
 // request; every unit of a request has `n_tiles` of them and block b of G takes tiles
 // [T b / G, T (b + 1) / G).
-constexpr int kReadEntries = 24;
+constexpr int kReadEntries = 64;
 struct ReadEntry {
     const float* q;
     float* out;

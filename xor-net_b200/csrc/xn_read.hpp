@@ -632,7 +632,7 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     std::stable_sort(items.begin(), items.end(), [](const TcItem& a, const TcItem& b) {
         return a.page_end - a.page_begin > b.page_end - b.page_begin;
     });
-    if (n_img + n_qimg > (1ll << 31) - 1)
+    if (2 * (n_img + n_qimg) > (1ll << 31) - 1)
         return fail(c, XN_ERR_CAPACITY, "%lld pages and row tiles in one submission are too many", n_img + n_qimg);
 
     // workspace: page images | query images | page factors | row factors | partial records
@@ -657,7 +657,7 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     const CacheView view = cache_view(c);
     const float scale_log2 = c->scale * 1.4426950408889634f;
     if (c->profile && (rc = profile_begin(c, 1)) != XN_OK) return rc;
-    XN_CUDA(c, launch_pdl(c, page_images_kernel, dim3(unsigned(n_img + n_qimg)), 256, 0, true, 0, reqs_d, int(subs.size()), n_img,
+    XN_CUDA(c, launch_pdl(c, page_images_kernel, dim3(unsigned(2 * (n_img + n_qimg))), 256, 0, true, 0, reqs_d, int(subs.size()), n_img,
                           pages_d, view, img, meta, qimg, row_meta, scale_log2, G));
     XN_CUDA(c, launch_pdl(c, read_tc_kernel, dim3(unsigned(items.size())), rt::kThreads, size_t(rt::kSmemBytes), true, 0, reqs_d,
                           reinterpret_cast<const TcItem*>(slot->dev + o_item), pages_d, view, img, meta, qimg, row_meta,

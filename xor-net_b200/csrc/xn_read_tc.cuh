@@ -63,13 +63,12 @@ struct TcKeyTile {
     int req, head, tile, qt_begin;
 };
 
-// What the softmax needs to know about a page: factors that undo the scaling of K and V, and the
-// rows that hold an infinity or a NaN (their images are zero; they are added exactly on the side).
+// What the softmax needs to know about a page's K [0] and V [1]: factors that undo the scaling, and
+// the rows that hold an infinity or a NaN (their images are zero; they are added exactly on the side).
 struct __align__(16) PageMeta {
-    float fk, fv;
-    unsigned bad;      // bit 0: bad_k is not empty, bit 1: bad_v
-    unsigned pad;
-    unsigned long long bad_k, bad_v;
+    float f[2];
+    unsigned any_bad[2];
+    unsigned long long bad[2];
 };
 
 // Where the cache rows are, for the rare exact path and the image kernel.
@@ -138,6 +137,13 @@ __device__ __forceinline__ void scale_of(float m, float& up, float& down) {
     down = __uint_as_float(uint32_t(127 - 13 + e) << 23);
 }
 
+// the larger of m and |x|, or NaN
+__device__ __forceinline__ float max_nan(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
     uint32_t r;
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
@@ -192,6 +198,43 @@ __device__ __forceinline__ void store_row_image(unsigned char* hi_img, unsigned 
     *reinterpret_cast<uint2*>(lo_img + at) = lo;
 }
 
+// Four columns (4 * lane ..) of token tk of a cache block, zeros past the row's end.
+__device__ __forceinline__ float4 cache_row4(const CacheView& c, size_t blk, int tk, int lane, bool v) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c.u8) {
+        const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
+        if (lane * 4 < c.dq) {
+            const float s = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq)[(v ? kPage : 0) + tk];
+            const uchar4 u = *reinterpret_cast<const uchar4*>(b + size_t((v ? kPage : 0) + tk) * c.dq + lane * 4);
+            // (bytes past head_dim hold 128, but 0 * s is NaN for an infinite scale)
+            if (lane * 4 + 0 < c.head_dim) x.x = (float(u.x) - 128.0f) * s;
+            if (lane * 4 + 1 < c.head_dim) x.y = (float(u.y) - 128.0f) * s;
+            if (lane * 4 + 2 < c.head_dim) x.z = (float(u.z) - 128.0f) * s;
+            if (lane * 4 + 3 < c.head_dim) x.w = (float(u.w) - 128.0f) * s;
+        }
+    } else if (lane < c.nv) {   // rows are padded with zeros to whole float4
+        x = *reinterpret_cast<const float4*>((v ? c.v : c.k) + (blk * kPage + tk) * size_t(c.nv) * 4 + size_t(lane) * 4);
+    }
+    return x;
+}
+
+// Four columns of a packed query row (row p of a KV head's group), zeros past the end.
+__device__ __forceinline__ float4 query_row4(const TcReq& r, int head, int group, int p, int lane, int D, bool vec) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d = lane * 4;
+    if (p >= r.rows * group || d >= D) return x;
+    const float* row = r.q + (long long)(head * group + p % group) * r.q_hs + (long long)(p / group) * r.q_ts + d;
+    if (vec) return *reinterpret_cast<const float4*>(row);
+    x.x = row[0];
+    if (d + 1 < D) x.y = row[1];
+    if (d + 2 < D) x.z = row[2];
+    if (d + 3 < D) x.w = row[3];
+    return x;
+}
+__device__ __forceinline__ bool query_vec(const TcReq& r, int D) {
+    return (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
+}
+
 // One element of a cached row, whatever the format (rare paths only).
 __device__ __forceinline__ float cache_elem(const CacheView& c, const int* pages, int layer, int head, int key, int d, bool v) {
     const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
@@ -206,160 +249,97 @@ __device__ __forceinline__ float cache_elem(const CacheView& c, const int* pages
 
 }  // namespace rt
 
-// Pass 1.  Blocks [0, n_page_blocks): one page of one KV head each (K and V); the rest: one 128-row
-// query tile each.  A warp handles a row per step, 4 columns per lane.  Bound by memory: 4 bytes
-// read and 4 written per element.
-__global__ void __launch_bounds__(256)
-page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_page_blocks,
+// Pass 1.  Blocks [0, 2 n_pages): K or V of one page of one KV head each; the rest: half a 128-row query
+// tile each.  A warp handles eight rows, 4 columns per lane.  Bound by memory: 4 bytes read and 4
+// written per element; blocks are small so that several per SM overlap one's loads with another's
+// stores.
+__global__ void __launch_bounds__(256, 4)
+page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages,
                    const int* __restrict__ page_ids, CacheView c, unsigned char* __restrict__ images,
                    PageMeta* __restrict__ meta, unsigned char* __restrict__ q_images,
                    float2* __restrict__ row_meta, float scale_log2, int group) {
     using namespace rt;
     pdl_launch_dependents();
-    __shared__ float s_max[2][8];
-    __shared__ unsigned s_bad[2][8];
+    __shared__ __align__(16) float s_max[8];
+    __shared__ __align__(8) unsigned char s_bad[8];
+    constexpr unsigned kFull = 0xffffffffu;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = c.head_dim, nb = blocks_of(D);
+    const bool is_q = (long long)blockIdx.x >= 2 * n_pages;
+    const long long id = (is_q ? (long long)blockIdx.x - 2 * n_pages : (long long)blockIdx.x) >> 1;
+    const int part = blockIdx.x & 1;      // K or V; half of the query tile
     pdl_wait();
-    if ((long long)blockIdx.x < n_page_blocks) {
-        const long long id = blockIdx.x;
-        int rq = 0;
-        while (rq + 1 < n_reqs && id >= reqs[rq + 1].img0) ++rq;
-        const TcReq& r = reqs[rq];
+    int rq = -1;                          // the last request that begins at or before id
+    for (int i = 0; i < n_reqs; i += 32)
+        rq += __popc(__ballot_sync(kFull, i + lane < n_reqs && id >= (is_q ? reqs[min(i + lane, n_reqs - 1)].qimg0
+                                                                              : reqs[min(i + lane, n_reqs - 1)].img0)));
+    const TcReq& r = reqs[rq];
+    float4 x[8];
+    if (!is_q) {
         const long long local = id - r.img0;
         const int page = int(local / c.num_kv_heads), h = int(local % c.num_kv_heads);
         const int ntok = min(kPage, r.kv_len - page * kPage);
         const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_ids[r.page_off + page])) * c.num_kv_heads + h;
-        float4 x[2][8];
-        if (c.u8) {
-            const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
-            const float* sc = reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq);
+        float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int tk = warp * 8 + i;
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    x[kv][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (tk < ntok && lane * 4 < c.dq) {
-                        const uchar4 u = *reinterpret_cast<const uchar4*>(b + size_t(kv * kPage + tk) * c.dq + lane * 4);
-                        const float s = sc[kv * kPage + tk];
-                        // (bytes past head_dim hold 128, but 0 * s is NaN for an infinite scale)
-                        if (lane * 4 + 0 < D) x[kv][i].x = (float(u.x) - 128.0f) * s;
-                        if (lane * 4 + 1 < D) x[kv][i].y = (float(u.y) - 128.0f) * s;
-                        if (lane * 4 + 2 < D) x[kv][i].z = (float(u.z) - 128.0f) * s;
-                        if (lane * 4 + 3 < D) x[kv][i].w = (float(u.w) - 128.0f) * s;
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int tk = warp * 8 + i;
-                x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (tk < ntok && lane < c.nv) {   // rows are padded with zeros to whole float4
-                    const size_t at = (blk * kPage + tk) * size_t(c.nv) * 4 + size_t(lane) * 4;
-                    x[0][i] = *reinterpret_cast<const float4*>(c.k + at);
-                    x[1][i] = *reinterpret_cast<const float4*>(c.v + at);
-                }
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int tk = warp * 8 + i;
+            x[i] = tk < ntok ? cache_row4(c, blk, tk, lane, part != 0) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        float mx[2] = {0.f, 0.f};
-        unsigned bad[2] = {0u, 0u};
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
+        for (int i = 0; i < 8; ++i) m = max_nan(max_nan(max_nan(max_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        unsigned bits = __reduce_max_sync(kFull, __float_as_uint(m)), bad = 0;   // as bits: finite < infinity < NaN
+        if (bits >= 0x7f800000u) {
+            m = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (!__all_sync(0xffffffffu, finite4(x[kv][i]))) {
-                    bad[kv] |= 1u << i;
-                    x[kv][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!__all_sync(kFull, finite4(x[i]))) {
+                    bad |= 1u << i;
+                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                mx[kv] = fmaxf(mx[kv], max4(x[kv][i]));
+                m = fmaxf(m, max4(x[i]));
             }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+            bits = __reduce_max_sync(kFull, __float_as_uint(m));
         }
         if (lane == 0) {
-            s_max[0][warp] = mx[0];
-            s_max[1][warp] = mx[1];
-            s_bad[0][warp] = bad[0];
-            s_bad[1][warp] = bad[1];
+            s_max[warp] = __uint_as_float(bits);
+            s_bad[warp] = (unsigned char)bad;
         }
         __syncthreads();
-        float up[2], down[2];
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            float m = 0.f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) m = fmaxf(m, s_max[kv][w]);
-            scale_of(m, up[kv], down[kv]);
-        }
+        float up, down;
+        scale_of(fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4))), up, down);
         if (threadIdx.x == 0) {
-            PageMeta pm = {};
-            pm.fk = down[0];
-            pm.fv = down[1];
-            for (int w = 0; w < 8; ++w) {
-                pm.bad_k |= (unsigned long long)(s_bad[0][w]) << (8 * w);
-                pm.bad_v |= (unsigned long long)(s_bad[1][w]) << (8 * w);
-            }
-            pm.bad = (pm.bad_k ? 1u : 0u) | (pm.bad_v ? 2u : 0u);
-            meta[id] = pm;
+            const unsigned long long rows = *reinterpret_cast<const unsigned long long*>(s_bad);
+            PageMeta& pm = meta[id];
+            pm.f[part] = down;
+            pm.any_bad[part] = rows != 0 ? 1u : 0u;
+            pm.bad[part] = rows;
         }
-        unsigned char* img = images + size_t(id) * page_image_bytes(D);
+        unsigned char* hi = images + size_t(id) * page_image_bytes(D) + size_t(part) * 2 * nb * kSub;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 y = make_float4(x[kv][i].x * up[kv], x[kv][i].y * up[kv], x[kv][i].z * up[kv], x[kv][i].w * up[kv]);
-                unsigned char* hi = img + size_t(kv) * 2 * nb * kSub;
-                store_row_image(hi, hi + size_t(nb) * kSub, kSub, warp * 8 + i, lane, nb, y, true);
-            }
+        for (int i = 0; i < 8; ++i)
+            store_row_image(hi, hi + size_t(nb) * kSub, kSub, warp * 8 + i, lane, nb,
+                            make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up), true);
     } else {
-        const long long qid = (long long)blockIdx.x - n_page_blocks;
-        int rq = 0;
-        while (rq + 1 < n_reqs && qid >= reqs[rq + 1].qimg0) ++rq;
-        const TcReq& r = reqs[rq];
-        const int local = int(qid - r.qimg0);
+        const int local = int(id - r.qimg0);
         const int h = local / r.n_qt, qt = local % r.n_qt;
-        const int n_packed = r.rows * group;
-        const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
-        unsigned char* img = q_images + size_t(qid) * q_image_bytes(D);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-            float4 x[8];
+        const bool vec = query_vec(r, D);
+        unsigned char* img = q_images + size_t(id) * q_image_bytes(D);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int pr = qt * kBM + half * 64 + warp * 8 + i;
-                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (pr < n_packed) {
-                    const float* row = r.q + size_t(h * group + pr % group) * r.q_hs + size_t(pr / group) * r.q_ts;
-                    const int d = lane * 4;
-                    if (vec) {
-                        if (d < D) x[i] = *reinterpret_cast<const float4*>(row + d);
-                    } else {
-                        if (d + 0 < D) x[i].x = row[d + 0];
-                        if (d + 1 < D) x[i].y = row[d + 1];
-                        if (d + 2 < D) x[i].z = row[d + 2];
-                        if (d + 3 < D) x[i].w = row[d + 3];
-                    }
-                }
-            }
+        for (int i = 0; i < 8; ++i) x[i] = query_row4(r, h, group, qt * kBM + part * 64 + warp * 8 + i, lane, D, vec);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int rr = half * 64 + warp * 8 + i;
-                const bool ok = __all_sync(0xffffffffu, finite4(x[i]));
-                float m = max4(x[i]);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                float up, down;
-                scale_of(ok ? m : 1.f, up, down);
-                const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
-                store_row_image(img, img + size_t(nb) * kRowsSub, kRowsSub, rr, lane, nb, y, ok);
-                // y: the log-sum-exp of the row, written by the attention kernel; rows past the end
-                // (and rows that see nothing) keep +inf, which gives them no weight anywhere
-                if (lane == 0) row_meta[size_t(qid) * kBM + rr] = make_float2(down * scale_log2, INFINITY);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int rr = part * 64 + warp * 8 + i;
+            const float m = max_nan(max_nan(max_nan(max_nan(0.f, x[i].x), x[i].y), x[i].z), x[i].w);
+            const unsigned bits = __reduce_max_sync(kFull, __float_as_uint(m));
+            const bool ok = bits < 0x7f800000u;
+            float up, down;
+            scale_of(ok ? __uint_as_float(bits) : 1.f, up, down);
+            store_row_image(img, img + size_t(nb) * kRowsSub, kRowsSub, rr, lane, nb,
+                            make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up), ok);
+            // y: the log-sum-exp of the row, written by the attention kernel; rows past the end
+            // (and rows that see nothing) keep +inf, which gives them no weight anywhere
+            if (lane == 0) row_meta[size_t(id) * kBM + rr] = make_float2(down * scale_log2, INFINITY);
         }
     }
 }
@@ -627,9 +607,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             // both pages' factors (uniform over the block)
             const PageMeta* pm0 = pm + size_t(2 * j) * c.num_kv_heads;
             const PageMeta* pm1 = two ? pm0 + c.num_kv_heads : pm0;
-            const float fv0 = pm0->fv, fv1 = pm1->fv;
-            const float cm = cq * (wg ? pm1 : pm0)->fk;
-            const unsigned bad = pm0->bad | pm1->bad;
+            const float fv0 = pm0->f[1], fv1 = pm1->f[1];
+            const float cm = cq * (wg ? pm1 : pm0)->f[0];
+            const bool bad_k = pm0->any_bad[0] | pm1->any_bad[0], bad_v = pm0->any_bad[1] | pm1->any_bad[1];
             const float fv = fmaxf(fv0, fv1);
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
             if (lane == 0 && dead) { sm_dead[sb] = 1; *abort_flag = 1; }
@@ -639,10 +619,10 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             const bool some_masked = key0 + kPage > limit_first;
             float mx = -INFINITY;
             if (!dead && have) {
-                if (bad & 1u) {
+                if (bad_k) {
                     // rows of K with an infinity or a NaN: their scores one by one, in f32, put where the
                     // MMA left zeros
-                    unsigned long long b = (wg ? pm1 : pm0)->bad_k;
+                    unsigned long long b = (wg ? pm1 : pm0)->bad[0];
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
                         b &= b - 1;
@@ -711,7 +691,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 tmem_st32(s_addr + 32, lo);
                 tmem_wait_st();
             }
-            if (bad & 2u) {
+            if (bad_v) {
                 // rows of V with an infinity or a NaN (uniform over the block): bring O up to date, then
                 // add p * v for the rows that see them; P of both pages is read back from tensor memory
                 if (j > 0) {
@@ -723,7 +703,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 wg_barrier();
                 fence_after_sync();
                 for (int p = 0; p < 2; ++p) {
-                    unsigned long long b = p == 0 ? pm0->bad_v : (two ? pm1->bad_v : 0ull);
+                    unsigned long long b = p == 0 ? pm0->bad[1] : (two ? pm1->bad[1] : 0ull);
                     const float unscale = fv / (kPScale * (p ? fv1 : fv0));
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
@@ -992,7 +972,7 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
         const bool in = key < r.kv_len;
         const int* pages = page_ids + r.page_off;
         const PageMeta pm = meta[img0 + (rr >= kPage && np > 1 ? c.num_kv_heads : 0)];
-        const bool bad = in && ((pm.bad_k >> (rr & 63)) & 1);
+        const bool bad = in && ((pm.bad[0] >> (rr & 63)) & 1);
         // packed rows from `first_row` on see the position
         const int first_row = r.causal ? max(0, (key - (r.kv_len - r.rows)) * group) : 0;
         float sum = 0.f;
@@ -1025,8 +1005,8 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
-                        const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * pm.fk, f.x, -f.y));
-                        const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * pm.fk, f.z, -f.w));
+                        const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * pm.f[0], f.x, -f.y));
+                        const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * pm.f[0], f.z, -f.w));
                         s0 += i >= from ? a : 0.f;
                         s1 += i + 1 >= from ? b : 0.f;
                     }
