@@ -669,10 +669,12 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     int cluster = 1, most_qt = 0;
     for (const TcReq& r : reqs) most_qt = std::max(most_qt, r.n_qt);
     while (cluster < ev::kMaxCluster && (long long)key_tiles.size() * cluster < 2 * c->sm_count && most_qt >= 4 * cluster) cluster *= 2;
-    if (want)
-        XN_CUDA(c, launch_pdl(c, account_tc_kernel, dim3(unsigned(key_tiles.size() * cluster)), rt::kThreads,
-                              size_t(rt::kAcctSmemBytes), true, unsigned(cluster), reqs_d, reinterpret_cast<const TcKeyTile*>(slot->dev + o_key), pages_d, view, img, meta, qimg,
-                              row_meta, c->acct_pool, scale_log2, G, cluster, c->status_d));
+    if (want) {
+        const int blocks = cluster > 1 ? int(key_tiles.size()) * cluster : std::min<int>(int(key_tiles.size()), c->sm_count);
+        XN_CUDA(c, launch_pdl(c, account_tc_kernel, dim3(unsigned(blocks)), rt::kThreads, size_t(rt::kAcctSmemBytes), true,
+                              unsigned(cluster), reqs_d, reinterpret_cast<const TcKeyTile*>(slot->dev + o_key), int(key_tiles.size()),
+                              pages_d, view, img, meta, qimg, row_meta, c->acct_pool, scale_log2, G, cluster, c->status_d));
+    }
     if (c->profile && (rc = profile_end(c)) != XN_OK) return rc;
     c->stats.prefill_launches += 1;
     return finish_slot(c, slot);

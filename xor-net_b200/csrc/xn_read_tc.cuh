@@ -99,8 +99,8 @@ constexpr int kTmemS = 0;                // 2 x 128 columns
 constexpr int kTmemO = 256;              // P_hi V_hi, then P_hi V_lo + P_lo V_hi: up to 128 columns each
 constexpr int kSoftWarps = 8;
 
-constexpr int kAcctQStages = 2;
-constexpr int kAcctSmemData = kKBytes + kAcctQStages * kQBytes;
+constexpr int kAcctStages = 3;           // 64 KB each: one K tile or 128 query rows
+constexpr int kAcctSmemData = kAcctStages * kKBytes;
 constexpr int kAcctSmemBytes = kAcctSmemData + 1024 + 4096;
 
 __host__ __device__ inline int blocks_of(int head_dim) { return head_dim > 64 ? 2 : 1; }
@@ -772,18 +772,20 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 }
             }
             wg_barrier();
+            // 16 rows per warp; lane i knows where row i goes
             const int w8 = warp - 2;
+            const int my_p = it.qt * kBM + w8 * 16 + (lane & 15);
             const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.out) | uintptr_t(r.o_hs * 4) | uintptr_t(r.o_ts * 4)) & 15) == 0;
-            for (int i = w8 * 16; i < w8 * 16 + 16; ++i) {
-                const int p = it.qt * kBM + i;
-                if (p >= n_packed || lane >= c.nv) continue;
-                const float4 x = tile[i * 32 + (lane ^ (i & 31))];
-                if (!whole) {
-                    *reinterpret_cast<float4*>(partials + size_t(it.part) * part_floats(c.nv * 4) + size_t(i) * c.nv * 4 + lane * 4) = x;
-                    continue;
-                }
-                float* row = r.out + size_t(it.head * group + p % group) * r.o_hs + size_t(p / group) * r.o_ts + lane * 4;
-                if (vec) {
+            const long long my_off = whole ? (long long)(it.head * group + my_p % group) * r.o_hs + (long long)(my_p / group) * r.o_ts
+                                           : (long long)(w8 * 16 + (lane & 15)) * c.nv * 4;
+            float* dst = whole ? r.out : partials + size_t(it.part) * part_floats(c.nv * 4);
+            const int n_rows = min(16, n_packed - it.qt * kBM - w8 * 16);
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                float* row = dst + __shfl_sync(kFull, my_off, i) + lane * 4;
+                if (i >= n_rows || lane >= c.nv) continue;
+                const float4 x = tile[(w8 * 16 + i) * 32 + (lane ^ ((w8 * 16 + i) & 31))];
+                if (vec || !whole) {
                     *reinterpret_cast<float4*>(row) = x;
                 } else {
                     row[0] = x.x;
@@ -848,6 +850,19 @@ read_merge_kernel(const TcReq* __restrict__ reqs, const TcMerge* __restrict__ me
         row_meta[size_t(r.qimg0 + (long long)mg.head * r.n_qt + mg.qt) * kBM + i].y = m + log2f(l);
 }
 
+// The three image slots of account_tc_kernel: one holds the K tile, the query images alternate between
+// the other two; the next K tile takes the one of those that falls free first.
+struct AcctSlots {
+    int k = 0, q0 = 1, q1 = 2;
+    __device__ int q(int j) const { return j & 1 ? q1 : q0; }
+    __device__ void next(int n_q) {
+        const int free = n_q & 1 ? q1 : q0, last = n_q & 1 ? q0 : q1;
+        q1 = k;
+        q0 = last;
+        k = free;
+    }
+};
+
 // Pass 4.  The account: S^T = K Q^T for 128 positions of one KV head against every tile of 128 packed
 // query rows that sees them, p = 2^(s - lse), summed over the rows in f32.  Positions are the rows of
 // the accumulator, so a thread owns a position and the sum needs no exchange and no atomics (its
@@ -855,7 +870,7 @@ read_merge_kernel(const TcReq* __restrict__ reqs, const TcMerge* __restrict__ me
 // query images stream through two stages.  With few positions and many rows the row tiles are dealt
 // out to a cluster of blocks, whose first block adds up the sums through the others' shared memory.
 __global__ void __launch_bounds__(rt::kThreads, 1)
-account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ tiles, const int* __restrict__ page_ids,
+account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ tiles, int n_tiles, const int* __restrict__ page_ids,
                   CacheView c, const unsigned char* __restrict__ images, const PageMeta* __restrict__ meta,
                   const unsigned char* __restrict__ q_images, const float2* __restrict__ row_meta,
                   float* __restrict__ pool, float scale_log2, int group, int cluster, int* __restrict__ status) {
@@ -868,38 +883,40 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
     using pf::tmem_wait_ld;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-    unsigned char* k_s = smem;
-    unsigned char* q_s = k_s + kKBytes;                       // [2] query images
     float2* rm_s = reinterpret_cast<float2*>(smem + kAcctSmemData);   // [2][128]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kAcctSmemData + 2 * kBM * 8);
-    uint64_t* k_full = bars + 0;
-    uint64_t* q_full = bars + 1;     // [2]
-    uint64_t* q_empty = bars + 3;    // [2]: one commit + 256 readers of the row factors
-    uint64_t* s_full = bars + 5;     // [2]
-    uint64_t* s_empty = bars + 7;    // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
+    uint64_t* full = bars + 0;       // [3], of the ring of images
+    uint64_t* empty = bars + 3;      // [3]
+    uint64_t* s_full = bars + 6;     // [2]
+    uint64_t* s_empty = bars + 8;    // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 10);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
-    float* xchg = reinterpret_cast<float*>(bars + 16);        // [128]
+    float* xchg = reinterpret_cast<float*>(bars + 16);        // [2][128]
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = int(ev::cluster_rank());
-    const TcKeyTile kt = tiles[int(blockIdx.x) / cluster];
-    const TcReq& r = reqs[kt.req];
     const int D = c.head_dim, nb = blocks_of(D);
     const int k_steps = (D + 15) / 16;
-    const int np = min(2, r.n_pages - 2 * kt.tile);
-    const int n_all = r.n_qt - kt.qt_begin;
-    const int n_q = n_all > rank ? (n_all - rank - 1) / cluster + 1 : 0;   // row tiles rank, rank + cluster, ...
-    const long long img0 = r.img0 + (long long)(2 * kt.tile) * c.num_kv_heads + kt.head;
-    const long long qid0 = r.qimg0 + (long long)kt.head * r.n_qt + kt.qt_begin + rank;
+    const int stride = int(gridDim.x) / cluster, first = int(blockIdx.x) / cluster;
+    // the block's tiles, heaviest first, every other round from the light end
+    auto tile_at = [&](int round) { return round * stride + ((round & 1) ? stride - 1 - first : first); };
+    const int n_rounds = (n_tiles + stride - 1) / stride;
+    const TcKeyTile kt0 = tiles[first];   // (plan data: there before the kernel before this one ends)
+    auto key_tile = [&](int round) { return round == 0 ? kt0 : tiles[tile_at(round)]; };
+    auto row_tiles = [&](const TcKeyTile& kt) {   // row tiles rank, rank + cluster, ...
+        const int n = reqs[kt.req].n_qt - kt.qt_begin;
+        return n > rank ? (n - rank - 1) / cluster + 1 : 0;
+    };
+    auto image0 = [&](const TcKeyTile& kt) { return reqs[kt.req].img0 + (long long)(2 * kt.tile) * c.num_kv_heads + kt.head; };
     if (tid == 0) {
-        mbar_init(k_full, 1);
+        for (int s = 0; s < kAcctStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&q_full[s], 1);
-            mbar_init(&q_empty[s], 257);
             mbar_init(&s_full[s], 1);
-            mbar_init(&s_empty[s], 256);
+            mbar_init(&s_empty[s], kSoftWarps);
         }
         *abort_flag = 0;
         mbar_fence_init();
@@ -919,19 +936,39 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
     if (warp == 0) {
         if (lane == 0) {
             const size_t img_bytes = page_image_bytes(D);
-            mbar_arrive_expect_tx(k_full, uint32_t(np * 2 * nb) * kSub);
-            for (int p = 0; p < np; ++p)
-                for (int b = 0; b < 2 * nb; ++b)
-                    bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
-                             images + (size_t(img0) + size_t(p) * c.num_kv_heads) * img_bytes + size_t(b) * kSub, kSub, k_full);
+            const uint32_t q_bytes = uint32_t(q_image_bytes(D));
             bool ok = true;
-            for (int j = 0; j < n_q && ok; ++j) {
-                const int s = j & 1;
-                if (j >= 2 && !mbar_spin_bounded(&q_empty[s], uint32_t(((j >> 1) - 1) & 1))) { ok = false; break; }
-                const uint32_t bytes = uint32_t(q_image_bytes(D));
-                mbar_arrive_expect_tx(&q_full[s], bytes + kBM * 8);
-                bulk_g2s(q_s + size_t(s) * kQBytes, q_images + size_t(qid0 + j * cluster) * bytes, bytes, &q_full[s]);
-                bulk_g2s(rm_s + s * kBM, row_meta + size_t(qid0 + j * cluster) * kBM, kBM * 8, &q_full[s]);
+            int js = 0;                     // query images so far
+            unsigned used = 0, odd = 0;     // per slot: used before; parity of its uses
+            AcctSlots sl;
+            auto take = [&](int s, uint32_t bytes) -> bool {
+                if ((used >> s & 1u) && !mbar_spin_bounded(&empty[s], (odd >> s & 1u) ^ 1u)) return false;
+                mbar_arrive_expect_tx(&full[s], bytes);
+                used |= 1u << s;
+                odd ^= 1u << s;
+                return true;
+            };
+            for (int round = 0; round < n_rounds && ok; ++round) {
+                if (tile_at(round) >= n_tiles) continue;
+                const TcKeyTile kt = key_tile(round);
+                const TcReq& r = reqs[kt.req];
+                const int np = min(2, r.n_pages - 2 * kt.tile), n_q = row_tiles(kt);
+                const long long qid0 = r.qimg0 + (long long)kt.head * r.n_qt + kt.qt_begin + rank;
+                const int ks = sl.k;
+                if (!take(ks, uint32_t(np * 2 * nb) * kSub)) { ok = false; break; }
+                for (int p = 0; p < np; ++p)
+                    for (int b = 0; b < 2 * nb; ++b)
+                        bulk_g2s(smem + size_t(ks) * kKBytes + size_t(b) * kRowsSub + size_t(p) * kSub,
+                                 images + (size_t(image0(kt)) + size_t(p) * c.num_kv_heads) * img_bytes + size_t(b) * kSub, kSub, &full[ks]);
+                for (int j = 0; j < n_q; ++j, ++js) {
+                    // (the row factors of two query images before have been read)
+                    if (js >= 2 && !mbar_spin_bounded(&s_empty[js & 1], uint32_t(((js >> 1) - 1) & 1))) { ok = false; break; }
+                    const int qs = sl.q(j);
+                    if (!take(qs, q_bytes + kBM * 8)) { ok = false; break; }
+                    bulk_g2s(smem + size_t(qs) * kKBytes, q_images + size_t(qid0 + j * cluster) * q_bytes, q_bytes, &full[qs]);
+                    bulk_g2s(rm_s + (js & 1) * kBM, row_meta + size_t(qid0 + j * cluster) * kBM, kBM * 8, &full[qs]);
+                }
+                sl.next(n_q);
                 if (*abort_flag) break;
             }
             if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
@@ -939,27 +976,41 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
     } else if (warp == 1) {
         if (lane == 0) {
             const uint32_t idesc = make_idesc16(kBM, kBM, 0);
-            const uint64_t kd = smem_desc(smem_u32(k_s), 0, 1024, pf::kLayoutSw128);
-            const uint64_t qd0 = smem_desc(smem_u32(q_s), 0, 1024, pf::kLayoutSw128);
+            const uint64_t d0 = smem_desc(smem_u32(smem), 0, 1024, pf::kLayoutSw128);
             const uint64_t lo_rows = uint64_t(nb) * kRowsSub >> 4;
-            bool ok = mbar_spin_bounded(k_full, 0);
-            for (int j = 0; j < n_q && ok; ++j) {
-                const int s = j & 1;
-                if (!mbar_spin_bounded(&q_full[s], uint32_t((j >> 1) & 1))) { ok = false; break; }
-                if (j >= 2 && !mbar_spin_bounded(&s_empty[s], uint32_t(((j >> 1) - 1) & 1))) { ok = false; break; }
-                fence_after_sync();
-                const uint64_t qd = qd0 + uint64_t(s) * (kQBytes >> 4);
-                const uint32_t d = tmem + s * 128;
+            bool ok = true;
+            int js = 0;
+            unsigned odd = 0;
+            AcctSlots sl;
+            auto filled = [&](int s) -> bool {
+                const bool there = mbar_spin_bounded(&full[s], odd >> s & 1u);
+                odd ^= 1u << s;
+                return there;
+            };
+            for (int round = 0; round < n_rounds && ok; ++round) {
+                if (tile_at(round) >= n_tiles) continue;
+                const int n_q = row_tiles(key_tile(round));
+                const int k_slot = sl.k;
+                if (!filled(k_slot)) { ok = false; break; }
+                for (int j = 0; j < n_q; ++j, ++js) {
+                    const int s = js & 1, q_slot = sl.q(j);
+                    if (!filled(q_slot) || (js >= 2 && !mbar_spin_bounded(&s_empty[s], uint32_t(((js >> 1) - 1) & 1)))) { ok = false; break; }
+                    fence_after_sync();
+                    const uint64_t kd = d0 + uint64_t(k_slot) * (kKBytes >> 4), qd = d0 + uint64_t(q_slot) * (kKBytes >> 4);
+                    const uint32_t d = tmem + s * 128;
 #pragma unroll
-                for (int term = 0; term < 3; ++term) {
-                    const uint64_t a0 = kd + (term == 0 ? lo_rows : 0), b0 = qd + (term == 1 ? lo_rows : 0);
-                    for (int ks = 0; ks < k_steps; ++ks) {
-                        const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
-                        mma16_ss(d, a0 + o, b0 + o, idesc, (term > 0 || ks > 0) ? 1u : 0u);
+                    for (int term = 0; term < 3; ++term) {
+                        const uint64_t a0 = kd + (term == 0 ? lo_rows : 0), b0 = qd + (term == 1 ? lo_rows : 0);
+                        for (int ks = 0; ks < k_steps; ++ks) {
+                            const uint64_t o = uint64_t(ks >> 2) * (kRowsSub >> 4) + uint64_t(ks & 3) * 2;
+                            mma16_ss(d, a0 + o, b0 + o, idesc, (term > 0 || ks > 0) ? 1u : 0u);
+                        }
                     }
+                    mma_commit(&empty[q_slot]);
+                    mma_commit(&s_full[s]);
                 }
-                mma_commit(&q_empty[s]);
-                mma_commit(&s_full[s]);
+                mma_commit(&empty[k_slot]);
+                sl.next(n_q);
             }
             if (!ok) { report_status(status, kDevWaitMma); *abort_flag = 1; }
         }
@@ -968,59 +1019,72 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
         const int quarter = warp & 3;
         const int rr = quarter * 32 + lane;
         const uint32_t lane_base = uint32_t(quarter * 32) << 16;
-        const int key = kt.tile * 128 + rr;
-        const bool in = key < r.kv_len;
-        const int* pages = page_ids + r.page_off;
-        const PageMeta pm = meta[img0 + (rr >= kPage && np > 1 ? c.num_kv_heads : 0)];
-        const bool bad = in && ((pm.bad[0] >> (rr & 63)) & 1);
-        // packed rows from `first_row` on see the position
-        const int first_row = r.causal ? max(0, (key - (r.kv_len - r.rows)) * group) : 0;
-        float sum = 0.f;
         bool dead = false;
-        for (int j = 0; j < n_q; ++j) {
-            const int s = j & 1;
-            if (!warp_spin_bounded(&s_full[s], uint32_t((j >> 1) & 1), lane)) { dead = true; break; }
-            fence_after_sync();
-            const int row0 = (kt.qt_begin + rank + j * cluster) * kBM + wg * 64;
-            const float2* rm = rm_s + s * kBM + wg * 64;
+        int js = 0, tp = 0;
+        for (int round = 0; round < n_rounds; ++round) {
+            if (tile_at(round) >= n_tiles) continue;
+            const TcKeyTile kt = key_tile(round);
+            const TcReq& r = reqs[kt.req];
+            const int n_q = row_tiles(kt);
+            const int key = kt.tile * kBM + rr;
+            const bool in = key < r.kv_len;
+            const int* pages = page_ids + r.page_off;
+            const PageMeta& pm = meta[image0(kt) + (rr >= kPage && 2 * kt.tile + 1 < r.n_pages ? c.num_kv_heads : 0)];
+            const float fk = pm.f[0];
+            const bool bad = in && ((pm.bad[0] >> (rr & 63)) & 1);
+            // packed rows from `first_row` on see the position
+            const int first_row = r.causal ? max(0, (key - (r.kv_len - r.rows)) * group) : 0;
+            float sum = 0.f;
+            for (int j = 0; j < n_q && !dead; ++j, ++js) {
+                const int s = js & 1;
+                if (!warp_spin_bounded(&s_full[s], uint32_t((js >> 1) & 1), lane)) { dead = true; break; }
+                fence_after_sync();
+                const int row0 = (kt.qt_begin + rank + j * cluster) * kBM + wg * 64;
+                const float2* rm = rm_s + s * kBM + wg * 64;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t x[32];
-                tmem_ld32(tmem + lane_base + s * 128 + wg * 64 + hf * 32, x);
-                tmem_wait_ld();
-                if (bad) {
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t x[32];
+                    tmem_ld32(tmem + lane_base + s * 128 + wg * 64 + hf * 32, x);
+                    tmem_wait_ld();
+                    if (bad) {
 #pragma unroll 1
-                    for (int i = 0; i < 32; ++i) {
-                        const int p = row0 + hf * 32 + i;
-                        if (p < first_row || p >= r.rows * group) continue;
-                        float dot = 0.f;
-                        for (int d = 0; d < D; ++d)
-                            dot = fmaf(r.q[size_t(kt.head * group + p % group) * r.q_hs + size_t(p / group) * r.q_ts + d],
-                                       cache_elem(c, pages, r.layer, kt.head, key, d, false), dot);
-                        sum += pf::ex2(dot * scale_log2 - rm[hf * 32 + i].y);
-                    }
-                } else {
-                    const int from = first_row - (row0 + hf * 32);   // columns before this one do not count
-                    float s0 = 0.f, s1 = 0.f;
+                        for (int i = 0; i < 32; ++i) {
+                            const int p = row0 + hf * 32 + i;
+                            if (p < first_row || p >= r.rows * group) continue;
+                            float dot = 0.f;
+                            for (int d = 0; d < D; ++d)
+                                dot = fmaf(r.q[size_t(kt.head * group + p % group) * r.q_hs + size_t(p / group) * r.q_ts + d],
+                                           cache_elem(c, pages, r.layer, kt.head, key, d, false), dot);
+                            sum += pf::ex2(dot * scale_log2 - rm[hf * 32 + i].y);
+                        }
+                    } else {
+                        const int from = first_row - (row0 + hf * 32);   // columns before this one do not count
+                        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
-                        const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * pm.f[0], f.x, -f.y));
-                        const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * pm.f[0], f.z, -f.w));
-                        s0 += i >= from ? a : 0.f;
-                        s1 += i + 1 >= from ? b : 0.f;
+                        for (int i = 0; i < 32; i += 2) {
+                            const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
+                            const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * fk, f.x, -f.y));
+                            const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * fk, f.z, -f.w));
+                            s0 += i >= from ? a : 0.f;
+                            s1 += i + 1 >= from ? b : 0.f;
+                        }
+                        sum += s0 + s1;
                     }
-                    sum += s0 + s1;
                 }
+                warp_arrive(&s_empty[s], lane);
             }
-            fence_before_sync();
-            mbar_arrive(&q_empty[s]);
-            mbar_arrive(&s_empty[s]);
+            // the two halves of the rows (a warp that gave up waiting still comes to every barrier)
+            float* xc = xchg + tp * kBM;
+            if (wg == 1) xc[rr] = sum;
+            named_bar_sync(1, 256);
+            if (wg == 0) {
+                sum += xc[rr];
+                if (cluster > 1) xc[rr] = sum;   // (one tile per block then)
+                else if (in && !dead) account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum);
+            }
+            tp ^= 1;
         }
         if (dead && lane == 0) { report_status(status, kDevWaitFull); *abort_flag = 1; }
-        if (wg == 1) xchg[rr] = sum;
-        named_bar_sync(1, 256);
-        if (wg == 0) xchg[rr] += sum;
     }
     __syncwarp();
 
@@ -1033,14 +1097,14 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
     if (cluster > 1) {
         __syncwarp();
         ev::cluster_sync_all();
-    }
-    const int key = kt.tile * kBM + tid;
-    if (rank == 0 && tid < kBM && key < r.kv_len) {
-        float sum = xchg[tid];
-        for (int p = 1; p < cluster; ++p) sum += __uint_as_float(ev::peer_ld(&xchg[tid], uint32_t(p)));
-        account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum);
-    }
-    if (cluster > 1) {
+        const TcKeyTile kt = kt0;
+        const TcReq& r = reqs[kt.req];
+        const int key = kt.tile * kBM + tid;
+        if (rank == 0 && tid < kBM && key < r.kv_len) {
+            float sum = xchg[tid];
+            for (int p = 1; p < cluster; ++p) sum += __uint_as_float(ev::peer_ld(&xchg[tid], uint32_t(p)));
+            account_store(r.acct, page_ids, pool, c.pool_pages, c.num_kv_heads, kt.head, key, sum);
+        }
         __syncwarp();
         ev::cluster_sync_all();   // no block leaves while its sums are read
     }
