@@ -50,8 +50,7 @@ def context(monkeypatch, path, *args, **kw):
     """path: "few", "mid" and "tc" force the f32 kernels, the warp-MMA one and the tcgen05 passes (where the
     shape allows them), "auto" leaves the choice."""
     if path != "auto":
-        monkeypatch.setenv("XORNET_ATTN_READ_TC_MIN_ROWS", "1" if path == "tc" else "1000000000")
-        monkeypatch.setenv("XORNET_ATTN_READ_MID_MIN_ROWS", "1" if path == "mid" else "1000000000")
+        monkeypatch.setenv("XORNET_ATTN_READ_PATH", path)
     return xn.Context(*args, **kw)
 
 

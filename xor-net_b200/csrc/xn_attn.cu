@@ -235,8 +235,7 @@ struct xn_ctx {
     float* read_ws = nullptr; size_t read_ws_cap = 0;      // floats: operand images, scores, partial records
     float* acct_pool = nullptr;                            // account of attention weight, paged like K and V
                                                            // (allocated by the first call that keeps one)
-    int read_mid_min_rows = 5;    // packed rows (rows x heads of a group) from which the mid kernel takes a read
-    int read_tc_min_rows = 65;    // ... from which the tcgen05 passes take it
+    int read_path = 0;            // a ReadPath for all reads of some rows that it can take, or 0: by estimate
     CUtensorMap v_map_rows;       // the V pool like k_map (128-byte swizzle of 16-byte chunks), for the mid kernel
     bool read_funcs_ready = false;
     ReadTable read_table;         // the launch parameter of a read, filled in place
@@ -1872,8 +1871,8 @@ int32_t xn_ctx_create(const xn_ctx_desc* d, xn_ctx** out_ctx) {
     if (const char* env = getenv("XORNET_ATTN_OUTPROJ_PDL")) c->out_pdl = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_OUTPROJ_ROWS")) c->out_rows_kernel = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_PREFILL_PDL")) c->pf_pdl = atoi(env) != 0;
-    if (const char* env = getenv("XORNET_ATTN_READ_TC_MIN_ROWS")) c->read_tc_min_rows = std::max(1, atoi(env));
-    if (const char* env = getenv("XORNET_ATTN_READ_MID_MIN_ROWS")) c->read_mid_min_rows = std::max(1, atoi(env));
+    if (const char* env = getenv("XORNET_ATTN_READ_PATH"))
+        c->read_path = !strcmp(env, "few") ? kPathFew : !strcmp(env, "mid") ? kPathMid : !strcmp(env, "tc") ? kPathTc : kPathAuto;
     if (const char* env = getenv("XORNET_ATTN_F32_TILED")) c->f32_tiled = atoi(env) != 0;
     if (const char* env = getenv("XORNET_ATTN_F32_TILED_MIN_ROWS")) c->f32_tiled_min_rows = std::max(1, atoi(env));
 

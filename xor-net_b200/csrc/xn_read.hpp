@@ -369,11 +369,14 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
     }
     // Small calls: a cluster per (request, KV head), of as many blocks (of 32 positions or more) as there
     // are SMs for, if a block's share of the positions is then small.
-    static const int small_max = getenv("XN_SMALL") ? atoi(getenv("XN_SMALL")) : 128;
+    // (20 query heads over 5, one row: at 1025 positions 14.2 us beside 17.1 with an account and 11.0 beside
+    // 10.8 without; at 2000, 15.5 beside 17.5 and 15.1 beside 14.1 -- the split-KV kernel adds a launch for
+    // the account, and reads faster once every block has a few tiles)
+    const int small_max = want ? 256 : 128;
     if (mt == 0 && c->head_dim <= 128 && n * Hkv <= c->sm_count) {
         int cluster = 1;
         while (cluster < ev::kMaxCluster && n * Hkv * cluster * 2 <= c->sm_count && max_kv > cluster * 32) cluster *= 2;
-        if ((max_kv + cluster - 1) / cluster <= std::min(small_max, rs::kMaxTokens)) {
+        if ((max_kv + cluster - 1) / cluster <= small_max) {
             if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
             XN_CUDA(c, launch_pdl(c, read_small_kernel, dim3(unsigned(n * Hkv * cluster)), rs::kThreads, 0, true, unsigned(cluster), t,
                                   c->k_pool, c->v_pool, c->acct_pool, c->pool_pages, Hkv, c->head_dim, c->nv, c->scale, cluster,
@@ -680,6 +683,43 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     return finish_slot(c, slot);
 }
 
+// Which kernels take the requests of a call that are between a few rows and two tiles of them.  Measured
+// over 1 to 20 requests of 300-2500 positions, head counts 20/5, 32/32 and 16/2 and head sizes 64, 100 and
+// 128, the times follow, in us, with P thousands of (position, KV head) pairs:
+//   split-KV, per row   10 + 0.12 u P           u: passes over the cache, rows x ceil(group / 4)
+//   mid kernel          10 + {0.33, 0.46, 0.6, 0.85} P + (4.5 + 0.27 blocks / units) mt   for mt tiles of 16 rows
+//   tensor-core passes  20 + 0.55 P             (0.28 P up to head size 64)
+// and the account adds about 5 + 2 rows, 6 + 1.5 rows and 5 + 0.17 P to them.
+// e.g. 20 requests x 8 rows, 32/32 heads of 100, 1000 positions: 520 / 212 / 366; 1 x 8 rows, 20/5 of 128,
+// 2000 positions: 19 / 39 / 25; 20 x 12 rows, 20/5 of 128, 1000 positions: 161 / 87 / 81.
+enum ReadPath { kPathAuto = 0, kPathFew, kPathMid, kPathTc };
+struct ReadEstimate {
+    double pairs = 0, few = 0, mid = 0;
+    long long units = 0;
+    int mt = 0, rows = 0;
+    bool want = false;
+    void add(const xn_ctx* c, const ReadSub& s) {
+        const double p = double(s.kv) * c->num_kv_heads * 1e-3;
+        const int m = int((std::min<long long>((long long)s.rows * c->group, 128) + 15) / 16), rt = (m + 3) / 4;
+        static const double rate[5] = {0, 0.33, 0.46, 0.6, 0.85};
+        pairs += p;
+        few += 0.12 * p * s.rows * c->subs;
+        mid += rate[std::min(m, 4)] * rt * p;
+        mt = std::max(mt, std::min(m, 4));
+        units += (long long)c->num_kv_heads * rt;
+        want = want || s.want;
+        rows = std::max(rows, s.rows);
+    }
+    ReadPath best(const xn_ctx* c) const {
+        if (units == 0) return kPathFew;
+        const double f = 10 + few + (want ? 5 + 2 * rows : 0);
+        const double m = 10 + mid + (4.5 + 0.27 * c->sm_count / double(units)) * mt + (want ? 6 + 1.5 * rows : 0);
+        const double t = 20 + (c->head_dim > 64 ? 0.55 : 0.28) * pairs + (want ? 5 + 0.17 * pairs : 0);
+        if (c->kv_u8 || !c->tf32_ok) return f <= t ? kPathFew : kPathTc;   // (the mid kernel: f32 only, by tensor map)
+        return f <= std::min(m, t) ? kPathFew : (m <= t ? kPathMid : kPathTc);
+    }
+};
+
 // Bytes of images, and of scores, that one launch may need at most; more goes out in several.
 constexpr size_t kReadImageBudget = size_t(4) << 30;
 constexpr size_t kReadScoreBudget = size_t(512) << 20;
@@ -723,9 +763,10 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
         if ((rc = grow_io(c, io_in + io_out)) != XN_OK) return rc;
     }
     size_t in_at = 0, out_at = io_in;
-    // [1]: with weights.  table: few rows that all see the whole prefix; few: the others, and the u8 format
-    // mid: the mid kernel's
-    std::vector<ReadSub> table[2], mid[2], few[2], tc;
+    // [1]: with weights.  table: few rows that all see the whole prefix; few: the others, and the u8 format;
+    // mid: the mid kernel's; between: to be dealt out by the estimates
+    std::vector<ReadSub> table[2], mid[2], few[2], tc, between;
+    ReadEstimate estimate;
     struct Zero { float* out; long long o_hs, o_ts; int rows; };
     std::vector<Zero> zeros;
     for (int i = 0; i < n; ++i) {
@@ -771,17 +812,28 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
             if (r.rows > 0) zeros.push_back({s.out, s.o_hs, s.o_ts, r.rows});
             continue;
         }
-        const bool use_tc = D <= 128 && r.rows > 0 &&
-                            ((long long)r.rows * c->group >= c->read_tc_min_rows || (c->kv_u8 && s.want));
-        if (use_tc) {
-            tc.push_back(s);
+        const long long packed = (long long)r.rows * c->group;
+        if (D <= 128 && r.rows > 0 && (c->kv_u8 && s.want)) tc.push_back(s);   // (the only ones for those)
+        else if (D > 128 || r.rows == 0 || (c->read_path == kPathAuto && (long long)r.rows * c->subs <= 2)) few[0].push_back(s);
+        else if (c->read_path == kPathAuto && packed > rt::kBM) tc.push_back(s);
+        else {
+            estimate.add(c, s);
+            between.push_back(s);
+        }
+    }
+    const ReadPath path = c->read_path != kPathAuto ? ReadPath(c->read_path) : estimate.best(c);
+    (path == kPathTc ? tc : few[0]).insert((path == kPathTc ? tc : few[0]).end(), between.begin(), between.end());
+    std::vector<ReadSub> rest;
+    rest.swap(few[0]);
+    for (const ReadSub& s : rest) {
+        const bool fits = !s.want || align_up(size_t(s.kv), 4) * Hq * size_t(s.rows) <= kReadScoreBudget / 4;
+        const bool plain_rows = s.rows > 0 && !c->kv_u8 && fits;
+        if (plain_rows && path == kPathMid && D <= 128 && c->tf32_ok && (c->read_path == kPathMid || (long long)s.rows * c->subs > 2)) {
+            mid[s.want ? 1 : 0].push_back(s);
             continue;
         }
-        const bool fits = !s.want || align_up(size_t(kv), 4) * Hq * size_t(r.rows) <= kReadScoreBudget / 4;
-        const bool use_mid = c->tf32_ok && !c->kv_u8 && r.rows > 0 && (long long)r.rows * c->group >= c->read_mid_min_rows && fits;
-        if (!use_mid && s.causal && r.rows > kv) zeros.push_back({s.out, s.o_hs, s.o_ts, int(r.rows - kv)});
-        if (use_mid) mid[s.want ? 1 : 0].push_back(s);
-        else if (!c->kv_u8 && r.rows > 0 && (!s.causal || r.rows == 1) && fits) table[s.want ? 1 : 0].push_back(s);
+        if (s.causal && s.rows > s.kv) zeros.push_back({s.out, s.o_hs, s.o_ts, int(s.rows - s.kv)});
+        if (plain_rows && (!s.causal || s.rows == 1)) table[s.want ? 1 : 0].push_back(s);
         else few[s.want ? 1 : 0].push_back(s);
     }
     if (host && io_in) {
