@@ -1,0 +1,50 @@
+"""CPU-only checks of the calls that read, write, account and evict without appending: the layout of
+their request structures, and their refusal of handles that are not live."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+import xor_net_b200 as xn
+from xor_net_b200._ffi import EvictReq, ReadReq
+
+
+@pytest.mark.parametrize("struct,name", [(ReadReq, "xn_read_req"), (EvictReq, "xn_evict_req")])
+def test_request_layout_matches_the_header(tmp_path, repo_root, struct, name):
+    fields = [f for f, _ in struct._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "xn_attn.h"\nint main(void) {\n'
+                   f'    printf("%zu", sizeof({name}));\n'
+                   + "".join(f'    printf(" %zu", offsetof({name}, {f}));\n' for f in fields) + "    return 0;\n}\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(repo_root, "include"), "-o", exe, src], check=True)
+    want = [int(x) for x in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    assert [C.sizeof(struct)] + [getattr(struct, f).offset for f in fields] == want
+
+
+def test_flag_values_match_the_header(tmp_path, repo_root):
+    names = ["XN_READ_CAUSAL", "XN_READ_ACCOUNT", "XN_READ_ACCOUNT_SET", "XN_EVICT_COPY"]
+    src = tmp_path / "flags.c"
+    src.write_text('#include <stdio.h>\n#include "xn_attn.h"\nint main(void) {\n'
+                   + "".join(f'    printf("%u ", (unsigned){n});\n' for n in names) + "    return 0;\n}\n")
+    exe = tmp_path / "flags"
+    subprocess.run(["gcc", "-I", os.path.join(repo_root, "include"), "-o", exe, src], check=True)
+    want = [int(x) for x in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    assert [xn.READ_CAUSAL, xn.READ_ACCOUNT, xn.READ_ACCOUNT_SET, xn.EVICT_COPY] == want
+    # none of them is a flag that the appending calls know
+    assert not any(f & (xn.REQ_DEVICE_PTRS | xn.REQ_ROPE | xn.REQ_SEQ_MAJOR) for f in want)
+
+
+def test_contexts_that_are_not_live_are_refused():
+    lib = xn.load()
+    dead = C.create_string_buffer(1 << 16)   # zeros: no context, no stream
+    for ctx in (None, C.cast(dead, C.c_void_p)):
+        read, evict = ReadReq(), EvictReq()
+        assert lib.xn_kv_write(ctx, None, 0, 0, 1, None, None, 0) == 3
+        assert lib.xn_cross_attention(ctx, 1, C.byref(read)) == 3
+        assert lib.xn_cross_attention(ctx, 0, None) == 3
+        assert lib.xn_kv_account_get(ctx, None, 0, 0, 1, None, 0) == 3
+        assert lib.xn_kv_account_set(ctx, None, 0, 0, 1, None, 0) == 3
+        assert lib.xn_kv_evict(ctx, 1, C.byref(evict)) == 3
+        assert lib.xn_stream_evicted(ctx, None, 0) == -1

@@ -334,173 +334,173 @@ splitkv_body(const ReqDev* __restrict__ reqs, const UnitDev* __restrict__ units,
                 cur = unit0 + tile_end;
             }
         } else {
-        const ReqPatchTable& patch = *patch_p;
-        int chunk = blockIdx.x;
-        while (ok && chunk < n_chunks) {
-            const int it_lo = chunk_item_begin[chunk], it_hi = chunk_item_begin[chunk + 1];
-            for (int base = it_lo; base < it_hi && ok; base += 32) {
-                // ---- every lane resolves one item of this batch of 32 ----
-                const int my_it = base + lane;
-                ItemDev item = {0, 0, 0, -1};
-                UnitDev u = {};
-                const float* q_ptr = nullptr;
-                float* o_ptr = nullptr;
-                long long q_hs = 0, o_hs = 0;
-                const int* pages = page_ids;
-                size_t layer_base = 0;
-                const float* k_new = nullptr;  // fused append: the new token's rows of this KV head
-                const float* v_new = nullptr;
-                int fused = 0;                 // bit 0 fused append, bit 1 rotate, bit 2 this unit stores
-                int pos = 0;
-                float* sc_ptr = nullptr;       // EXT: scores and log-sum-exp of the unit's first head
-                float* lse_ptr = nullptr;
-                long long sc_hs = 0, lse_hs = 0;
-                if (my_it < it_hi) {
-                    item = items[my_it];
-                    u = units[item.unit];
-                    const ReqDev& r = reqs[u.req];
-                    // a reused plan: addresses and layer come with the launch
-                    const bool patched = patch.n != 0;
-                    const float* rq = patched ? patch.e[u.req].q : r.q;
-                    const float* rk = patched ? patch.e[u.req].k : r.k;
-                    const float* rv = patched ? patch.e[u.req].v : r.v;
-                    float* ro = patched ? patch.e[u.req].out : r.out;
-                    const int rlayer = patched ? patch.layer : r.layer;
-                    q_ptr = rq + size_t(u.head0) * r.q_hs + size_t(u.t_q) * r.q_ts;
-                    o_ptr = ro + size_t(u.head0) * r.o_hs + size_t(u.t_q) * r.o_ts;
-                    q_hs = r.q_hs;
-                    o_hs = r.o_hs;
-                    pages = page_ids + r.page_off;
-                    layer_base = size_t(rlayer) * size_t(pool_pages);
-                    if (r.flags & 8u) {
-                        k_new = rk + size_t(u.kv_head) * r.kv_hs;
-                        v_new = rv + size_t(u.kv_head) * r.kv_hs;
-                        fused = 1 | ((r.flags & 1u) ? 2 : 0) | (u.store_new ? 4 : 0);
-                        pos = r.index_pos + r.rope_off;
+            const ReqPatchTable& patch = *patch_p;
+            int chunk = blockIdx.x;
+            while (ok && chunk < n_chunks) {
+                const int it_lo = chunk_item_begin[chunk], it_hi = chunk_item_begin[chunk + 1];
+                for (int base = it_lo; base < it_hi && ok; base += 32) {
+                    // ---- every lane resolves one item of this batch of 32 ----
+                    const int my_it = base + lane;
+                    ItemDev item = {0, 0, 0, -1};
+                    UnitDev u = {};
+                    const float* q_ptr = nullptr;
+                    float* o_ptr = nullptr;
+                    long long q_hs = 0, o_hs = 0;
+                    const int* pages = page_ids;
+                    size_t layer_base = 0;
+                    const float* k_new = nullptr;  // fused append: the new token's rows of this KV head
+                    const float* v_new = nullptr;
+                    int fused = 0;                 // bit 0 fused append, bit 1 rotate, bit 2 this unit stores
+                    int pos = 0;
+                    float* sc_ptr = nullptr;       // EXT: scores and log-sum-exp of the unit's first head
+                    float* lse_ptr = nullptr;
+                    long long sc_hs = 0, lse_hs = 0;
+                    if (my_it < it_hi) {
+                        item = items[my_it];
+                        u = units[item.unit];
+                        const ReqDev& r = reqs[u.req];
+                        // a reused plan: addresses and layer come with the launch
+                        const bool patched = patch.n != 0;
+                        const float* rq = patched ? patch.e[u.req].q : r.q;
+                        const float* rk = patched ? patch.e[u.req].k : r.k;
+                        const float* rv = patched ? patch.e[u.req].v : r.v;
+                        float* ro = patched ? patch.e[u.req].out : r.out;
+                        const int rlayer = patched ? patch.layer : r.layer;
+                        q_ptr = rq + size_t(u.head0) * r.q_hs + size_t(u.t_q) * r.q_ts;
+                        o_ptr = ro + size_t(u.head0) * r.o_hs + size_t(u.t_q) * r.o_ts;
+                        q_hs = r.q_hs;
+                        o_hs = r.o_hs;
+                        pages = page_ids + r.page_off;
+                        layer_base = size_t(rlayer) * size_t(pool_pages);
+                        if (r.flags & 8u) {
+                            k_new = rk + size_t(u.kv_head) * r.kv_hs;
+                            v_new = rv + size_t(u.kv_head) * r.kv_hs;
+                            fused = 1 | ((r.flags & 1u) ? 2 : 0) | (u.store_new ? 4 : 0);
+                            pos = r.index_pos + r.rope_off;
+                        }
+                        if constexpr (EXT) {
+                            sc_ptr = r.scores + size_t(u.head0) * r.sc_hs + size_t(u.t_q) * r.sc_ts;
+                            lse_ptr = r.lse + size_t(u.head0) * r.lse_hs + u.t_q;
+                            sc_hs = r.sc_hs;
+                            lse_hs = r.lse_hs;
+                        }
                     }
-                    if constexpr (EXT) {
-                        sc_ptr = r.scores + size_t(u.head0) * r.sc_hs + size_t(u.t_q) * r.sc_ts;
-                        lse_ptr = r.lse + size_t(u.head0) * r.lse_hs + u.t_q;
-                        sc_hs = r.sc_hs;
-                        lse_hs = r.lse_hs;
-                    }
-                }
-                const int n_here = min(32, it_hi - base);
-                for (int k = 0; k < n_here && ok; ++k) {
-                    __syncwarp();
-                    const int tile_begin = __shfl_sync(kFull, item.tile_begin, k);
-                    const int tile_end = __shfl_sync(kFull, item.tile_end, k);
-                    const int kv_len = __shfl_sync(kFull, u.kv_len, k);
-                    const int kv_head = __shfl_sync(kFull, u.kv_head, k);
-                    const unsigned long long pages_k =
-                        __shfl_sync(kFull, reinterpret_cast<unsigned long long>(pages), k);
-                    const unsigned long long lbase_k = __shfl_sync(kFull, (unsigned long long)layer_base, k);
-                    Hdr h;
-                    float* sc_k = nullptr;
-                    if constexpr (EXT) {
-                        sc_k = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(sc_ptr), k));
-                        h.lse = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(lse_ptr), k));
-                        h.sc_hs = __shfl_sync(kFull, sc_hs, k);
-                        h.lse_hs = __shfl_sync(kFull, lse_hs, k);
-                    }
-                    h.q = reinterpret_cast<const float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(q_ptr), k));
-                    h.out = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(o_ptr), k));
-                    h.q_hs = __shfl_sync(kFull, q_hs, k);
-                    h.o_hs = __shfl_sync(kFull, o_hs, k);
-                    h.nheads = __shfl_sync(kFull, u.nheads, k);
-                    h.part = __shfl_sync(kFull, item.part, k);
-                    h.part_begin = __shfl_sync(kFull, u.part_begin, k);
-                    h.part_count = __shfl_sync(kFull, u.part_count, k);
-                    h.merge_slot = __shfl_sync(kFull, u.merge_slot, k);
-                    h.new_key = -1;
-                    h.k_dst = nullptr;
-                    h.v_dst = nullptr;
-                    const int fused_k = __shfl_sync(kFull, fused, k);
-                    const int pos_k = __shfl_sync(kFull, pos, k);
-                    const float* k_new_k = reinterpret_cast<const float*>(
-                        __shfl_sync(kFull, reinterpret_cast<unsigned long long>(k_new), k));
-                    const float* v_new_k = reinterpret_cast<const float*>(
-                        __shfl_sync(kFull, reinterpret_cast<unsigned long long>(v_new), k));
-                    const bool stage_q = Sm::kStageQ && (head_dim % 4 == 0) &&
-                                         ((reinterpret_cast<uintptr_t>(h.q) | uintptr_t(h.q_hs * 4)) & 15) == 0;
-                    const int* pages_ptr = reinterpret_cast<const int*>(pages_k);
-                    for (int tb = tile_begin; tb < tile_end && ok; tb += 32) {
-                        // page ids of the next 32 tiles, one per lane
-                        const int my_tile = tb + lane;
-                        int my_page = 0;
-                        if (my_tile < tile_end) my_page = pages_ptr[(my_tile * TPS) / kPageTokens];
-                        const int n_t = min(32, tile_end - tb);
-                        for (int tt = 0; tt < n_t; ++tt, ++fill) {
-                            __syncwarp();
-                            const int page = __shfl_sync(kFull, my_page, tt);
-                            if (lane == 0) {
-                                const int tile = tb + tt;
-                                const int s = fill % ST;
-                                if (fill >= ST && !XN_DECODE_WAIT(&empty_bar[s], ((fill / ST) - 1) & 1)) {
-                                    report_status(status, kDevWaitEmpty);
-                                    *abort_flag = 1;
-                                    ok = false;
-                                } else if (!XN_PAGE_OK(page, pool_pages)) {
-                                    report_status(status, kDevBadIndex);
-                                    *abort_flag = 1;
-                                    ok = false;
-                                } else {
-                                    const int tok0 = tile * TPS;
-                                    const int ntok = min(TPS, kv_len - tok0);
-                                    const size_t src = ((size_t(lbase_k) + size_t(page)) * num_kv_heads + kv_head) *
-                                                           page_floats +
-                                                       size_t(tok0 % kPageTokens) * dp;
-                                    const bool first = tile == tile_begin;
-                                    // fused append: the tile that ends the unit takes its last
-                                    // row from the request instead of the cache
-                                    const bool has_new = (fused_k & 1) && tok0 + ntok == kv_len;
-                                    const int n_cache = has_new ? ntok - 1 : ntok;
-                                    const uint32_t bytes = uint32_t(n_cache) * dp * 4;
-                                    const uint32_t row_bytes = uint32_t(dp) * 4;
-                                    const bool rope_here = (fused_k & 2) && (first || has_new);
-                                    h.flags = (first ? kHdrFirst : 0) | (tile == tile_end - 1 ? kHdrLast : 0) |
-                                              (first && stage_q ? kHdrQStaged : 0) | ((fused_k & 2) ? kHdrRope : 0);
-                                    h.ntok = ntok;
-                                    h.new_key = has_new ? ntok - 1 : -1;
-                                    h.k_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(k_pool) + src + size_t(ntok - 1) * dp : nullptr;
-                                    h.v_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(v_pool) + src + size_t(ntok - 1) * dp : nullptr;
-                                    if constexpr (EXT) h.scores = sc_k + tok0;
-                                    hdr[s] = h;
-                                    float* dst = stage_ptr(s);
-                                    const uint32_t q_bytes = (first && stage_q) ? uint32_t(h.nheads) * row_bytes : 0u;
-                                    mbar_arrive_expect_tx(&full_bar[s], 2 * bytes + q_bytes + (has_new ? 2 * row_bytes : 0u) +
-                                                                            (rope_here ? row_bytes : 0u));
-                                    if (bytes) {
-                                        bulk_g2s(dst, k_pool + src, bytes, &full_bar[s]);
-                                        bulk_g2s(dst + TPS * NV * 4, v_pool + src, bytes, &full_bar[s]);
-                                    }
-                                    if (has_new) {
-                                        bulk_g2s(dst + size_t(n_cache) * dp, k_new_k, row_bytes, &full_bar[s]);
-                                        bulk_g2s(dst + TPS * NV * 4 + size_t(n_cache) * dp, v_new_k, row_bytes, &full_bar[s]);
-                                    }
-                                    if (q_bytes)
-                                        for (int hh = 0; hh < h.nheads; ++hh)
-                                            bulk_g2s(dst + Cfg::kStageFloats + hh * dp, h.q + size_t(hh) * h.q_hs,
-                                                     row_bytes, &full_bar[s]);
-                                    if (rope_here) {  // cos row then sin row of the token's position
-                                        const int half = head_dim / 2;
-                                        float* cs = dst + Cfg::kStageFloats + GT * NV * 4;
-                                        bulk_g2s(cs, cos_t + size_t(pos_k) * half, row_bytes / 2, &full_bar[s]);
-                                        bulk_g2s(cs + half, sin_t + size_t(pos_k) * half, row_bytes / 2, &full_bar[s]);
+                    const int n_here = min(32, it_hi - base);
+                    for (int k = 0; k < n_here && ok; ++k) {
+                        __syncwarp();
+                        const int tile_begin = __shfl_sync(kFull, item.tile_begin, k);
+                        const int tile_end = __shfl_sync(kFull, item.tile_end, k);
+                        const int kv_len = __shfl_sync(kFull, u.kv_len, k);
+                        const int kv_head = __shfl_sync(kFull, u.kv_head, k);
+                        const unsigned long long pages_k =
+                            __shfl_sync(kFull, reinterpret_cast<unsigned long long>(pages), k);
+                        const unsigned long long lbase_k = __shfl_sync(kFull, (unsigned long long)layer_base, k);
+                        Hdr h;
+                        float* sc_k = nullptr;
+                        if constexpr (EXT) {
+                            sc_k = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(sc_ptr), k));
+                            h.lse = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(lse_ptr), k));
+                            h.sc_hs = __shfl_sync(kFull, sc_hs, k);
+                            h.lse_hs = __shfl_sync(kFull, lse_hs, k);
+                        }
+                        h.q = reinterpret_cast<const float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(q_ptr), k));
+                        h.out = reinterpret_cast<float*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(o_ptr), k));
+                        h.q_hs = __shfl_sync(kFull, q_hs, k);
+                        h.o_hs = __shfl_sync(kFull, o_hs, k);
+                        h.nheads = __shfl_sync(kFull, u.nheads, k);
+                        h.part = __shfl_sync(kFull, item.part, k);
+                        h.part_begin = __shfl_sync(kFull, u.part_begin, k);
+                        h.part_count = __shfl_sync(kFull, u.part_count, k);
+                        h.merge_slot = __shfl_sync(kFull, u.merge_slot, k);
+                        h.new_key = -1;
+                        h.k_dst = nullptr;
+                        h.v_dst = nullptr;
+                        const int fused_k = __shfl_sync(kFull, fused, k);
+                        const int pos_k = __shfl_sync(kFull, pos, k);
+                        const float* k_new_k = reinterpret_cast<const float*>(
+                            __shfl_sync(kFull, reinterpret_cast<unsigned long long>(k_new), k));
+                        const float* v_new_k = reinterpret_cast<const float*>(
+                            __shfl_sync(kFull, reinterpret_cast<unsigned long long>(v_new), k));
+                        const bool stage_q = Sm::kStageQ && (head_dim % 4 == 0) &&
+                                             ((reinterpret_cast<uintptr_t>(h.q) | uintptr_t(h.q_hs * 4)) & 15) == 0;
+                        const int* pages_ptr = reinterpret_cast<const int*>(pages_k);
+                        for (int tb = tile_begin; tb < tile_end && ok; tb += 32) {
+                            // page ids of the next 32 tiles, one per lane
+                            const int my_tile = tb + lane;
+                            int my_page = 0;
+                            if (my_tile < tile_end) my_page = pages_ptr[(my_tile * TPS) / kPageTokens];
+                            const int n_t = min(32, tile_end - tb);
+                            for (int tt = 0; tt < n_t; ++tt, ++fill) {
+                                __syncwarp();
+                                const int page = __shfl_sync(kFull, my_page, tt);
+                                if (lane == 0) {
+                                    const int tile = tb + tt;
+                                    const int s = fill % ST;
+                                    if (fill >= ST && !XN_DECODE_WAIT(&empty_bar[s], ((fill / ST) - 1) & 1)) {
+                                        report_status(status, kDevWaitEmpty);
+                                        *abort_flag = 1;
+                                        ok = false;
+                                    } else if (!XN_PAGE_OK(page, pool_pages)) {
+                                        report_status(status, kDevBadIndex);
+                                        *abort_flag = 1;
+                                        ok = false;
+                                    } else {
+                                        const int tok0 = tile * TPS;
+                                        const int ntok = min(TPS, kv_len - tok0);
+                                        const size_t src = ((size_t(lbase_k) + size_t(page)) * num_kv_heads + kv_head) *
+                                                               page_floats +
+                                                           size_t(tok0 % kPageTokens) * dp;
+                                        const bool first = tile == tile_begin;
+                                        // fused append: the tile that ends the unit takes its last
+                                        // row from the request instead of the cache
+                                        const bool has_new = (fused_k & 1) && tok0 + ntok == kv_len;
+                                        const int n_cache = has_new ? ntok - 1 : ntok;
+                                        const uint32_t bytes = uint32_t(n_cache) * dp * 4;
+                                        const uint32_t row_bytes = uint32_t(dp) * 4;
+                                        const bool rope_here = (fused_k & 2) && (first || has_new);
+                                        h.flags = (first ? kHdrFirst : 0) | (tile == tile_end - 1 ? kHdrLast : 0) |
+                                                  (first && stage_q ? kHdrQStaged : 0) | ((fused_k & 2) ? kHdrRope : 0);
+                                        h.ntok = ntok;
+                                        h.new_key = has_new ? ntok - 1 : -1;
+                                        h.k_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(k_pool) + src + size_t(ntok - 1) * dp : nullptr;
+                                        h.v_dst = (has_new && (fused_k & 4)) ? const_cast<float*>(v_pool) + src + size_t(ntok - 1) * dp : nullptr;
+                                        if constexpr (EXT) h.scores = sc_k + tok0;
+                                        hdr[s] = h;
+                                        float* dst = stage_ptr(s);
+                                        const uint32_t q_bytes = (first && stage_q) ? uint32_t(h.nheads) * row_bytes : 0u;
+                                        mbar_arrive_expect_tx(&full_bar[s], 2 * bytes + q_bytes + (has_new ? 2 * row_bytes : 0u) +
+                                                                                (rope_here ? row_bytes : 0u));
+                                        if (bytes) {
+                                            bulk_g2s(dst, k_pool + src, bytes, &full_bar[s]);
+                                            bulk_g2s(dst + TPS * NV * 4, v_pool + src, bytes, &full_bar[s]);
+                                        }
+                                        if (has_new) {
+                                            bulk_g2s(dst + size_t(n_cache) * dp, k_new_k, row_bytes, &full_bar[s]);
+                                            bulk_g2s(dst + TPS * NV * 4 + size_t(n_cache) * dp, v_new_k, row_bytes, &full_bar[s]);
+                                        }
+                                        if (q_bytes)
+                                            for (int hh = 0; hh < h.nheads; ++hh)
+                                                bulk_g2s(dst + Cfg::kStageFloats + hh * dp, h.q + size_t(hh) * h.q_hs,
+                                                         row_bytes, &full_bar[s]);
+                                        if (rope_here) {  // cos row then sin row of the token's position
+                                            const int half = head_dim / 2;
+                                            float* cs = dst + Cfg::kStageFloats + GT * NV * 4;
+                                            bulk_g2s(cs, cos_t + size_t(pos_k) * half, row_bytes / 2, &full_bar[s]);
+                                            bulk_g2s(cs + half, sin_t + size_t(pos_k) * half, row_bytes / 2, &full_bar[s]);
+                                        }
                                     }
                                 }
+                                ok = __shfl_sync(kFull, ok ? 1 : 0, 0) != 0;
+                                if (!ok) break;
                             }
-                            ok = __shfl_sync(kFull, ok ? 1 : 0, 0) != 0;
-                            if (!ok) break;
                         }
                     }
                 }
+                // next chunk: dynamic
+                int next = 0;
+                if (lane == 0) next = atomicAdd(&sync[kSyncChunk], 1) + int(gridDim.x);
+                chunk = __shfl_sync(kFull, next, 0);
             }
-            // next chunk: dynamic
-            int next = 0;
-            if (lane == 0) next = atomicAdd(&sync[kSyncChunk], 1) + int(gridDim.x);
-            chunk = __shfl_sync(kFull, next, 0);
-        }
         }
         if (lane == 0) {
             if (ok) {

@@ -372,7 +372,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
     // (20 query heads over 5, one row: at 1025 positions 14.2 us beside 17.1 with an account and 11.0 beside
     // 10.8 without; at 2000, 15.5 beside 17.5 and 15.1 beside 14.1 -- the split-KV kernel adds a launch for
     // the account, and reads faster once every block has a few tiles)
-    const int small_max = want ? 256 : 128;
+    const int small_max = want ? rs::kMaxTokens : rs::kMaxTokens / 2;
     if (mt == 0 && c->head_dim <= 128 && n * Hkv <= c->sm_count) {
         int cluster = 1;
         while (cluster < ev::kMaxCluster && n * Hkv * cluster * 2 <= c->sm_count && max_kv > cluster * 32) cluster *= 2;

@@ -1,14 +1,16 @@
-// A read of some query rows (about 5 to 64 per KV head with the heads of its group) over an f32 cache:
-// few enough that the read of K and V bounds it, too many for the split-KV kernel, which goes over the
-// cache once per row and four heads.
+// A read of some query rows (a few to about 48 per KV head with the heads of its group) over an f32 cache:
+// few enough that the read of K and V should bound it, too many for the split-KV kernel, which goes over
+// the cache once per row and four heads.
 //
 // Bulk tensor copies bring 64-token tiles of K and V as they are (f32) into a ring of shared-memory
 // stages; eight warps do the arithmetic with warp-level MMAs (m16n8k16, f16 in, f32 accumulators)
 // on operands split into two f16 values as in xn_read_tc.cuh -- three products, 22 bits -- but
 // converted here, in registers, so that nothing is written back and read again: a conversion pass of
-// its own would move as many bytes as the whole read.  (The tcgen05 MMAs want their operands in shared
-// memory or tensor memory in f16, i.e. that pass; at this few rows their rate is not needed: the
-// warps' MMAs take less time than the copies.)
+// its own moves twice the bytes of the whole read.  (The tcgen05 MMAs want their operands in shared
+// memory or tensor memory in f16, i.e. that pass.  Two forms of the tcgen05 kernel whose own warps
+// converted each tile took 90 to 110 us where this one takes 40 to 60: every converted element goes
+// through a chain of load, maximum over the rows that share a scale, split and store, and with 4 or 8
+// warps per SM that chain's latency, 2000 cycles per 8 KB, is what one waits for.)
 //
 //   S = Q K^T   warp w owns positions [8 w, 8 w + 8) of the tile, all rows: it converts them once, with a
 //               scale of their own;
@@ -22,6 +24,11 @@
 // tile.  Work is cut as in the table form of the split-KV kernel: block b of G takes an equal share of
 // the tiles of all (request, KV head, row tile) units; the block that delivers a cut unit's last
 // partial record combines them.
+//
+// Measured: 6000 cycles per 64-token tile for up to 16 rows (8500 instructions over the eight warps; two
+// warps per scheduler wait for one another's latencies), i.e. 3.1 TB/s; 20 requests of 500-1500
+// positions, 20/5 heads of 128, 4 rows each (16 per KV head): 48 us, the split-KV kernel 64, the
+// tensor-core passes 80.
 #pragma once
 #include <cuda.h>
 
@@ -37,9 +44,9 @@ constexpr int kSub = 8192;                // a column block: 64 rows of 128 byte
 __host__ __device__ constexpr int stages(int mt) { return mt <= 2 ? 3 : 2; }
 __host__ __device__ constexpr int rows(int mt) { return 16 * mt; }
 __host__ __device__ constexpr size_t smem_bytes(int mt) {
-    // stages | Q hi, lo (later the O of the upper position half) | P hi, lo | maxima | row factors, sums | barriers
+    // stages | Q hi, lo (later the O of the upper position half) | P hi, lo | maxima, sums by warp | row factors, maxima | barriers
     return size_t(stages(mt)) * kStageBytes + size_t(rows(mt)) * 512 + size_t(rows(mt)) * 256 + size_t(rows(mt)) * 32 +
-           size_t(rows(mt)) * 8 * 4 + 512;
+           size_t(rows(mt)) * 2 * 4 + 512;
 }
 __host__ __device__ constexpr size_t part_floats(int mt, int dp) { return size_t(rows(mt)) * (size_t(dp) + 2); }
 
@@ -95,9 +102,8 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
     unsigned char* p_s = q_s + size_t(R) * 512;                        // [hi | lo][R][128 bytes]
     float* xm = reinterpret_cast<float*>(p_s + size_t(R) * 256);       // [R][8]
     float* cq_s = xm + R * 8;                                          // [R] row factors
-    float* l_s = cq_s + R;                                             // [R] sums, one per warp half would do
-    float* m_s = l_s + R;                                              // [R]
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(m_s + 6 * R);
+    float* m_s = cq_s + R;                                             // [R] maxima
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(m_s + R);
     uint64_t* empty_bar = full_bar + ST;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(empty_bar + ST);
     volatile int* last_flag = abort_flag + 1;

@@ -8,7 +8,8 @@
 // are wanted.  One launch, no partial records, no counters in global memory.  What it is made of is
 // latencies of 300 to 1200 cycles, about 6000 cycles in all, so loads are issued together and
 // nothing is read remotely.  (A version whose blocks pulled their peers' states, with a barrier
-// before and behind, took 13000 cycles; the split-KV kernel and its second launch take 16000.)
+// before and behind, took 13000 cycles.)  197 positions, 20/5 heads of 128, one row: 6.7 us; 1025 with
+// an account: 12.0 us (the split-KV kernel and the account's launch: 17).
 #pragma once
 #include "xn_decode.cuh"
 #include "xn_evict.cuh"
@@ -20,7 +21,7 @@ namespace rs {
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHeads = 4;             // heads per pass over the rows
-constexpr int kMaxTokens = 512;       // positions of one block
+constexpr int kMaxTokens = 256;       // positions of one block
 constexpr int kKeys = 4;              // pairs of keys that a warp has in flight
 constexpr int kAhead = 8;             // rows of V that a warp has in flight
 
