@@ -545,25 +545,43 @@ int32_t launch_read_few(xn_ctx* c, const std::vector<ReadSub>& subs, bool want) 
 
 // How the row tiles of a launch are cut along the cache: with fewer tiles than SMs, or a last round
 // of blocks that leaves most SMs idle, tiles are split into ranges of pages whose partial results
-// are merged.  Every candidate piece size is rated by its rounds of blocks times the piece's
-// duration, in units of one 128-position tile; a split block costs about as much again as
-// kReadPieceCost tiles (query load, partial record, merge).
-constexpr double kReadPieceCost = 2.0;
+// are merged.  Every candidate piece size is rated by dealing its pieces out to the SMs, longest first
+// and every other round from the end, which is nearly what the hardware does.  In units of one
+// 128-position tile (2.7 us): a block costs kReadBlockCost beside its tiles, a split one kReadSplitCost
+// more, and the merge its launch and two transfers of 64 KB per piece.  (Against a rating by rounds of
+// blocks times their mean load: 4 x 37 rows over 130-1501 positions, 32 heads: 12.6 units for 15.0;
+// 1024 rows over 8192 positions, 32/8 heads: 135 without a merge for 140 and a merge of 1024 pieces.)
+constexpr double kReadBlockCost = 3.6, kReadSplitCost = 0.4, kReadMergeCost = 1.1, kReadPieceCost = 0.007;
 int read_piece_tiles(const std::vector<int>& tiles, int sms) {
-    long long total = 0;
     int longest = 1;
-    for (int t : tiles) { total += t; longest = std::max(longest, t); }
+    for (int t : tiles) longest = std::max(longest, t);
+    std::vector<int> whole(size_t(longest) + 1), parts(size_t(longest) + 1);
+    std::vector<double> load(static_cast<size_t>(sms));
     int best = longest;
     double best_cost = -1;
     for (int piece = longest;; piece = std::max(1, piece * 7 / 8)) {
-        long long pieces = 0, sum = 0;
-        for (int t : tiles) { const int n = (t + piece - 1) / piece; pieces += n; sum += t; }
-        const double over = pieces > (long long)tiles.size() ? kReadPieceCost : kReadPieceCost / 2;
-        // blocks go out heaviest first: no worse than the mean load plus one piece, no better than either
-        const double mean = double(sum) / double(pieces) + over;
-        const double rounds = std::ceil(double(pieces) / sms);
-        const double cost = std::max({rounds * mean, double(std::min(piece, longest)) + over});
-        if (best_cost < 0 || cost < best_cost * 0.98) { best_cost = cost; best = piece; }
+        std::fill(whole.begin(), whole.end(), 0);
+        std::fill(parts.begin(), parts.end(), 0);
+        long long n_parts = 0;
+        for (int t : tiles) {
+            const int n = (t + piece - 1) / piece;
+            if (n == 1) {
+                ++whole[size_t(t)];
+                continue;
+            }
+            n_parts += n;   // t % n pieces of t / n + 1 tiles, the others of t / n
+            parts[size_t(t / n)] += n - t % n;
+            if (t % n) parts[size_t(t / n + 1)] += t % n;
+        }
+        std::fill(load.begin(), load.end(), 0.0);
+        long long at = 0;
+        for (int t = longest; t >= 0; --t)
+            for (int k = 0; k < whole[size_t(t)] + parts[size_t(t)]; ++k, ++at) {
+                const long long lane = at % sms;
+                load[size_t((at / sms) & 1 ? sms - 1 - lane : lane)] += t + kReadBlockCost + (k < parts[size_t(t)] ? kReadSplitCost : 0);
+            }
+        const double cost = *std::max_element(load.begin(), load.end()) + (n_parts ? kReadMergeCost + kReadPieceCost * double(n_parts) : 0);
+        if (best_cost < 0 || cost < best_cost * 0.99) { best_cost = cost; best = piece; }
         if (piece <= 2) break;
     }
     return best;
