@@ -288,6 +288,28 @@ def test_values_over_many_orders_of_magnitude(monkeypatch, path):
 
 
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
+@pytest.mark.parametrize("n,R", [(3, 4), (200, 9), (2000, 40)])
+def test_scores_of_minus_infinity_throughout_are_no_numbers(monkeypatch, path, n, R):
+    """0 / 0, as in a plain softmax; the causal rows that see nothing stay zeros."""
+    rng = np.random.default_rng(n)
+    ctx = context(monkeypatch, path, 1, 4, 2, 64, pool_pages=64)
+    st = ctx.new_stream(n)
+    k, v = rows(rng, 2, n, 64), rows(rng, 2, n, 64)
+    k[0, :, 5] = -np.inf
+    st.write(0, 0, k, v)
+    q = np.abs(rows(rng, 4, R, 64)) + 0.1
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+    none = max(0, R - n)
+    assert np.all(out[:, :none] == 0)
+    assert np.all(np.isnan(out[:2, none:])) and np.all(np.isnan(w[0]))
+    with np.errstate(invalid="ignore"):
+        want, ww = plain(q, k, v, causal=True)
+    near(out[2:], want[2:], "the other head")
+    near(w[1], ww[1], "its weights", abs_tol=4e-6 * R * 2)
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 def test_infinities_and_nan_stay_where_they_are_seen(monkeypatch, path, value):
     rng = np.random.default_rng(4)

@@ -701,7 +701,8 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     return finish_slot(c, slot);
 }
 
-// Which kernels take the requests of a call that are between a few rows and two tiles of them.  Measured
+// Which kernels take the requests of a call that have more than a row or two but no more than 128 packed
+// ones (rows x heads of a group).  Measured
 // over 1 to 20 requests of 300-2500 positions, head counts 20/5, 32/32 and 16/2 and head sizes 64, 100 and
 // 128, the times follow, in us, with P thousands of (position, KV head) pairs:
 //   split-KV, per row   10 + 0.12 u P           u: passes over the cache, rows x ceil(group / 4)

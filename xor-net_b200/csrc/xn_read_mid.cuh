@@ -135,7 +135,7 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
         // =============================== copies ===============================
         if (lane == 0) {
             bool ok = true;
-            int fill = 0, rq = 0;
+            int fill = 0, rq = 0, issued = 0;
             for (long long cur = t_lo; cur < t_hi && ok; ++cur, ++fill) {
                 while (rq + 1 < tab.n && cur >= tab.e[rq + 1].tile0) ++rq;
                 const ReadEntry& e = tab.e[rq];
@@ -157,11 +157,14 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                 const int row = int(((long long)e.layer * pool_pages + page) * num_kv_heads + h) * kPageTokens;
                 unsigned char* at = mid_smem + size_t(s) * kStageBytes;
                 mbar_arrive_expect_tx(&full_bar[s], uint32_t(2 * n_kb) * kSub);
+                ++issued;
                 for (int kb = 0; kb < n_kb; ++kb) pf::tma_load_2d(at + kb * kSub, &k_map, kb * 32, row, &full_bar[s]);
                 for (int kb = 0; kb < n_kb; ++kb) pf::tma_load_2d(at + kTileBytes + kb * kSub, &v_map, kb * 32, row, &full_bar[s]);
                 if (*abort_flag) break;
             }
             if (!ok) *abort_flag = 1;
+            if (*abort_flag)   // nobody may be waiting for them any more: no copy outlives the block
+                for (int f = max(0, issued - ST); f < issued; ++f) mbar_spin_bounded(&full_bar[f % ST], uint32_t((f / ST) & 1));
         }
         return;
     }
@@ -533,14 +536,14 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                     const float4 a = *reinterpret_cast<const float4*>(xm + rr * 8), b = *reinterpret_cast<const float4*>(xm + rr * 8 + 4);
                     const float l = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
                     if (p >= n_packed) continue;
-                    const float inv = whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+                    const float inv = whole ? (limit[mt][hf] <= 0 ? 0.f : 1.0f / l) : 1.0f;   // (scores of -inf throughout: NaN)
                     const int head = h * tab.group + p % tab.group, t = p / tab.group;
                     if (cbw == 0 && t4 == 0) {
                         if (!whole) {
                             rec[size_t(R) * dp + rr] = m_s[rr];
                             rec[size_t(R) * dp + R + rr] = l;
                         } else if (want) {
-                            e.lse[(long long)head * e.lse_hs + t] = l == 0.f ? INFINITY : (m_s[rr] + log2f(l)) * kLn2;
+                            e.lse[(long long)head * e.lse_hs + t] = limit[mt][hf] <= 0 ? INFINITY : (m_s[rr] + log2f(l)) * kLn2;
                         }
                     }
                     if (!my_cols) continue;
@@ -597,11 +600,12 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                 x.z = fmaf(wgt, y.z, x.z);
                 x.w = fmaf(wgt, y.w, x.w);
             }
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int head = h * tab.group + p % tab.group, t = p / tab.group;
+            const bool sees = !e.causal || e.kv_len - e.rows + t >= 0;
+            const float inv = sees ? 1.0f / l : 0.f;
             float* row = e.out + (long long)head * e.o_hs + (long long)t * e.o_ts + ch * 4;
             row[0] = x.x * inv; row[1] = x.y * inv; row[2] = x.z * inv; row[3] = x.w * inv;
-            if (want && ch == 0) e.lse[(long long)head * e.lse_hs + t] = l == 0.f ? INFINITY : (m + log2f(l)) * kLn2;
+            if (want && ch == 0) e.lse[(long long)head * e.lse_hs + t] = sees ? (m + log2f(l)) * kLn2 : INFINITY;
         }
     }
 }

@@ -450,10 +450,12 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             const unsigned char* base = images + size_t(img0) * img_bytes;
             mbar_arrive_expect_tx(q_full, uint32_t(q_image_bytes(D)));
             bulk_g2s(q_s, q_images + size_t(qid) * q_image_bytes(D), uint32_t(q_image_bytes(D)), q_full);
+            int k_tiles[2] = {0, 0}, v_pages = 0;          // asked for so far
             auto load_k = [&](int j, int part) -> bool {   // part 0: lo, 1: hi
                 if (j > 0 && !mbar_spin_bounded(&k_empty[part], uint32_t((j - 1) & 1))) return false;
                 const int np = min(2, n_pages - 2 * j), b0 = part ? 0 : nb;
                 mbar_arrive_expect_tx(&k_full[part], uint32_t(np * nb) * kSub);
+                ++k_tiles[part];
                 for (int p = 0; p < np; ++p)
                     for (int b = b0; b < b0 + nb; ++b)
                         bulk_g2s(k_s + size_t(b) * kRowsSub + size_t(p) * kSub,
@@ -465,6 +467,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 if (pg >= kVStages && !mbar_spin_bounded(&v_empty[st], uint32_t((pg / kVStages - 1) & 1))) return false;
                 const uint32_t bytes = uint32_t(2 * nb) * kSub;
                 mbar_arrive_expect_tx(&v_full[st], bytes);
+                ++v_pages;
                 bulk_g2s(v_s + size_t(st) * kVBytes, base + size_t(pg) * step + size_t(2 * nb) * kSub, bytes, &v_full[st]);
                 return true;
             };
@@ -475,6 +478,13 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 if (*abort_flag) break;
             }
             if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
+            if (*abort_flag) {   // nobody may be waiting for them any more: no copy outlives the block
+                mbar_spin_bounded(q_full, 0);
+                for (int part = 0; part < 2; ++part)
+                    if (k_tiles[part]) mbar_spin_bounded(&k_full[part], uint32_t((k_tiles[part] - 1) & 1));
+                for (int pg = max(0, v_pages - kVStages); pg < v_pages; ++pg)
+                    mbar_spin_bounded(&v_full[pg % kVStages], uint32_t((pg / kVStages) & 1));
+            }
         }
     } else if (warp == 1) {
         // =============================== MMA issuer ===============================
@@ -754,13 +764,13 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             wg_barrier();
             const float l_tot = l_sum + xc[(wg ^ 1) * 128 + rr];
             const bool whole = it.part < 0;
-            const float inv = whole ? (l_tot == 0.f ? 0.f : 1.0f / l_tot) : 1.0f;
+            const float inv = whole ? (limit <= 0 ? 0.f : 1.0f / l_tot) : 1.0f;   // (scores of -inf throughout: NaN)
             if (wg == 0) {
                 if (!whole) {
                     float* rec = partials + size_t(it.part) * part_floats(c.nv * 4) + size_t(kBM) * c.nv * 4;
                     rec[rr] = m_ref;
                     rec[kBM + rr] = l_tot;
-                } else if (want_lse && pr < n_packed && l_tot != 0.f) {
+                } else if (want_lse && limit > 0) {
                     row_meta[size_t(qid) * kBM + rr].y = m_ref + log2f(l_tot);
                 }
             }
@@ -841,14 +851,15 @@ read_merge_kernel(const TcReq* __restrict__ reqs, const TcMerge* __restrict__ me
             o.w = fmaf(w, x.w, o.w);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const bool sees = !r.causal || r.kv_len - r.rows + p / group >= 0;
+    const float inv = sees ? 1.0f / l : 0.f;
     float* row = r.out + size_t(mg.head * group + p % group) * r.o_hs + size_t(p / group) * r.o_ts;
     const int d = lane * 4;
     if (d + 0 < head_dim) row[d + 0] = o.x * inv;
     if (d + 1 < head_dim) row[d + 1] = o.y * inv;
     if (d + 2 < head_dim) row[d + 2] = o.z * inv;
     if (d + 3 < head_dim) row[d + 3] = o.w * inv;
-    if (want_lse && lane == 0 && l != 0.f)
+    if (want_lse && lane == 0 && sees)
         row_meta[size_t(r.qimg0 + (long long)mg.head * r.n_qt + mg.qt) * kBM + i].y = m + log2f(l);
 }
 
@@ -977,6 +988,9 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
                 if (*abort_flag) break;
             }
             if (!ok) { report_status(status, kDevWaitEmpty); *abort_flag = 1; }
+            if (*abort_flag)     // (as above)
+                for (int s = 0; s < kAcctStages; ++s)
+                    if (used >> s & 1u) mbar_spin_bounded(&full[s], (odd >> s & 1u) ^ 1u);
         }
     } else if (warp == 1) {
         if (lane == 0) {
