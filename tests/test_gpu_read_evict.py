@@ -713,3 +713,64 @@ def test_reads_between_appends_see_what_was_appended():
     q = rows(rng, Hq, 3, D)
     near(ctx.cross_attention([st], 0, [q])[0], plain(q, kk, vv)[0])
     ctx.close()
+
+
+@pytest.mark.parametrize("R", [24, 40, 75])
+def test_account_of_more_key_tiles_than_blocks(monkeypatch, R):
+    """Resident blocks take several key tiles each, with one, two or three tiles of query rows to a key tile."""
+    rng = np.random.default_rng(R)
+    ctx = context(monkeypatch, "tc", 1, 16, 4, 64, pool_pages=400, shuffle_seed=3)
+    made = [filled(ctx, rng, n) for n in (2900, 5001, 3333)]
+    qs = [rows(rng, 16, R, 64) for _ in made]
+    got, w = ctx.cross_attention([st for st, _, _ in made], 0, qs, causal=True, weights=True, account="set")
+    for (st, k, v), q, out, acct in zip(made, qs, got, w):
+        want, want_w = plain(q, k, v, causal=True)
+        near(out, want)
+        near(acct, want_w, abs_tol=ABS)
+        assert np.array_equal(st.account(0, 0, k.shape[1]), acct)
+    ctx.close()
+
+
+@pytest.mark.parametrize("account", [None, "add"])
+def test_many_requests_of_all_sizes_in_one_call(account):
+    rng = np.random.default_rng(12)
+    ctx = xn.Context(1, 6, 2, 64, pool_pages=600, shuffle_seed=2)
+    sizes = [(int(n), int(r)) for n, r in zip(rng.integers(1, 400, 90), rng.choice([1, 1, 1, 2, 5, 17, 60], 90))] + [(130, 0), (200, 100)]
+    made = [filled(ctx, rng, n) for n, _ in sizes]
+    qs = [rows(rng, 6, r, 64) for _, r in sizes]
+    for turn in range(2):
+        got, w = ctx.cross_attention([st for st, _, _ in made], 0, qs, weights=True, account=account)
+        for (n, r), (st, k, v), q, out, acct in zip(sizes, made, qs, got, w):
+            want, want_w = plain(q, k, v)
+            if r:
+                near(out, want, f"n={n} r={r}")
+            times = turn + 1 if account else 1
+            near(acct, want_w * times, f"account n={n} r={r}", abs_tol=ABS * 3 * max(1, r)) if r else np.testing.assert_array_equal(acct, 0.0)
+    ctx.close()
+
+
+def test_captured_attention_replays_after_reads_and_evictions():
+    """A graph of another library's work on the caller's stream is not disturbed by calls made in between."""
+    import torch
+
+    rng = np.random.default_rng(5)
+    ctx = xn.Context(1, 4, 2, 64, pool_pages=64)
+    st, k, v = filled(ctx, rng, 300)
+    q = torch.from_numpy(rows(rng, 4, 3, 64)).cuda()
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    x = torch.arange(64.0, device="cuda")
+    with torch.cuda.stream(side):
+        y = x * 2
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            y.copy_(x * 3)
+    # the context's own stream is not the captured one: its calls go on
+    ctx.submit_reads(ctx.make_read_batch([(st, 0, 3, 300, q.data_ptr(), out.data_ptr(), None, 0)], xn.REQ_DEVICE_PTRS))
+    g.replay()
+    ctx.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(y, x * 3)
+    near(out.cpu().numpy(), plain(q.cpu().numpy(), k, v)[0])
+    ctx.close()
