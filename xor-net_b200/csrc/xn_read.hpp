@@ -711,6 +711,8 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
 // and the account adds about 5 + 2 rows, 6 + 1.5 rows and 5 + 0.17 P to them.
 // e.g. 20 requests x 8 rows, 32/32 heads of 100, 1000 positions: 520 / 212 / 366; 1 x 8 rows, 20/5 of 128,
 // 2000 positions: 19 / 39 / 25; 20 x 12 rows, 20/5 of 128, 1000 positions: 161 / 87 / 81.
+// Over the u8 format, which the mid kernel does not read: 30 + 0.05 u P, and 20 + 0.75 P (0.45 P up to
+// head size 64); e.g. 20 x 8 rows, 20/5 of 128, 1000 positions: 71 / 89, x 20 rows: 141 / 90.
 enum ReadPath { kPathAuto = 0, kPathFew, kPathMid, kPathTc };
 struct ReadEstimate {
     double pairs = 0, few = 0, mid = 0;
@@ -734,7 +736,8 @@ struct ReadEstimate {
         const double f = 10 + few + (want ? 5 + 2 * rows : 0);
         const double m = 10 + mid + (4.5 + 0.27 * c->sm_count / double(units)) * mt + (want ? 6 + 1.5 * rows : 0);
         const double t = 20 + (c->head_dim > 64 ? 0.55 : 0.28) * pairs + (want ? 5 + 0.17 * pairs : 0);
-        if (c->kv_u8 || !c->tf32_ok) return f <= t ? kPathFew : kPathTc;   // (the mid kernel: f32 only, by tensor map)
+        if (c->kv_u8) return 30 + few * (0.05 / 0.12) <= 20 + (c->head_dim > 64 ? 0.75 : 0.45) * pairs ? kPathFew : kPathTc;
+        if (!c->tf32_ok) return f <= t ? kPathFew : kPathTc;   // (the mid kernel reads by tensor map)
         return f <= std::min(m, t) ? kPathFew : (m <= t ? kPathMid : kPathTc);
     }
 };

@@ -93,7 +93,7 @@ constexpr int kQBytes = 4 * kRowsSub;    // 64 KB: hi and lo, two column blocks
 constexpr int kKBytes = 4 * kRowsSub;
 constexpr int kVBytes = 4 * kSub;        // 32 KB
 constexpr int kSmemData = kQBytes + kKBytes + kVStages * kVBytes;
-constexpr int kSmemBytes = kSmemData + 3072;   // 227 KB, all there is: the block's window starts 1024-byte aligned
+constexpr int kSmemBytes = kSmemData + 3 * 1024;   // 227 KB, all there is: the block's window starts 1024-byte aligned
 static_assert(kSmemBytes <= 232448, "shared memory of a block");
 constexpr int kTmemS = 0;                // 2 x 128 columns
 constexpr int kTmemO = 256;              // P_hi V_hi, then P_hi V_lo + P_lo V_hi: up to 128 columns each
