@@ -686,10 +686,13 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     if (!merges.empty())
         XN_CUDA(c, launch_pdl(c, read_merge_kernel, dim3(unsigned(merges.size()), rt::kBM / 8), 256, 0, true, 0, reqs_d,
                               reinterpret_cast<const TcMerge*>(slot->dev + o_merge), parts, row_meta, G, D, c->nv, want ? 1 : 0));
-    // a cluster of blocks per key tile while that still adds SMs and leaves each block two row tiles
+    // a cluster of blocks per key tile while a quarter of the SMs would have nothing to do, and each block is
+    // left two row tiles (prompts of 600 over 8 heads 50 us, 4 of 300 over 2 heads 68, one of 2000 over 2 heads
+    // 130, one of 2048 over 5 heads 156; doubling until there are two rounds of blocks 61, 81, 122 and 153;
+    // only up to half the SMs 56, 64, 130 and 207)
     int cluster = 1, most_qt = 0;
     for (const TcReq& r : reqs) most_qt = std::max(most_qt, r.n_qt);
-    while (cluster < ev::kMaxCluster && (long long)key_tiles.size() * cluster < 2 * c->sm_count && most_qt >= 4 * cluster) cluster *= 2;
+    while (cluster < ev::kMaxCluster && (long long)key_tiles.size() * cluster * 4 < 3 * c->sm_count && most_qt >= 4 * cluster) cluster *= 2;
     if (want) {
         const int blocks = cluster > 1 ? int(key_tiles.size()) * cluster : std::min<int>(int(key_tiles.size()), c->sm_count);
         XN_CUDA(c, launch_pdl(c, account_tc_kernel, dim3(unsigned(blocks)), rt::kThreads, size_t(rt::kAcctSmemBytes), true,
