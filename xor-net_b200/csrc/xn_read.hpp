@@ -679,7 +679,7 @@ int32_t launch_read_tc(xn_ctx* c, const std::vector<ReadSub>& subs) {
     const float scale_log2 = c->scale * 1.4426950408889634f;
     if (c->profile && (rc = profile_begin(c, 1)) != XN_OK) return rc;
     XN_CUDA(c, launch_pdl(c, page_images_kernel, dim3(unsigned(2 * (n_img + n_qimg))), 256, 0, true, 0, reqs_d, int(subs.size()), n_img,
-                          pages_d, view, img, meta, qimg, row_meta, scale_log2, G));
+                          pages_d, view, img, meta, qimg, row_meta, scale_log2, G, c->status_d));
     XN_CUDA(c, launch_pdl(c, read_tc_kernel, dim3(unsigned(items.size())), rt::kThreads, size_t(rt::kSmemBytes), true, 0, reqs_d,
                           reinterpret_cast<const TcItem*>(slot->dev + o_item), pages_d, view, img, meta, qimg, row_meta,
                           parts, scale_log2, G, want ? 1 : 0, c->status_d));

@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256, 4)
 page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages,
                    const int* __restrict__ page_ids, CacheView c, unsigned char* __restrict__ images,
                    PageMeta* __restrict__ meta, unsigned char* __restrict__ q_images,
-                   float2* __restrict__ row_meta, float scale_log2, int group) {
+                   float2* __restrict__ row_meta, float scale_log2, int group, int* __restrict__ status) {
     using namespace rt;
     pdl_launch_dependents();
     __shared__ __align__(16) float s_max[8];
@@ -278,8 +278,11 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
     if (!is_q) {
         const long long local = id - r.img0;
         const int page = int(local / c.num_kv_heads), h = int(local % c.num_kv_heads);
-        const int ntok = min(kPage, r.kv_len - page * kPage);
-        const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_ids[r.page_off + page])) * c.num_kv_heads + h;
+        const int page_id = page_ids[r.page_off + page];
+        const bool page_ok = XN_PAGE_OK(page_id, c.pool_pages);
+        if (!page_ok && threadIdx.x == 0) report_status(status, kDevBadIndex);
+        const int ntok = page_ok ? min(kPage, r.kv_len - page * kPage) : 0;
+        const size_t blk = (size_t(r.layer) * size_t(c.pool_pages) + size_t(page_id)) * c.num_kv_heads + h;
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
