@@ -170,6 +170,34 @@ def test_batches_share_streams_mix_lengths_and_leave_neighbours_alone(monkeypatc
 
 
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
+@pytest.mark.parametrize("lens", [(100, 5000), (5000, 100), (4096, 4097), (4097, 4096)])
+def test_one_stream_with_a_short_and_a_long_prefix_in_one_call(monkeypatch, path, lens):
+    """The prefixes lie on both sides of 64 pages, where the stream's page table on the device grows; the
+    streams between and behind would take the place of a table that went away.  In another layer and in
+    the second round (tables there already) as well."""
+    rng = np.random.default_rng(lens[0])
+    Hq, Hkv, D, n = 4, 2, 64, 5000
+    for R, weights in [(1, False), (1, True), (9, False), (9, True)]:
+        ctx = context(monkeypatch, path, 2, Hq, Hkv, D, pool_pages=90, shuffle_seed=5)
+        st, k, v = filled(ctx, rng, n)
+        k1, v1 = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D)
+        st.write(1, 0, k1, v1)
+        b, kb, vb = filled(ctx, rng, 100)
+        c, kc, vc = filled(ctx, rng, 77)
+        entries = [(st, 0, lens[0], k, v), (b, 0, 100, kb, vb), (st, 0, lens[1], k, v), (c, 0, 77, kc, vc), (st, 1, lens[0], k1, v1)]
+        qs = [rows(rng, Hq, R, D) for _ in entries]
+        for turn in range(2):
+            got = ctx.cross_attention([e[0] for e in entries], [e[1] for e in entries], qs, kv_lens=[e[2] for e in entries], weights=weights)
+            outs, ws = got if weights else (got, [None] * len(entries))
+            for (_, layer, m, kk, vv), q, out, w in zip(entries, qs, outs, ws):
+                want, want_w = plain(q, kk[:, :m], vv[:, :m])
+                near(out, want, f"R={R} m={m} layer={layer} turn={turn}")
+                if weights:
+                    near(w, want_w, f"weights R={R} m={m} layer={layer} turn={turn}", abs_tol=ABS * R)
+        ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_account_adds_up_is_set_and_follows_writes(monkeypatch, path):
     rng = np.random.default_rng(8)
     Hq, Hkv, D, n = 6, 3, 64, 150

@@ -309,8 +309,10 @@ int32_t ready_read_kernels(xn_ctx* c) {
     return XN_OK;
 }
 
-// The stream's page table on the device, at least its first n entries.
-int32_t device_pages(xn_ctx* c, xn_stream* s, size_t n, const int** out) {
+// The stream's page table on the device: all of it, whatever part the caller reads, so that a stream
+// that occurs several times in a call has one address there (no page comes or goes during a read).
+int32_t device_pages(xn_ctx* c, xn_stream* s, const int** out) {
+    const size_t n = s->pages.size();
     if (n > s->pages_d_cap) {
         XN_CUDA(c, cudaStreamSynchronize(c->stream));   // launches in flight may still read the old one
         XN_CUDA(c, guarded_free(c, s->pages_d));
@@ -322,10 +324,9 @@ int32_t device_pages(xn_ctx* c, xn_stream* s, size_t n, const int** out) {
     }
     if (n > s->pages_d_valid) {
         // pageable memory: the call returns when the entries have been taken
-        const size_t to = std::min(s->pages.size(), s->pages_d_cap);
-        XN_CUDA(c, cudaMemcpyAsync(s->pages_d + s->pages_d_valid, s->pages.data() + s->pages_d_valid, (to - s->pages_d_valid) * 4,
+        XN_CUDA(c, cudaMemcpyAsync(s->pages_d + s->pages_d_valid, s->pages.data() + s->pages_d_valid, (n - s->pages_d_valid) * 4,
                                    cudaMemcpyHostToDevice, c->stream));
-        s->pages_d_valid = to;
+        s->pages_d_valid = n;
     }
     *out = s->pages_d;
     return XN_OK;
@@ -350,7 +351,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
         ReadEntry& e = t.e[i];
         e.q = s.q; e.q_hs = s.q_hs; e.q_ts = s.q_ts;
         e.out = s.out; e.o_hs = s.o_hs; e.o_ts = s.o_ts;
-        if ((rc = device_pages(c, s.stream, size_t((s.kv + kPageTokens - 1) / kPageTokens), &e.pages)) != XN_OK) return rc;
+        if ((rc = device_pages(c, s.stream, &e.pages)) != XN_OK) return rc;
         e.rows = s.rows; e.kv_len = s.kv; e.layer = s.layer;
         const int tile = mt ? kPageTokens : c->tile_tokens;
         e.n_tiles = (s.kv + tile - 1) / tile;
@@ -1078,7 +1079,7 @@ int32_t evict_locked(xn_ctx* c, int32_t n, const xn_evict_req* reqs) {
             e.v_out = r.v_out;
         }
         if (!o.copy && !o.move && !e.kept && !e.w_out) continue;   // nothing to do, nothing to report
-        if ((rc = device_pages(c, r.stream, size_t((o.len + kPageTokens - 1) / kPageTokens), &e.pages)) != XN_OK) return rc;
+        if ((rc = device_pages(c, r.stream, &e.pages)) != XN_OK) return rc;
         for (int l = o.l0; l < o.l0 + o.nl;) {
             int m = l + 1;
             while (m < o.l0 + o.nl && r.stream->acc_len[size_t(m)] == r.stream->acc_len[size_t(l)]) ++m;
