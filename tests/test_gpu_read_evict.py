@@ -197,6 +197,25 @@ def test_one_stream_with_a_short_and_a_long_prefix_in_one_call(monkeypatch, path
         ctx.close()
 
 
+@pytest.mark.parametrize("path", ["few", "mid", "tc", "auto"])
+@pytest.mark.parametrize("ctas", [1, 8, 32, 64])
+def test_reads_with_fewer_split_kv_blocks_than_sms(monkeypatch, path, ctas):
+    """Long units cut over all SMs by the read of some rows, whatever the split-KV launches are bounded to."""
+    monkeypatch.setenv("XORNET_ATTN_DECODE_CTAS", str(ctas))
+    rng = np.random.default_rng(ctas)
+    ctx = context(monkeypatch, path, 1, 8, 2, 64, pool_pages=300, shuffle_seed=4)
+    made = [filled(ctx, rng, n) for n in (9001, 3000, 5500)]
+    for R in (1, 3, 12):
+        qs = [rows(rng, 8, R, 64) for _ in made]
+        for _ in range(2):   # (the counters are left as they were found)
+            outs, ws = ctx.cross_attention([st for st, _, _ in made], 0, qs, causal=R > 1, weights=True)
+        for (st, k, v), q, out, w in zip(made, qs, outs, ws):
+            want, want_w = plain(q, k, v, causal=R > 1)
+            near(out, want, f"R={R}")
+            near(w, want_w, f"weights R={R}", abs_tol=ABS * R)
+    ctx.close()
+
+
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
 def test_account_adds_up_is_set_and_follows_writes(monkeypatch, path):
     rng = np.random.default_rng(8)

@@ -48,3 +48,17 @@ def test_contexts_that_are_not_live_are_refused():
         assert lib.xn_kv_account_set(ctx, None, 0, 0, 1, None, 0) == 3
         assert lib.xn_kv_evict(ctx, 1, C.byref(evict)) == 3
         assert lib.xn_stream_evicted(ctx, None, 0) == -1
+
+
+def test_arrival_counters_cover_every_launch(tmp_path, repo_root):
+    """A launch of b blocks over c chunks counts arrivals in words 2 .. 1 + max(b, c) of the context's array,
+    also where the split-KV launches are cut into fewer chunks than there are SMs."""
+    src = tmp_path / "counters.cpp"
+    src.write_text('#include <cstdio>\n#include "xn_plan.hpp"\nint main() {\n'
+                   "    for (int c : {1, 8, 32, 64, 147, 148, 149, 296, 1000})\n"
+                   "        for (int b : {1, 132, 148}) printf(\"%d %d %zu\\n\", c, b, xn::sync_words(c, b));\n}\n")
+    exe = tmp_path / "counters"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(repo_root, "xor-net_b200", "csrc"), "-o", exe, src], check=True)
+    for line in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.splitlines():
+        chunks, blocks, words = map(int, line.split())
+        assert words >= 2 + max(chunks, blocks)

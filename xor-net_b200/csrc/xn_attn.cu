@@ -1941,7 +1941,7 @@ int32_t xn_ctx_create(const xn_ctx_desc* d, xn_ctx** out_ctx) {
         XN_CREATE_CUDA(cudaMemcpyAsync(c->cos_d, d->rope_cos, tb, cudaMemcpyHostToDevice, c->stream));
         XN_CREATE_CUDA(cudaMemcpyAsync(c->sin_d, d->rope_sin, tb, cudaMemcpyHostToDevice, c->stream));
     }
-    c->sync_cap = size_t(c->decode_chunks) + 8;  // a unit is cut at most once per chunk boundary
+    c->sync_cap = sync_words(c->decode_chunks, c->sm_count);
     XN_CREATE_CUDA(guarded_malloc(c, reinterpret_cast<void**>(&c->sync_d), c->sync_cap * sizeof(int), "arrival counters"));
     XN_CREATE_CUDA(cudaMemsetAsync(c->sync_d, 0, c->sync_cap * sizeof(int), c->stream));
     XN_CREATE_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&c->status_h), sizeof(int), cudaHostAllocMapped));

@@ -1,10 +1,18 @@
 // Host-side planning for the split-KV attention launch.  Pure C++ (no CUDA): unit-tested on
 // machines without a GPU through xn_plan_split.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include <vector>
 
 namespace xn {
+
+// Words of a context's synchronisation array: a few of the launch's own, then one arrival counter per
+// unit that a launch can cut.  A unit is cut at most once per boundary between chunks (split-KV
+// kernels) or between blocks (the read of some rows, whose launch has up to one block per SM
+// however few chunks the other launches are cut into).
+constexpr int kSyncHeaderWords = 2;
+inline size_t sync_words(int chunks, int blocks) { return size_t(kSyncHeaderWords) + size_t(std::max(chunks, blocks)) + 6; }
 
 struct SplitItem {
     int32_t unit, tile_begin, tile_end, part;

@@ -399,6 +399,9 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
         }
     }
     t.n_blocks = int(std::min<long long>(t.n_tiles, mt ? c->sm_count : c->decode_ctas));
+    static_assert(kSyncHeaderWords == kSyncMerge0, "layout of the synchronisation array");
+    if (size_t(t.n_blocks) + kSyncMerge0 > c->sync_cap)
+        return fail(c, XN_ERR_CAPACITY, "internal: %d blocks exceed the arrival counters", t.n_blocks);
     const size_t part = mt ? rm::part_floats(mt, c->nv * 4) : c->gt * part_stride_floats(c->nv);
     if ((rc = grow_device(c, &c->partials, &c->partials_cap, size_t(2 * t.n_blocks) * part)) != XN_OK) return rc;
     if (c->profile && (rc = profile_begin(c, 0)) != XN_OK) return rc;
