@@ -376,7 +376,8 @@ typedef struct xn_read_req {
 XN_API int32_t xn_cross_attention(xn_ctx* ctx, int32_t n, const xn_read_req* reqs);
 
 /* The account of positions [t0, t0+n), [num_kv_heads, n]: read it, or replace it (positions before t0
- * that had none get zeros; those from t0+n on are forgotten).  flags: XN_REQ_DEVICE_PTRS or 0. */
+ * that had none get zeros; those from t0+n on are forgotten).  A folded stream has none: zeros, and
+ * set is refused.  flags: XN_REQ_DEVICE_PTRS or 0. */
 XN_API int32_t xn_kv_account_get(xn_ctx* ctx, xn_stream* stream, int32_t layer, int64_t t0, int64_t n,
                                  float* out, uint32_t flags);
 XN_API int32_t xn_kv_account_set(xn_ctx* ctx, xn_stream* stream, int32_t layer, int64_t t0, int64_t n,

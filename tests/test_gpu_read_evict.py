@@ -671,6 +671,22 @@ def test_folded_streams_and_bad_arguments_are_refused():
     ctx.close()
 
 
+@pytest.mark.parametrize("pos,S", [(60, 4), (60, 10), (63, 2), (64, 1)])
+def test_an_append_that_folds_takes_the_whole_account_with_it(pos, S):
+    """Positions 64.. of a stream of 64 overwrite slots 0..; an append that just reaches the end does not."""
+    rng = np.random.default_rng(S)
+    ctx = xn.Context(1, 4, 2, 64, pool_pages=8)
+    st, k, v = filled(ctx, rng, 64, cap=64)
+    st.set_account(0, 0, np.full((2, 64), 3.0))
+    x, kv = rows(rng, 1, 4, S, 64), rows(rng, 1, 2, S, 64)
+    ctx.attention(st, 0, pos, x, kv, kv)
+    want = np.zeros((2, 64), np.float32)
+    if pos + S <= 64:
+        want[:, :pos] = 3
+    assert np.array_equal(st.account(0), want)
+    ctx.close()
+
+
 def test_pool_exhaustion_by_a_write_leaves_the_stream_as_it_was():
     rng = np.random.default_rng(0)
     ctx = xn.Context(1, 2, 1, 16, pool_pages=2)

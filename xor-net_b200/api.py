@@ -157,7 +157,7 @@ class Stream:
 
     def account(self, layer: int, t0: int = 0, n: Optional[int] = None) -> np.ndarray:
         """xn_kv_account_get: the accumulated attention weight ``[Hkv, n]`` of positions t0..t0+n."""
-        n = self.length(layer) - t0 if n is None else n
+        n = min(self.length(layer), self.max_seq_len) - t0 if n is None else n
         out = np.zeros((self.ctx.num_kv_heads, max(n, 0)), dtype=np.float32)
         self.ctx._check(self.ctx.lib.xn_kv_account_get(self.ctx.handle, self.handle, layer, t0, n, _ptr(out), 0))
         return out

@@ -582,11 +582,12 @@ void free_call_buffer(xn_stream* s) {
     s->call_cap = 0;
 }
 
-// Rows are about to be written from position t on: the account of attention weight of those
-// positions belonged to the rows they replace.
-void forget_account(xn_stream* s, int layer, int64_t t) {
+// Rows are about to be written at positions [t, end): the account of attention weight from t on
+// belonged to the rows they replace.  Positions that fold overwrite slots from the start, and a folded
+// stream keeps no account at all.
+void forget_account(xn_stream* s, int layer, int64_t t, int64_t end) {
     int64_t& n = s->acc_len[size_t(layer)];
-    n = t >= s->cap ? 0 : std::min(n, t);   // (folded positions overwrite slots from the start)
+    n = end > s->cap ? 0 : std::min(n, t);
 }
 
 void release_pages(xn_ctx* c, xn_stream* s) {
@@ -918,7 +919,7 @@ bool submit_reusing_plan(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, i
         for (int i = 0; i < n; ++i) {
             int64_t& hw = reqs[i].stream->hw[size_t(layer)];
             hw = std::max(hw, reqs[i].index_pos + 1);
-            forget_account(reqs[i].stream, layer, reqs[i].index_pos);
+            forget_account(reqs[i].stream, layer, reqs[i].index_pos, reqs[i].index_pos + 1);
         }
         XN_CUDA(c, cudaEventRecord(pc.slot->ev, c->stream));
         pc.slot->used = true;
@@ -1341,7 +1342,8 @@ int32_t submit_locked(xn_ctx* c, int n, const xn_req* reqs, bool host_mode, cuda
     // -- launches: every sizing step above has succeeded, the cache positions are going to be written
     undo.commit();
     for (int i = 0; i < n; ++i)
-        if (reqs[i].seq_len > 0) forget_account(reqs[i].stream, reqs[i].layer, reqs[i].index_pos);
+        if (reqs[i].seq_len > 0)
+            forget_account(reqs[i].stream, reqs[i].layer, reqs[i].index_pos, reqs[i].index_pos + reqs[i].seq_len);
     for (const OutRun& run : qkv_runs) {   // x -> [q | k | v] rows, before anything reads them
         const OutRowDev* rows_d = reinterpret_cast<const OutRowDev*>(slot->dev + o_qkv) + run.row_begin;
         if (c->profile && (rc = profile_begin(c, 3)) != XN_OK) return rc;
@@ -2526,7 +2528,7 @@ int32_t xn_kv_fill_normal(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, in
                                                          n, 1, seed + 0x632BE59BD9B4E019ull * uint64_t(l));
         c->stats.kernel_launches += 1;
         s->hw[size_t(l)] = std::max<int64_t>(s->hw[size_t(l)], t0 + n);
-        forget_account(s, l, t0);
+        forget_account(s, l, t0, t0 + n);
     }
     XN_CUDA(c, cudaGetLastError());
     XN_CUDA(c, cudaEventRecord(slot->ev, c->stream));

@@ -169,7 +169,7 @@ int32_t kv_write_locked(xn_ctx* c, xn_stream* s, int32_t layer, int64_t t0, int6
         c->stats.kernel_launches += 1;
     }
     hw = std::max(hw, t0 + n);
-    forget_account(s, layer, t0);
+    forget_account(s, layer, t0, t0 + n);
     const long long rows = n * 2 * Hkv;
     const ReqDev* req_d = reinterpret_cast<const ReqDev*>(slot->dev + o_req);
     if (c->kv_u8) {
