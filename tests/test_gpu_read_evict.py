@@ -334,6 +334,58 @@ def test_values_over_many_orders_of_magnitude(monkeypatch, path):
     ctx.close()
 
 
+def spread_rows(rng, what, e):
+    """256 positions and 190 causal query rows (the first sees 67), with values 2^e times the others' in a
+    whole page of V or in one row of V or of K.  "behind": in positions that most query rows do not see;
+    "unweighted": seen by all of them, with a score that leaves them no weight (exp(-200) and less).
+    "faint": a page of zeros beside pages of 2^-e."""
+    Hq, Hkv, D, n, R = 4, 2, 64, 256, 190
+    k, v, q = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D), np.abs(rows(rng, Hq, R, D)) + np.float32(0.1)
+    big = np.float32(2.0 ** e)
+    if what == "faint":
+        v /= big
+        v[:, 64:128] = 0
+        v[:, 130] = 0
+        return k, v, q
+    kind, how = what.split("_")
+    at = {("page", "behind"): slice(192, 256), ("page", "unweighted"): slice(64, 128),
+          ("row", "behind"): slice(200, 201), ("row", "unweighted"): slice(40, 41),
+          ("krow", "behind"): slice(200, 201), ("krow", "unweighted"): slice(40, 41)}[kind, how]
+    if kind == "krow":
+        k[:, at] = -np.abs(k[:, at]) * big if how == "unweighted" else k[:, at] * big
+    else:
+        v[:, at] *= big
+        if how == "unweighted":
+            k[:, at] = -40 - np.abs(k[:, at])   # score below -(0.1 + 0) * 40 * 64 / 8 = -32, about -260
+    return k, v, q
+
+
+def check_spread(monkeypatch, path, what, e):
+    """Row by row, each against its own norm: what a query row gives no weight to must not coarsen the rest
+    of its output.  Rows that share a page and lie within 2^16 of one another have an element error of
+    2^-23 of their own largest element from the scale they share, beside the 2^-23 of the split; that
+    and the neighbours' factors (up to 2^10: 2^-29 of the weights) stay well inside the tolerance above."""
+    rng = np.random.default_rng(1000 + e)
+    ctx = context(monkeypatch, path, 1, 4, 2, 64, pool_pages=8, shuffle_seed=3)
+    k, v, q = spread_rows(rng, what, e)
+    st = ctx.new_stream(256)
+    st.write(0, 0, k, v)
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+    want, want_w = plain(q, k, v, True)
+    for h in range(4):
+        for t in range(190):
+            near(out[h, t], want[h, t], f"{what} 2^{e} row {h} {t}", abs_tol=np.inf)
+    near(w, want_w, f"{what} 2^{e} weights", abs_tol=ABS * 190)
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
+@pytest.mark.parametrize("e", [9, 11, 20, 30, 40])
+@pytest.mark.parametrize("what", ["page_behind", "page_unweighted", "faint"])
+def test_neighbouring_pages_of_very_different_sizes(monkeypatch, path, what, e):
+    check_spread(monkeypatch, path, what, e)
+
+
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("n,R", [(3, 4), (200, 9), (2000, 40)])
 def test_scores_of_minus_infinity_throughout_are_no_numbers(monkeypatch, path, n, R):

@@ -63,8 +63,9 @@ struct TcKeyTile {
     int req, head, tile, qt_begin;
 };
 
-// What the softmax needs to know about a page's K [0] and V [1]: factors that undo the scaling, and
-// the rows that hold an infinity or a NaN (their images are zero; they are added exactly on the side).
+// What the softmax needs to know about a page's K [0] and V [1]: factors that undo the scaling (of a V
+// image that is all zeros: kZeroFactor), and the rows that hold an infinity or a NaN (their images are
+// zero; they are added exactly on the side).
 struct __align__(16) PageMeta {
     float f[2];
     unsigned any_bad[2];
@@ -87,6 +88,8 @@ constexpr int kPage = 64;
 constexpr int kSub = kPage * 128;        // one column block (64 halves) of one page
 constexpr int kRowsSub = kBM * 128;      // one column block of 128 rows
 constexpr float kPScale = 16384.0f;      // 2^14: P is split at this scale
+constexpr float kApart = 0x1p-10f;       // pages whose V factors are further apart than this do not share a sum
+constexpr float kZeroFactor = 0x1p-100f; // (factors of other pages are 2^-73 and more: scale_of)
 constexpr int kThreads = 320;            // copy warp, MMA warp, two softmax warpgroups
 constexpr int kVStages = 3;
 constexpr int kQBytes = 4 * kRowsSub;    // 64 KB: hi and lo, two column blocks
@@ -309,12 +312,15 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
             s_bad[warp] = (unsigned char)bad;
         }
         __syncthreads();
+        const float page_max = fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4)));
+        const bool empty = page_max == 0.f;
         float up, down;
-        scale_of(fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4))), up, down);
+        scale_of(page_max, up, down);
         if (threadIdx.x == 0) {
             const unsigned long long rows = *reinterpret_cast<const unsigned long long*>(s_bad);
             PageMeta& pm = meta[id];
-            pm.f[part] = down;
+            // (a V page of zeros takes no part in the choice of its neighbour's scale; K's factor undoes scores)
+            pm.f[part] = part && empty ? kZeroFactor : down;
             pm.any_bad[part] = rows != 0 ? 1u : 0u;
             pm.bad[part] = rows;
         }
@@ -622,10 +628,15 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             // both pages' factors (uniform over the block)
             const PageMeta* pm0 = pm + size_t(2 * j) * c.num_kv_heads;
             const PageMeta* pm1 = two ? pm0 + c.num_kv_heads : pm0;
-            const float fv0 = pm0->f[1], fv1 = pm1->f[1];
-            const float cm = cq * (wg ? pm1 : pm0)->f[0];
-            const bool bad_k = pm0->any_bad[0] | pm1->any_bad[0], bad_v = pm0->any_bad[1] | pm1->any_bad[1];
-            const float fv = fmaxf(fv0, fv1);
+            const uint4 a0 = *reinterpret_cast<const uint4*>(pm0), a1 = *reinterpret_cast<const uint4*>(pm1);   // f[2], any_bad[2]
+            const float fv0 = __uint_as_float(a0.y), fv1 = __uint_as_float(a1.y);
+            const float cm = cq * __uint_as_float(wg ? a1.x : a0.x);
+            // The products of both pages' V images go to one accumulator, so P of the page with the smaller
+            // factor is scaled down by their ratio.  Up to 2^10 that leaves weights a resolution of 2^-29 of
+            // the largest; a page further below keeps its P and is added on the side, row by row in f32.
+            const float fv = fmaxf(fv0, fv1), fv_low = fminf(fv0, fv1);
+            const bool bad_k = a0.z | a1.z;
+            const bool bad_v = (a0.w | a1.w) != 0u || (fv_low < fv * kApart && fv_low != kZeroFactor);
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
             if (lane == 0 && dead) { sm_dead[sb] = 1; *abort_flag = 1; }
             fence_after_sync();
@@ -678,7 +689,8 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             m_ref = m_new;
             l_sum *= alpha;
             if (have) {
-                const float pscale = kPScale * ((wg ? fv1 : fv0) / fv);   // powers of two: exact
+                float pscale = (wg ? fv1 : fv0) / fv;   // powers of two: exact
+                pscale = pscale < kApart ? kPScale : kPScale * pscale;
                 float2 ps = make_float2(0.f, 0.f);
                 const float2 cm2 = make_float2(cm, cm), nm2 = make_float2(neg_m, neg_m), sc2 = make_float2(pscale, pscale);
                 uint32_t hi[32], lo[32];
@@ -707,8 +719,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 tmem_wait_st();
             }
             if (bad_v) {
-                // rows of V with an infinity or a NaN (uniform over the block): bring O up to date, then
-                // add p * v for the rows that see them; P of both pages is read back from tensor memory
+                // rows of V with an infinity or a NaN, or all of a page that is set apart (uniform over the
+                // block): bring O up to date, then add p * v for the rows that see them; P of both pages is
+                // read back from tensor memory
                 if (j > 0) {
                     if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
                 }
@@ -718,8 +731,14 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 wg_barrier();
                 fence_after_sync();
                 for (int p = 0; p < 2; ++p) {
+                    const float fp = p ? fv1 : fv0;
+                    const bool apart = fp < fv * kApart, side = apart && fp != kZeroFactor;
                     unsigned long long b = p == 0 ? pm0->bad[1] : (two ? pm1->bad[1] : 0ull);
-                    const float unscale = fv / (kPScale * (p ? fv1 : fv0));
+                    if (side) {
+                        const int ntok = r.kv_len - (it.page_begin + 2 * j + p) * kPage;
+                        b = ntok >= kPage ? ~0ull : (1ull << ntok) - 1;
+                    }
+                    const float unscale = apart ? 1.0f / kPScale : fv / (kPScale * fp);
                     while (b) {
                         const int cidx = __ffsll((long long)b) - 1;
                         b &= b - 1;
@@ -746,6 +765,11 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 }
                 fence_before_sync();
                 wg_barrier();
+                if ((wg ? fv1 : fv0) < fv * kApart) {   // nothing of that page is left for the MMAs
+                    fence_after_sync();
+#pragma unroll 1
+                    for (int i = 0; i < 64; ++i) tmem_st1(s_addr + i, 0u);
+                }
             } else if (j > 0) {
                 warp_arrive(&p_full[sb], lane);
                 if (!add_tile(j - 1, alpha_prev, f_prev)) { report_status(status, kDevWaitMma); *abort_flag = 1; }
