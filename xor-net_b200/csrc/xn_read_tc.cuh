@@ -7,12 +7,15 @@
 // Arithmetic.  Every f32 operand x is scaled by a power of two (per query row, per 64-token page of
 // K and of V, so that the largest magnitude lies in [2^13, 2^14)) and split into two f16 values,
 // x = hi + lo with hi = f16(x) and lo = f16(x - hi): 22 significand bits, and an absolute floor of
-// 2^-39 of the page's (or row's) largest value for elements far below it.  A product takes three
-// MMAs, lo*hi + hi*lo + hi*hi, with f32 accumulators; the lo*lo term (2^-22 relative) is left out.
-// kind::f16 runs at twice the rate of kind::tf32, whose hi/lo split has as many bits, and its
-// operands are half as large.  P is split the same way (scaled by 2^14).  Sums over more than 128
-// positions are not left to the tensor cores' accumulator: every 128-position tile of O starts from
-// zero there and is added up in f32 registers; so are the softmax sums.
+// 2^-39 of the page's (or row's) largest value for elements far below it.  A page's rows that are far
+// larger or smaller than its median row are kept out of its scale and multiplied in f32, so that the
+// floor is never above 2^-23 of a row's own largest element.  A product takes three MMAs, lo*hi +
+// hi*lo + hi*hi, with f32 accumulators; the lo*lo term (2^-22 relative) is left out.  kind::f16 runs
+// at twice the rate of kind::tf32, whose hi/lo split has as many bits, and its operands are half as
+// large.  P is split the same way, scaled by 2^14: a weight has a floor of 2^-39 of its query row's
+// largest.  Sums over more than 128 positions are not left to the tensor cores' accumulator: every
+// 128-position tile of O starts from zero there and is added up in f32 registers; so are the softmax
+// sums.
 //
 // Passes: (1) page_images_kernel writes K, V and Q once as hi/lo images in the shared-memory layout
 // (128-byte swizzle) that the MMAs read, so that no later block converts anything; (2)
@@ -64,8 +67,8 @@ struct TcKeyTile {
 };
 
 // What the softmax needs to know about a page's K [0] and V [1]: factors that undo the scaling (of a V
-// image that is all zeros: kZeroFactor), and the rows that hold an infinity or a NaN (their images are
-// zero; they are added exactly on the side).
+// image that is all zeros: kZeroFactor), and the rows that hold an infinity or a NaN or are far larger or
+// smaller than the page's others (their images are zero; they are added on the side, in f32).
 struct __align__(16) PageMeta {
     float f[2];
     unsigned any_bad[2];
@@ -88,6 +91,7 @@ constexpr int kPage = 64;
 constexpr int kSub = kPage * 128;        // one column block (64 halves) of one page
 constexpr int kRowsSub = kBM * 128;      // one column block of 128 rows
 constexpr float kPScale = 16384.0f;      // 2^14: P is split at this scale
+constexpr float kRowSpread = 0x1p-16f;   // rows of a page that share a scale lie within this of one another
 constexpr float kApart = 0x1p-10f;       // pages whose V factors are further apart than this do not share a sum
 constexpr float kZeroFactor = 0x1p-100f; // (factors of other pages are 2^-73 and more: scale_of)
 constexpr int kThreads = 320;            // copy warp, MMA warp, two softmax warpgroups
@@ -264,7 +268,9 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
     using namespace rt;
     pdl_launch_dependents();
     __shared__ __align__(16) float s_max[8];
+    __shared__ unsigned s_least[8];
     __shared__ __align__(8) unsigned char s_bad[8];
+    __shared__ float s_row[kPage], s_median;
     constexpr unsigned kFull = 0xffffffffu;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = c.head_dim, nb = blocks_of(D);
@@ -292,11 +298,19 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
             const int tk = warp * 8 + i;
             x[i] = tk < ntok ? cache_row4(c, blk, tk, lane, part != 0) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        // the largest magnitude, and the smallest of any lane's four columns that are not all zeros (as bits
+        // minus one, so that zeros count as the largest)
+        unsigned least = ~0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max_nan(max_nan(max_nan(max_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        for (int i = 0; i < 8; ++i) {
+            const float q = max_nan(max_nan(max_nan(fabsf(x[i].x), x[i].y), x[i].z), x[i].w);
+            m = max_nan(m, q);
+            least = min(least, __float_as_uint(q) - 1u);
+        }
         unsigned bits = __reduce_max_sync(kFull, __float_as_uint(m)), bad = 0;   // as bits: finite < infinity < NaN
         if (bits >= 0x7f800000u) {
             m = 0.f;
+            least = ~0u;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (!__all_sync(kFull, finite4(x[i]))) {
@@ -304,15 +318,56 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
                     x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
                 m = fmaxf(m, max4(x[i]));
+                least = min(least, __float_as_uint(max4(x[i])) - 1u);
             }
             bits = __reduce_max_sync(kFull, __float_as_uint(m));
         }
+        least = __reduce_min_sync(kFull, least);
         if (lane == 0) {
             s_max[warp] = __uint_as_float(bits);
+            s_least[warp] = least;
             s_bad[warp] = (unsigned char)bad;
         }
         __syncthreads();
-        const float page_max = fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4)));
+        float page_max = fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) least = min(least, s_least[i]);
+        if (least != ~0u && __uint_as_float(least + 1u) < page_max * kRowSpread) {
+            // Rows that share a scale have an absolute floor of 2^-39 of its largest element, which is a
+            // matter of f32 only while their own largest ones lie within 2^16 of one another.  Rows further
+            // than 2^8 from the median row's (zeros aside) leave the image and are added on the side, like
+            // rows with an infinity.  (Seldom: the whole block comes here or nobody does.)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned row = __reduce_max_sync(kFull, __float_as_uint(max4(x[i])));
+                if (lane == 0) s_row[warp * 8 + i] = __uint_as_float(row);
+            }
+            __syncthreads();
+            if (threadIdx.x < kPage) {
+                const float mine = s_row[threadIdx.x];
+                int before = 0, all = 0;
+                for (int i = 0; i < kPage; ++i) {
+                    const float v = s_row[i];
+                    all += v > 0.f;
+                    before += v > 0.f && (v < mine || (v == mine && i < int(threadIdx.x)));
+                }
+                if (mine > 0.f && before == all / 2) s_median = mine;
+            }
+            __syncthreads();
+            const float lo = s_median * 0x1p-8f, hi = s_median * 0x1p8f;
+            page_max = 0.f;
+            for (int i = 0; i < kPage; ++i)
+                if (s_row[i] >= lo && s_row[i] <= hi) page_max = fmaxf(page_max, s_row[i]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float row = s_row[warp * 8 + i];
+                if (row == 0.f || (row >= lo && row <= hi)) continue;
+                bad |= 1u << i;
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            if (lane == 0) s_bad[warp] = (unsigned char)bad;
+            __syncthreads();
+        }
         const bool empty = page_max == 0.f;
         float up, down;
         scale_of(page_max, up, down);
@@ -634,7 +689,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             // The products of both pages' V images go to one accumulator, so P of the page with the smaller
             // factor is scaled down by their ratio.  Up to 2^10 that leaves weights a resolution of 2^-29 of
             // the largest; a page further below keeps its P and is added on the side, row by row in f32.
+            // (Below at all, where rows are added on the side anyway: they may be large, and need the P.)
             const float fv = fmaxf(fv0, fv1), fv_low = fminf(fv0, fv1);
+            const float apart_below = (a0.w | a1.w) != 0u ? 1.f : kApart;
             const bool bad_k = a0.z | a1.z;
             const bool bad_v = (a0.w | a1.w) != 0u || (fv_low < fv * kApart && fv_low != kZeroFactor);
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
@@ -646,7 +703,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             float mx = -INFINITY;
             if (!dead && have) {
                 if (bad_k) {
-                    // rows of K with an infinity or a NaN: their scores one by one, in f32, put where the
+                    // rows of K that are not in the image: their scores one by one, in f32, put where the
                     // MMA left zeros
                     unsigned long long b = (wg ? pm1 : pm0)->bad[0];
                     while (b) {
@@ -690,7 +747,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             l_sum *= alpha;
             if (have) {
                 float pscale = (wg ? fv1 : fv0) / fv;   // powers of two: exact
-                pscale = pscale < kApart ? kPScale : kPScale * pscale;
+                pscale = pscale < apart_below ? kPScale : kPScale * pscale;
                 float2 ps = make_float2(0.f, 0.f);
                 const float2 cm2 = make_float2(cm, cm), nm2 = make_float2(neg_m, neg_m), sc2 = make_float2(pscale, pscale);
                 uint32_t hi[32], lo[32];
@@ -719,7 +776,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 tmem_wait_st();
             }
             if (bad_v) {
-                // rows of V with an infinity or a NaN, or all of a page that is set apart (uniform over the
+                // rows of V that are not in the image, or all of a page that is set apart (uniform over the
                 // block): bring O up to date, then add p * v for the rows that see them; P of both pages is
                 // read back from tensor memory
                 if (j > 0) {
@@ -732,7 +789,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 fence_after_sync();
                 for (int p = 0; p < 2; ++p) {
                     const float fp = p ? fv1 : fv0;
-                    const bool apart = fp < fv * kApart, side = apart && fp != kZeroFactor;
+                    const bool apart = fp < fv * apart_below, side = apart && fp != kZeroFactor;
                     unsigned long long b = p == 0 ? pm0->bad[1] : (two ? pm1->bad[1] : 0ull);
                     if (side) {
                         const int ntok = r.kv_len - (it.page_begin + 2 * j + p) * kPage;
@@ -765,7 +822,7 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                 }
                 fence_before_sync();
                 wg_barrier();
-                if ((wg ? fv1 : fv0) < fv * kApart) {   // nothing of that page is left for the MMAs
+                if ((wg ? fv1 : fv0) < fv * apart_below) {   // nothing of that page is left for the MMAs
                     fence_after_sync();
 #pragma unroll 1
                     for (int i = 0; i < 64; ++i) tmem_st1(s_addr + i, 0u);
