@@ -393,14 +393,14 @@ def test_neighbouring_pages_of_very_different_sizes(monkeypatch, path, what, e):
     check_spread(monkeypatch, path, what, e)
 
 
-@pytest.mark.parametrize("path", ["few", "tc"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("e", [7, 9, 15, 17, 20, 30, 40])
 @pytest.mark.parametrize("what", ["row_behind", "row_unweighted", "rows_unweighted", "krow_behind", "krow_unweighted", "krows_unweighted"])
 def test_rows_of_one_page_of_very_different_sizes(monkeypatch, path, what, e):
     check_spread(monkeypatch, path, what, e)
 
 
-@pytest.mark.parametrize("path", ["few", "tc"])
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("e", [10, 20, 30])
 def test_a_large_row_of_little_weight(monkeypatch, path, e):
     """A position that gets about e^-20 of the weight, with values of 2^e, in a page that is 2^-5 of its

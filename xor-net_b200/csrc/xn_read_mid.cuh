@@ -61,11 +61,8 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float warp_max(float m) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
-}
+// (magnitudes: their bits order as they do)
+__device__ __forceinline__ float warp_max(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
 __device__ __forceinline__ float finite_max4(const float4& x) {   // infinities and NaNs do not set a scale
     float m = 0.f;
     m = fabsf(x.x) < INFINITY ? fmaxf(m, fabsf(x.x)) : m;
@@ -259,7 +256,8 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) sc[mt][0] = sc[mt][1] = sc[mt][2] = sc[mt][3] = 0.f;
             float fk;
-            unsigned bad_k;               // lanes that hold an infinity or a NaN of K: four bits per position
+            unsigned bad_k;               // lanes whose part of K the MMAs do not take (an infinity, a NaN, values far
+                                          // below their neighbours'): four bits per position
             {
                 const int key = w * 8 + g;
                 float4 kx[8];
@@ -280,8 +278,20 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) mx = fmaxf(mx, finite_max4(kx[ks]));
                 }
+                const float largest = warp_max(mx);
+                if (__any_sync(kFull, mx > 0.f && mx < largest * rt::kRowSpread)) {
+                    // positions far below the largest of the eight would lose bits to its scale: their scores
+                    // in f32 as well (seldom)
+                    float row = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+                    row = fmaxf(row, __shfl_xor_sync(kFull, row, 2));
+                    const bool small = row > 0.f && row < largest * rt::kRowSpread;
+                    bad_k |= __ballot_sync(kFull, small);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        if (small) kx[ks] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
                 float up;
-                rt::scale_of(warp_max(mx), up, fk);
+                rt::scale_of(largest, up, fk);
                 const float2 up2 = make_float2(up, up);
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
@@ -316,7 +326,7 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                 for (int hf = 0; hf < 2; ++hf) {
                     const float cm = cq[mt][hf] * fk;
                     float a = sc[mt][2 * hf] * cm, b = sc[mt][2 * hf + 1] * cm;
-                    if (bad_k) {   // a split product of an infinity is not one: those positions' scores in f32
+                    if (bad_k) {   // those positions' scores in f32 (a split product of an infinity is not one)
                         const int p = row0 + mt * 16 + hf * 8 + g;
 #pragma unroll 1
                         for (int u = 0; u < 2; ++u) {
@@ -381,6 +391,7 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
             if (my_cols) {
                 float4 vx[2][4];
                 float mx = 0.f;
+                unsigned least = ~0u;   // the smallest magnitude of any lane's four columns that are not all zeros, as bits minus one
                 bool ok = true;
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
@@ -389,12 +400,15 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                         const int key = kh * 32 + st * 16 + 2 * t4 + (r & 1) + 8 * (r >> 1);
                         vx[st][r] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (key < ntok) vx[st][r] = *reinterpret_cast<const float4*>(vs_s + cbw * kSub + key * 128 + ((g ^ (key & 7)) << 4));
-                        mx = fmaxf(mx, rt::max4(vx[st][r]));
+                        const float q = rt::max4(vx[st][r]);
+                        mx = fmaxf(mx, q);
+                        least = __viaddmin_u32(__float_as_uint(q), ~0u, least);
                         ok = ok && rt::finite4(vx[st][r]);
                     }
                 ok = __all_sync(kFull, ok);
                 if (!ok) {   // infinities and NaNs: left out here, added below for the rows that see them
                     mx = 0.f;
+                    least = ~0u;
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -404,11 +418,30 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                             x.y = fabsf(x.y) < INFINITY ? x.y : 0.f;
                             x.z = fabsf(x.z) < INFINITY ? x.z : 0.f;
                             x.w = fabsf(x.w) < INFINITY ? x.w : 0.f;
-                            mx = fmaxf(mx, rt::max4(x));
+                            const float q = rt::max4(x);
+                            mx = fmaxf(mx, q);
+                            least = __viaddmin_u32(__float_as_uint(q), ~0u, least);
                         }
                 }
+                const float largest = warp_max(mx);
+                unsigned small = 0u;   // of the 32 positions, those whose 32 columns are far below the largest: added below too
+                if (__any_sync(kFull, least < __float_as_uint(largest * rt::kRowSpread))) {
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float q = rt::max4(vx[st][r]);
+                            q = fmaxf(q, __shfl_xor_sync(kFull, q, 4));
+                            q = fmaxf(q, __shfl_xor_sync(kFull, q, 8));
+                            q = fmaxf(q, __shfl_xor_sync(kFull, q, 16));
+                            if (!(q > 0.f && q < largest * rt::kRowSpread)) continue;
+                            small |= 1u << (st * 16 + 2 * t4 + (r & 1) + 8 * (r >> 1));
+                            vx[st][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                    small = __reduce_or_sync(kFull, small);
+                }
                 float up, fv;
-                rt::scale_of(warp_max(mx), up, fv);
+                rt::scale_of(largest, up, fv);
                 const float f = fv * (1.0f / kPScale);
                 const float2 up2 = make_float2(up, up);
                 // columns i of the lane's four go to the MMA's column tile i
@@ -459,7 +492,7 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
                                         fmaf(c[2][2 * hf + 1], f, y.z * al_), fmaf(c[3][2 * hf + 1], f, y.w * al_));
                     }
                 }
-                if (!ok) {
+                if (!ok || small != 0u) {
 #pragma unroll 1
                     for (int k = 0; k < 32; ++k) {
                         const int key = kh * 32 + k;
@@ -469,7 +502,7 @@ read_mid_kernel(const __grid_constant__ ReadTable tab, const __grid_constant__ C
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {   // the lane's columns 8 t .. 8 t + 7
                             v[i] = *reinterpret_cast<const float*>(vs_s + cbw * kSub + key * 128 + (((2 * t4 + (i >> 2)) ^ (key & 7)) << 4) + (i & 3) * 4);
-                            if (fabsf(v[i]) < INFINITY) v[i] = 0.f;
+                            if (fabsf(v[i]) < INFINITY && !(small >> k & 1u)) v[i] = 0.f;
                             else any = true;
                         }
                         if (!any) continue;
