@@ -905,6 +905,32 @@ def test_many_requests_of_all_sizes_in_one_call(account):
     ctx.close()
 
 
+def test_more_rows_with_weights_than_one_launch_takes(monkeypatch):
+    """140 000 small causal reads (4.5 million units of work) in one call; and one of 70 000 rows."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    ctx = context(monkeypatch, "few", 1, 16, 16, 4, pool_pages=2)
+    st, k, v = filled(ctx, rng, 2)
+    qh = rows(rng, 16, 2, 4)
+    want, want_w = plain(qh, k, v, causal=True)
+    q = torch.from_numpy(qh).cuda()
+    out, w = torch.zeros_like(q), torch.zeros(16, 2, device="cuda")
+    torch.cuda.synchronize()
+    one = (st, 0, 2, 2, q.data_ptr(), out.data_ptr(), w.data_ptr(), 0)
+    ctx.submit_reads(ctx.make_read_batch([one] * 140_000, xn.REQ_DEVICE_PTRS | xn.READ_CAUSAL))
+    ctx.synchronize()
+    near(out.cpu().numpy(), want)
+    near(w.cpu().numpy(), want_w)
+    q = np.zeros((16, 70_000, 4), np.float32)
+    q[:, -2:] = qh
+    (o,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+    assert not o[:, :-2].any()
+    near(o[:, -2:], want)
+    near(w, want_w)
+    ctx.close()
+
+
 def test_captured_attention_replays_after_reads_and_evictions():
     """A graph of another library's work on the caller's stream is not disturbed by calls made in between."""
     import torch

@@ -904,7 +904,7 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
             i = j;
         }
     }
-    // the other few rows: all at once without weights; with weights in portions whose scores fit, a request of
+    // the other few rows, in portions of a quarter of the units that a launch takes; with weights, whose scores fit, a request of
     // too many rows (long prompts of head_dim > 128) in several row blocks whose weights add up
     if (!few[0].empty()) {
         std::vector<ReadSub> part;
@@ -934,20 +934,25 @@ int32_t read_locked(xn_ctx* c, int32_t n, const xn_read_req* reqs) {
     }
     std::vector<ReadSub> part;
     size_t floats = 0;
+    long long units = 0;
+    const long long per_row = (long long)Hkv * c->subs, most_units = kMaxUnits / 4;
     auto flush = [&]() -> int32_t {
         if (part.empty()) return XN_OK;
         const int32_t e = launch_read_few(c, part, true);
         part.clear();
         floats = 0;
+        units = 0;
         return e;
     };
     for (const ReadSub& s : few[1]) {
         const size_t row = align_up(size_t(s.kv), 4) * Hq;
-        const int most = int(std::min<size_t>(size_t(1) << 20, std::max<size_t>(1, kReadScoreBudget / 4 / row)));
+        const int most = int(std::max<long long>(1, std::min<long long>((long long)(kReadScoreBudget / 4 / row), most_units / per_row)));
         if (s.rows <= most) {
-            if (floats + row * s.rows > kReadScoreBudget / 4 && (rc = flush()) != XN_OK) return rc;
+            if ((floats + row * s.rows > kReadScoreBudget / 4 || units + s.rows * per_row > most_units) && (rc = flush()) != XN_OK)
+                return rc;
             part.push_back(s);
             floats += row * s.rows;
+            units += s.rows * per_row;
             continue;
         }
         if ((rc = flush()) != XN_OK) return rc;
