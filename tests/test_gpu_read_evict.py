@@ -552,6 +552,66 @@ def test_evict_keeps_what_the_account_says(n, keep, recent):
     ctx.close()
 
 
+@pytest.mark.parametrize("n,keep,recent", [(262_200, 5, 0), (300_001, 1_000, 7), (270_000, 200_001, 63), (530_000, 3, 2)])
+def test_evict_of_more_positions_than_the_selection_keeps_on_chip(n, keep, recent):
+    """Above 262 144 candidates the selection reads its keys again in every pass."""
+    rng = np.random.default_rng(n)
+    Hkv, D = 2, 4
+    ctx = xn.Context(1, 2, Hkv, D, pool_pages=(n + 63) // 64, shuffle_seed=9)
+    st = ctx.new_stream(n)
+    k, v = rows(rng, Hkv, n, D), rows(rng, Hkv, n, D)
+    w = np.exp(2 * rows(rng, Hkv, n))
+    w[0] = np.round(w[0])
+    w[1, rng.random(n) < 0.01] = np.nan
+    st.write(0, 0, k, v)
+    st.set_account(0, 0, w)
+    want = np.stack([kept_of(w[h], keep, recent) for h in range(Hkv)])
+    kept, ck, cv, cw = st.evict_copy(keep, recent)
+    assert np.array_equal(kept[0], want)
+    assert np.array_equal(st.evict(keep, recent)[0], want)
+    gk, gv = st.read_range(0, 0, keep)
+    for h in range(Hkv):
+        assert np.array_equal(ck[0, h], k[h, want[h]]) and np.array_equal(cv[0, h], v[h, want[h]])
+        assert np.array_equal(cw[0, h], w[h, want[h]], equal_nan=True)
+        assert np.array_equal(gk[h], k[h, want[h]]) and np.array_equal(gv[h], v[h, want[h]])
+        assert np.array_equal(st.account(0)[h], w[h, want[h]], equal_nan=True)
+    ctx.close()
+
+
+@pytest.mark.parametrize("fmt", [xn.KV_F32, xn.KV_U8])
+def test_more_evictions_than_one_launch_takes_and_accounts_of_different_lengths(fmt):
+    """31 streams of three layers, whose accounts are complete, end in the middle, or are not there."""
+    rng = np.random.default_rng(31)
+    L, Hkv, D, keep, recent = 3, 2, 32, 40, 9
+    ctx = xn.Context(L, 4, Hkv, D, pool_pages=200, shuffle_seed=4, kv_format=fmt)
+    made = []
+    for i in range(31):
+        n = int(rng.integers(1, 300))
+        st = ctx.new_stream(n)
+        w = np.zeros((L, Hkv, n), np.float32)
+        for l in range(L):
+            st.write(l, 0, rows(rng, Hkv, n, D), rows(rng, Hkv, n, D))
+            ends = (n, n // 2, 0)[(l + i) % 3]
+            if ends:
+                w[l, :, :ends] = rows(rng, Hkv, ends)
+                st.set_account(l, 0, w[l, :, :ends])
+        made.append((st, n, w, [st.read_range(l, 0, n) for l in range(L)]))
+    kepts = [np.zeros((L, Hkv, min(keep, n)), np.int32) for _, n, _, _ in made]
+    ws = [np.zeros((L, Hkv, min(keep, n)), np.float32) for _, n, _, _ in made]
+    ctx.submit_evict(ctx.make_evict_batch([(m[0], -1, keep, recent, a.ctypes.data, None, None, b.ctypes.data)
+                                           for m, a, b in zip(made, kepts, ws)]))
+    for (st, n, w, kv), kept, got_w in zip(made, kepts, ws):
+        for l in range(L):
+            gk, gv = st.read_range(l, 0, min(keep, n))
+            for h in range(Hkv):
+                want = kept_of(w[l, h], keep, recent)
+                assert np.array_equal(kept[l, h], want), (n, l, h)
+                assert np.array_equal(got_w[l, h], w[l, h, want])
+                assert np.array_equal(gk[h], kv[l][0][h, want]) and np.array_equal(gv[h], kv[l][1][h, want])
+                assert np.array_equal(st.account(l)[h], w[l, h, want])
+    ctx.close()
+
+
 def test_evict_without_an_account_keeps_the_first_and_the_last():
     rng = np.random.default_rng(1)
     ctx = xn.Context(1, 2, 1, 32, pool_pages=8)
@@ -955,4 +1015,54 @@ def test_captured_attention_replays_after_reads_and_evictions():
     torch.cuda.synchronize()
     assert torch.equal(y, x * 3)
     near(out.cpu().numpy(), plain(q.cpu().numpy(), k, v)[0])
+    ctx.close()
+
+
+def test_a_captured_decode_replays_beside_reads_that_grow_and_evictions():
+    """The library's own call that can be captured (the allocation-free decode), replayed between reads whose
+    workspaces and page tables grow, writes, and an eviction of the stream the cache rows came from."""
+    import torch
+
+    rng = np.random.default_rng(6)
+    Hq, Hkv, D, n = 8, 2, 64, 400
+    lib = xn.load()
+    ctx = xn.Context(1, Hq, Hkv, D, pool_pages=200)
+    st, k, v = filled(ctx, rng, n)
+    kc, vc = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda()
+    q = torch.from_numpy(rows(rng, Hq, D)).cuda()
+    out = torch.zeros(Hq, D, device="cuda")
+    side = torch.cuda.Stream()
+    call = lambda: lib.xn_decode_attention_static(q.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), Hq, Hkv, D, n, n,
+                                                  side.cuda_stream)
+    torch.cuda.synchronize()
+    assert call() == 0          # (the first call on a device comes before any capture)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        assert call() == 0
+
+    def check_replay():
+        x = rows(rng, Hq, D)
+        q.copy_(torch.from_numpy(x))
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        near(out.cpu().numpy(), plain(x[:, None], k, v)[0][:, 0])
+
+    check_replay()
+    for m, R in [(50, 1), (300, 9), (2000, 150), (5000, 3)]:   # page tables, scores, images, partial records grow
+        other, ok, ov = filled(ctx, rng, m)
+        x = rows(rng, Hq, R, D)
+        (o,), (w,) = ctx.cross_attention([other], 0, [x], causal=True, weights=True, account="set")
+        want, want_w = plain(x, ok, ov, causal=True)
+        near(o, want)
+        near(w, want_w, abs_tol=ABS * R)
+        check_replay()
+        assert np.array_equal(other.evict(m // 2, m // 4)[0], np.stack([kept_of(w[h], m // 2, m // 4) for h in range(Hkv)]))
+        check_replay()
+        other.destroy()
+    st.set_account(0, 0, np.ones((Hkv, n)))
+    st.evict(100, 20)
+    check_replay()
     ctx.close()
