@@ -965,6 +965,38 @@ def test_many_requests_of_all_sizes_in_one_call(account):
     ctx.close()
 
 
+def test_a_call_that_finds_no_memory_fails_alone():
+    """The account's pool does not fit: that call is refused, the stream stays as it is, and the calls behind
+    it, of the library and of others, do not inherit the error."""
+    import torch
+
+    rng = np.random.default_rng(3)
+    Hkv, D, pages = 8, 4, 1 << 18     # account: 8 * 64 * 4 bytes a page, 512 MB
+    ctx = xn.Context(1, Hkv, Hkv, D, pool_pages=pages)
+    st, k, v = filled(ctx, rng, 100, cap=200)
+    q = rows(rng, Hkv, 2, D)
+    (before,) = ctx.cross_attention([st], 0, [q])
+    x, kv = rows(rng, 1, Hkv, 1, D), rows(rng, 1, Hkv, 1, D)
+    ctx.attention(st, 0, 100, x, kv, kv)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    hog = torch.empty(free - (256 << 20), dtype=torch.uint8, device="cuda")
+    with pytest.raises(xn.XnError) as e:
+        ctx.cross_attention([st], 0, [q], account="add")
+    assert e.value.code == 6
+    ctx.attention(st, 0, 101, x, kv, kv)
+    assert np.array_equal(ctx.cross_attention([st], 0, [q], kv_lens=[100])[0], before)
+    with pytest.raises(xn.XnError):
+        st.account(0)
+    hog[:16].zero_()                  # (a launch of another library, which looks for errors behind it)
+    del hog
+    torch.cuda.empty_cache()
+    (out,) = ctx.cross_attention([st], 0, [q], kv_lens=[100], account="add")
+    near(out, plain(q, k, v)[0])
+    near(st.account(0, 0, 100), plain(q, k, v)[1])
+    ctx.close()
+
+
 def test_more_rows_with_weights_than_one_launch_takes(monkeypatch):
     """140 000 small causal reads (4.5 million units of work) in one call; and one of 70 000 rows."""
     import torch

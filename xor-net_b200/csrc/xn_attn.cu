@@ -309,8 +309,10 @@ int32_t fail(xn_ctx* ctx, int32_t code, const char* fmt, ...) {
 #define XN_CUDA(ctx, expr)                                                                    \
     do {                                                                                      \
         cudaError_t e__ = (expr);                                                             \
-        if (e__ != cudaSuccess)                                                               \
+        if (e__ != cudaSuccess) {                                                             \
+            cudaGetLastError(); /* reported here: the next call's launches must not see it */ \
             return fail(ctx, XN_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__));   \
+        }                                                                                     \
     } while (0)
 
 bool ctx_ok(const xn_ctx* c) { return c && c->magic == kCtxMagic; }
