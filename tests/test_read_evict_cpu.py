@@ -62,3 +62,36 @@ def test_arrival_counters_cover_every_launch(tmp_path, repo_root):
     for line in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.splitlines():
         chunks, blocks, words = map(int, line.split())
         assert words >= 2 + max(chunks, blocks)
+
+
+class FakeLib:
+    """Stands in for the library: records a request, writes what a call on a stream of `length` would."""
+
+    def __init__(self, length, layers, heads, dim):
+        self.length, self.layers, self.heads, self.dim = length, layers, heads, dim
+
+    def xn_kv_evict(self, ctx, n, reqs):
+        r = reqs[0]
+        m = min(r.keep, self.length)
+        heads = (self.layers if r.layer < 0 else 1) * self.heads
+        for ptr, kind, width in ((r.kept, C.c_int32, 1), (r.weights_out, C.c_float, 1), (r.k_out, C.c_float, self.dim)):
+            if ptr:
+                (kind * (heads * m * width)).from_address(ptr)[:] = [kind(i % 100).value for i in range(heads * m * width)]
+        return 0
+
+    def xn_stream_len(self, ctx, stream, layer):
+        return 3          # what it was before another thread appended
+
+
+@pytest.mark.parametrize("length,keep,layer", [(3, 2, -1), (3, 8, 0), (50, 40, -1), (0, 4, -1), (64, 1000, 1)])
+def test_eviction_buffers_hold_what_the_call_keeps(length, keep, layer):
+    """... also when the stream has grown since its length was last asked for."""
+    ctx = object.__new__(xn.Context)
+    ctx.lib, ctx.handle = FakeLib(length, 2, 3, 4), None
+    ctx.num_layers, ctx.num_kv_heads, ctx.num_heads, ctx.head_dim = 2, 3, 3, 4
+    st = xn.Stream(ctx, 0, 64)
+    layers, m = 2 if layer < 0 else 1, min(keep, length)
+    assert st.evict(keep, layer=layer).shape == (layers, 3, m)
+    kept, k, v, w = st.evict_copy(keep, layer=layer)
+    assert kept.shape == w.shape == (layers, 3, m) and k.shape == v.shape == (layers, 3, m, 4)
+    assert k.ravel().tolist() == [i % 100 for i in range(layers * 3 * m * 4)]

@@ -180,22 +180,30 @@ class Stream:
         last positions and those of the largest account, ``keep`` in all.  Returns the kept positions
         ``[layers, Hkv, kept]``; decoding goes on at ``length(layer)``."""
         c = self.ctx
-        layers = c.num_layers if layer < 0 else 1
-        kept = np.zeros((layers, c.num_kv_heads, max(0, min(keep, self.length(max(layer, 0))))), dtype=np.int32)
+        kept, layers = self._kept_buffer(keep, layer)
         c.submit_evict(c.make_evict_batch([(self, layer, keep, recent, kept.ctypes.data, None, None, None)]))
-        return kept
+        n = np.count_nonzero(kept >= 0)
+        return kept[:n].reshape(layers, c.num_kv_heads, n // (layers * c.num_kv_heads))
+
+    def _kept_buffer(self, keep: int, layer: int):
+        """A buffer for the kept positions, -1 where nothing gets written, and the number of layers.  The
+        library keeps min(keep, length at the time of the call); so there is room for `keep` of a full
+        stream, since the length may be another one by then."""
+        layers = self.ctx.num_layers if layer < 0 else 1
+        return np.full(layers * self.ctx.num_kv_heads * max(0, min(keep, self.max_seq_len)), -1, dtype=np.int32), layers
 
     def evict_copy(self, keep: int, recent: int = 0, layer: int = -1):
         """The kept rows without touching the stream: (kept ``[layers, Hkv, kept]``, k and v
         ``[layers, Hkv, kept, D]``, their accounts)."""
-        c = self.ctx
-        layers = c.num_layers if layer < 0 else 1
-        shape = (layers, c.num_kv_heads, max(0, min(keep, self.length(max(layer, 0)))))
-        kept, w = np.zeros(shape, dtype=np.int32), np.zeros(shape, dtype=np.float32)
-        k, v = np.zeros(shape + (c.head_dim,), dtype=np.float32), np.zeros(shape + (c.head_dim,), dtype=np.float32)
+        c, D = self.ctx, self.ctx.head_dim
+        kept, layers = self._kept_buffer(keep, layer)
+        w = np.empty(kept.size, dtype=np.float32)
+        k, v = np.empty((kept.size, D), dtype=np.float32), np.empty((kept.size, D), dtype=np.float32)
         c.submit_evict(c.make_evict_batch([(self, layer, keep, recent, kept.ctypes.data, _ptr(k), _ptr(v), _ptr(w))],
                                           EVICT_COPY))
-        return kept, k, v, w
+        n = np.count_nonzero(kept >= 0)
+        shape = (layers, c.num_kv_heads, n // (layers * c.num_kv_heads))
+        return kept[:n].reshape(shape), k[:n].reshape(shape + (D,)), v[:n].reshape(shape + (D,)), w[:n].reshape(shape)
 
     def evicted(self, layer: int) -> int:
         """Positions that evictions took from a layer since the stream was created or reset."""
