@@ -95,3 +95,16 @@ def test_eviction_buffers_hold_what_the_call_keeps(length, keep, layer):
     kept, k, v, w = st.evict_copy(keep, layer=layer)
     assert kept.shape == w.shape == (layers, 3, m) and k.shape == v.shape == (layers, 3, m, 4)
     assert k.ravel().tolist() == [i % 100 for i in range(layers * 3 * m * 4)]
+
+
+def test_lists_of_different_lengths_are_refused():
+    import numpy as np
+
+    ctx = object.__new__(xn.Context)
+    ctx.lib, ctx.handle = FakeLib(3, 1, 1, 4), None
+    ctx.num_layers = ctx.num_kv_heads = ctx.num_heads = 1
+    ctx.head_dim = 4
+    st, q = xn.Stream(ctx, 0, 64), np.zeros((1, 1, 4), np.float32)
+    for streams, layer, qs, lens in [([st], 0, [q, q], None), ([st, st], 0, [q], None), ([st], [0, 0], [q], None), ([st], 0, [q], [1, 2])]:
+        with pytest.raises(ValueError):
+            ctx.cross_attention(streams, layer, qs, kv_lens=lens)

@@ -436,6 +436,9 @@ class Context:
         call's weights) ``[Hkv, kv_len]``."""
         if account not in (None, "add", "set"):
             raise ValueError('account must be None, "add" or "set"')
+        lists = [qs] + [x for x in (kv_lens, layer) if isinstance(x, (list, tuple))]
+        if any(len(x) != len(streams) for x in lists):
+            raise ValueError("qs, kv_lens and a list of layers must have one entry per stream")
         qs = [_f32(q) for q in qs]
         width = self.num_heads * self.head_dim
         for q in qs:
