@@ -68,7 +68,8 @@ struct TcKeyTile {
 
 // What the softmax needs to know about a page's K [0] and V [1]: factors that undo the scaling (of a V
 // image that is all zeros: kZeroFactor), and the rows that hold an infinity or a NaN or are far larger or
-// smaller than the page's others (their images are zero; they are added on the side, in f32).
+// smaller than the page's others (their images are zero; they are added on the side, in f32).  any_bad: bit
+// 0 there are such rows, bit 1 there are large ones among them.
 struct __align__(16) PageMeta {
     float f[2];
     unsigned any_bad[2];
@@ -242,6 +243,33 @@ __device__ __forceinline__ bool query_vec(const TcReq& r, int D) {
     return (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
 }
 
+// q . k of one query row and one cached row in f32, for the positions whose K is not in the images.  (Not
+// inlined: in line it takes registers from the loops around it, 447 us becomes 453 for 1024 rows over 8192
+// positions, 32/8 heads.)
+__device__ __noinline__ float exact_dot(const CacheView& c, const int* pages, int layer, int head, int key, const float* q,
+                                        bool vec, int D) {
+    const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
+    float dot = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+        const float4 k = cache_row4(c, blk, key % kPage, d >> 2, false);
+        float4 x;
+        if (vec) {
+            x = *reinterpret_cast<const float4*>(q + d);
+        } else {
+            x = make_float4(q[d], 0.f, 0.f, 0.f);
+            if (d + 1 < D) x.y = q[d + 1];
+            if (d + 2 < D) x.z = q[d + 2];
+            if (d + 3 < D) x.w = q[d + 3];
+        }
+        dot = fmaf(x.x, k.x, dot);
+        dot = fmaf(x.y, k.y, dot);
+        dot = fmaf(x.z, k.z, dot);
+        dot = fmaf(x.w, k.w, dot);
+    }
+    return dot;
+}
+
 // One element of a cached row, whatever the format (rare paths only).
 __device__ __forceinline__ float cache_elem(const CacheView& c, const int* pages, int layer, int head, int key, int d, bool v) {
     const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
@@ -329,6 +357,7 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
             s_bad[warp] = (unsigned char)bad;
         }
         __syncthreads();
+        unsigned large = 0u;
         float page_max = fmaxf(max4(*reinterpret_cast<const float4*>(s_max)), max4(*reinterpret_cast<const float4*>(s_max + 4)));
 #pragma unroll
         for (int i = 0; i < 8; ++i) least = min(least, s_least[i]);
@@ -355,6 +384,7 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
             }
             __syncthreads();
             const float lo = s_median * 0x1p-8f, hi = s_median * 0x1p8f;
+            large = page_max > hi ? 2u : 0u;
             page_max = 0.f;
             for (int i = 0; i < kPage; ++i)
                 if (s_row[i] >= lo && s_row[i] <= hi) page_max = fmaxf(page_max, s_row[i]);
@@ -376,7 +406,7 @@ page_images_kernel(const TcReq* __restrict__ reqs, int n_reqs, long long n_pages
             PageMeta& pm = meta[id];
             // (a V page of zeros takes no part in the choice of its neighbour's scale; K's factor undoes scores)
             pm.f[part] = part && empty ? kZeroFactor : down;
-            pm.any_bad[part] = rows != 0 ? 1u : 0u;
+            pm.any_bad[part] = (rows != 0 ? 1u : 0u) | large;
             pm.bad[part] = rows;
         }
         unsigned char* hi = images + size_t(id) * page_image_bytes(D) + size_t(part) * 2 * nb * kSub;
@@ -689,9 +719,9 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
             // The products of both pages' V images go to one accumulator, so P of the page with the smaller
             // factor is scaled down by their ratio.  Up to 2^10 that leaves weights a resolution of 2^-29 of
             // the largest; a page further below keeps its P and is added on the side, row by row in f32.
-            // (Below at all, where rows are added on the side anyway: they may be large, and need the P.)
+            // (Below at all, where large rows are added on the side: they need the P.)
             const float fv = fmaxf(fv0, fv1), fv_low = fminf(fv0, fv1);
-            const float apart_below = (a0.w | a1.w) != 0u ? 1.f : kApart;
+            const float apart_below = ((a0.w | a1.w) & 2u) ? 1.f : kApart;
             const bool bad_k = a0.z | a1.z;
             const bool bad_v = (a0.w | a1.w) != 0u || (fv_low < fv * kApart && fv_low != kZeroFactor);
             if (!warp_spin_bounded(&s_full[sb], uint32_t((j >> 1) & 1), lane)) dead = true;
@@ -711,9 +741,8 @@ read_tc_kernel(const TcReq* __restrict__ reqs, const TcItem* __restrict__ items,
                         b &= b - 1;
                         float dot = 0.f;
                         if (pr < n_packed)
-                            for (int d = 0; d < D; ++d)
-                                dot = fmaf(r.q[size_t(it.head * group + pr % group) * r.q_hs + size_t(t) * r.q_ts + d],
-                                           cache_elem(c, pages, r.layer, it.head, key0 + cidx, d, false), dot);
+                            dot = exact_dot(c, pages, r.layer, it.head, key0 + cidx,
+                                            r.q + size_t(it.head * group + pr % group) * r.q_hs + size_t(t) * r.q_ts, query_vec(r, D), D);
                         __syncwarp();
                         tmem_st1(s_addr + cidx, __float_as_uint(dot * scale_log2 / cm));
                     }
@@ -1135,6 +1164,7 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
             const PageMeta& pm = meta[image0(kt) + (rr >= kPage && 2 * kt.tile + 1 < r.n_pages ? c.num_kv_heads : 0)];
             const float fk = pm.f[0];
             const bool bad = in && ((pm.bad[0] >> (rr & 63)) & 1);
+            const unsigned bad_lanes = __ballot_sync(0xffffffffu, bad);
             // packed rows from `first_row` on see the position
             const int first_row = r.causal ? max(0, (key - (r.kv_len - r.rows)) * group) : 0;
             float sum = 0.f;
@@ -1149,29 +1179,29 @@ account_tc_kernel(const TcReq* __restrict__ reqs, const TcKeyTile* __restrict__ 
                     uint32_t x[32];
                     tmem_ld32(tmem + lane_base + s * 128 + wg * 64 + hf * 32, x);
                     tmem_wait_ld();
-                    if (bad) {
-#pragma unroll 1
-                        for (int i = 0; i < 32; ++i) {
-                            const int p = row0 + hf * 32 + i;
-                            if (p < first_row || p >= r.rows * group) continue;
-                            float dot = 0.f;
-                            for (int d = 0; d < D; ++d)
-                                dot = fmaf(r.q[size_t(kt.head * group + p % group) * r.q_hs + size_t(p / group) * r.q_ts + d],
-                                           cache_elem(c, pages, r.layer, kt.head, key, d, false), dot);
-                            sum += pf::ex2(dot * scale_log2 - rm[hf * 32 + i].y);
-                        }
-                    } else {
-                        const int from = first_row - (row0 + hf * 32);   // columns before this one do not count
-                        float s0 = 0.f, s1 = 0.f;
+                    const int from = first_row - (row0 + hf * 32);   // columns before this one do not count
+                    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
-                            const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * fk, f.x, -f.y));
-                            const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * fk, f.z, -f.w));
-                            s0 += i >= from ? a : 0.f;
-                            s1 += i + 1 >= from ? b : 0.f;
-                        }
-                        sum += s0 + s1;
+                    for (int i = 0; i < 32; i += 2) {
+                        const float4 f = *reinterpret_cast<const float4*>(rm + hf * 32 + i);
+                        const float a = pf::ex2(fmaf(__uint_as_float(x[i]) * fk, f.x, -f.y));
+                        const float b = pf::ex2(fmaf(__uint_as_float(x[i + 1]) * fk, f.z, -f.w));
+                        s0 += i >= from ? a : 0.f;
+                        s1 += i + 1 >= from ? b : 0.f;
+                    }
+                    if (!bad) sum += s0 + s1;
+                    // positions whose K is not in the image: a lane per query row
+                    for (unsigned left = bad_lanes; left != 0u; left &= left - 1) {
+                        const int src = __ffs(int(left)) - 1, p = row0 + hf * 32 + lane;
+                        const int from_row = __shfl_sync(0xffffffffu, first_row, src);
+                        float w = 0.f;
+                        if (p >= from_row && p < r.rows * group)
+                            w = pf::ex2(exact_dot(c, pages, r.layer, kt.head, key - lane + src,
+                                                  r.q + size_t(kt.head * group + p % group) * r.q_hs + size_t(p / group) * r.q_ts,
+                                                  query_vec(r, D), D) * scale_log2 - rm[hf * 32 + lane].y);
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+                        if (lane == src) sum += w;
                     }
                 }
                 warp_arrive(&s_empty[s], lane);
