@@ -400,6 +400,28 @@ def test_rows_of_one_page_of_very_different_sizes(monkeypatch, path, what, e):
     check_spread(monkeypatch, path, what, e)
 
 
+@pytest.mark.parametrize("D", [64, 50])
+@pytest.mark.parametrize("what", ["page_behind", "row_behind", "row_unweighted", "rows_unweighted", "krow_behind"])
+def test_u8_rows_of_very_different_sizes(monkeypatch, what, D):
+    """Over the u8 format, whose rows have a scale each, against the values that it holds; head sizes with and
+    without padding bytes, queries that cannot be read four at a time."""
+    rng = np.random.default_rng(D)
+    ctx = context(monkeypatch, "tc", 1, 4, 2, D, pool_pages=8, shuffle_seed=3, kv_format=xn.KV_U8)
+    k, v, q = (np.ascontiguousarray(x[..., :D]) for x in spread_rows(rng, what, 30))
+    st = ctx.new_stream(256)
+    st.write(0, 0, k, v)
+    k, v = st.read_range(0, 0, 256)
+    (out,), (w,) = ctx.cross_attention([st], 0, [q], causal=True, weights=True)
+    want, want_w = plain(q, k, v, True)
+    seen_by = 200 - 66 if what == "krow_behind" else 190
+    for h in range(4):
+        for t in range(seen_by):
+            near(out[h, t], want[h, t], f"{what} row {h} {t}", abs_tol=np.inf)
+    if seen_by == 190:
+        near(w, want_w, f"{what} weights", abs_tol=ABS * 190)
+    ctx.close()
+
+
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("e", [10, 20, 30])
 def test_a_large_row_of_little_weight(monkeypatch, path, e):

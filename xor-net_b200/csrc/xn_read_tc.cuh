@@ -243,31 +243,42 @@ __device__ __forceinline__ bool query_vec(const TcReq& r, int D) {
     return (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(r.q) | uintptr_t(r.q_hs * 4) | uintptr_t(r.q_ts * 4)) & 15) == 0;
 }
 
-// q . k of one query row and one cached row in f32, for the positions whose K is not in the images.  (Not
-// inlined: in line it takes registers from the loops around it, 447 us becomes 453 for 1024 rows over 8192
-// positions, 32/8 heads.)
-__device__ __noinline__ float exact_dot(const CacheView& c, const int* pages, int layer, int head, int key, const float* q,
-                                        bool vec, int D) {
-    const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
+// q . k of one query row and one cached row in f32, for the positions whose K is not in the images: k is
+// the row's floats, or with u8 its bytes, of scale s.  (Not inlined: in line it takes registers from the
+// loops around it, 447 us becomes 453 for 1024 rows over 8192 positions, 32/8 heads.)
+__device__ __noinline__ float dot_row(const void* __restrict__ k, float s, bool u8, const float* __restrict__ q, bool vec, int D) {
     float dot = 0.f;
 #pragma unroll 4
     for (int d = 0; d < D; d += 4) {
-        const float4 k = cache_row4(c, blk, key % kPage, d >> 2, false);
-        float4 x;
-        if (vec) {
-            x = *reinterpret_cast<const float4*>(q + d);
+        float4 x, y;
+        if (u8) {   // (bytes and floats behind head_dim are not looked at: 0 * s is NaN for an infinite scale)
+            const uchar4 b = *reinterpret_cast<const uchar4*>(static_cast<const uint8_t*>(k) + d);
+            x = make_float4((float(b.x) - 128.0f) * s, (float(b.y) - 128.0f) * s, (float(b.z) - 128.0f) * s, (float(b.w) - 128.0f) * s);
         } else {
-            x = make_float4(q[d], 0.f, 0.f, 0.f);
-            if (d + 1 < D) x.y = q[d + 1];
-            if (d + 2 < D) x.z = q[d + 2];
-            if (d + 3 < D) x.w = q[d + 3];
+            x = *reinterpret_cast<const float4*>(static_cast<const float*>(k) + d);
         }
-        dot = fmaf(x.x, k.x, dot);
-        dot = fmaf(x.y, k.y, dot);
-        dot = fmaf(x.z, k.z, dot);
-        dot = fmaf(x.w, k.w, dot);
+        if (vec) {
+            y = *reinterpret_cast<const float4*>(q + d);
+        } else {
+            y = make_float4(q[d], 0.f, 0.f, 0.f);
+            if (d + 1 < D) y.y = q[d + 1]; else x.y = 0.f;
+            if (d + 2 < D) y.z = q[d + 2]; else x.z = 0.f;
+            if (d + 3 < D) y.w = q[d + 3]; else x.w = 0.f;
+        }
+        dot = fmaf(y.x, x.x, dot);
+        dot = fmaf(y.y, x.y, dot);
+        dot = fmaf(y.z, x.z, dot);
+        dot = fmaf(y.w, x.w, dot);
     }
     return dot;
+}
+__device__ __forceinline__ float exact_dot(const CacheView& c, const int* pages, int layer, int head, int key, const float* q,
+                                           bool vec, int D) {
+    const size_t blk = (size_t(layer) * size_t(c.pool_pages) + size_t(pages[key / kPage])) * c.num_kv_heads + head;
+    const int tk = key % kPage;
+    if (!c.u8) return dot_row(c.k + (blk * kPage + tk) * size_t(c.nv) * 4, 0.f, false, q, vec, D);
+    const uint8_t* b = c.u8 + blk * (size_t(kPage) * (2 * size_t(c.dq) + 8));
+    return dot_row(b + size_t(tk) * c.dq, reinterpret_cast<const float*>(b + 2 * size_t(kPage) * c.dq)[tk], true, q, vec, D);
 }
 
 // One element of a cached row, whatever the format (rare paths only).
