@@ -329,6 +329,17 @@ XN_API int64_t xn_stream_pages(xn_ctx* ctx, xn_stream* stream, int32_t* out, int
  * document), and a decoder's own cache that is to keep the positions its queries look at.
  * None of them may be made while the context's CUDA stream is being captured (XN_ERR_ARG).
  *
+ * With device pointers the calls return after enqueueing, once what they need is there.  A call that finds
+ * a workspace, a plan slot or a stream's page table on the device missing or too small waits for the
+ * context's stream and allocates: half a millisecond for the first read of a context, 0.1 ms and more for
+ * the first call with an account (its pool), about 10 us for the first read or eviction of a stream (its
+ * table).  It must not be made while any stream is captured in the global mode, which forbids
+ * allocations.  The same call on the same streams finds everything in place the next time.
+ *
+ * Arguments are checked before anything is enqueued.  A call that fails behind its checks (XN_ERR_CUDA,
+ * XN_ERR_DEVICE_WAIT, XN_ERR_NOMEM) may have served some of its requests: the outputs that it names and
+ * the accounts that it keeps are unknown then.
+ *
  * Writes n rows of K and V at positions t0.. of one layer, without any attention: k and v are
  * [num_kv_heads, n, head_dim], or [n, num_kv_heads * head_dim] with XN_REQ_SEQ_MAJOR.  flags:
  * XN_REQ_DEVICE_PTRS (enqueues; else host pointers, blocks until they are read), XN_REQ_SEQ_MAJOR,
@@ -353,7 +364,7 @@ typedef struct xn_read_req {
     int32_t rows;       /* query rows                                                                */
     int64_t kv_len;     /* positions 0 .. kv_len - 1 are read; -1: all that the layer holds          */
     const float* q;     /* [num_heads, rows, head_dim], rotated already where the model rotates      */
-    float* out;         /* same layout; kv_len = 0 gives zeros                                       */
+    float* out;         /* same layout, another place than q; kv_len = 0 gives zeros                 */
     float* weights;     /* NULL, or [num_kv_heads][weights_stride]: receives, for every KV head and  */
                         /* position j < kv_len, the account after this call (without an account      */
                         /* flag: this call's own weights)                                            */
@@ -365,8 +376,15 @@ typedef struct xn_read_req {
 /* Attention of n groups of query rows over what their streams hold, appending nothing: scale
  * 1/sqrt(head_dim), softmax, weighted V sum; query head h reads KV head h / (num_heads /
  * num_kv_heads).  With XN_REQ_DEVICE_PTRS on every request the call returns after enqueueing;
- * otherwise it blocks until the host outputs are written.  Results are f32-grade in every variant
- * (split f16 operands on the tensor cores for many rows, f32 arithmetic for few).
+ * otherwise it blocks until the host outputs are written.
+ *
+ * Precision.  Few rows are computed in f32.  From a few rows on (a rule on sizes) the tensor cores take
+ * split f16 operands with f32 sums: elements of q, k and v keep 22 significand bits, or 2^-23 of the
+ * largest element of their row where that is more; a weight keeps 22 bits, or 2^-39 of its query row's
+ * largest weight.  So a result is as good as f32 arithmetic's unless values of V that are 2^17 and more
+ * times the others' meet weights below 2^-17: such a term is off by up to 2^-39 of the value.  What a
+ * query row does not see does not affect it, nor do finite values that it gives no weight to, however
+ * large.
  *
  * The account of attention weight, per layer, KV head and position j, is the sum over the
  * accounted rows and the heads of the KV head's group of the weight they gave j.  It is kept in

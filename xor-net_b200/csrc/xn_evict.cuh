@@ -424,7 +424,9 @@ evict_copy_kernel(const __grid_constant__ EvictTable tab, EvictPools p) {
 // of the next step are issued before the stores of this one (they read positions behind them).
 // One block per (layer, KV head, K or V, slice of 128 bytes of a row); the account moves with the
 // slice of K that holds a row's first bytes.  `unit` is 16 bytes for f32 rows and, for u8 rows,
-// 4 bytes (their scales move with the first slice of K and of V).
+// 4 bytes (their scales move with the first slice of K and of V).  Bound by that chain: a step is a
+// kept position, its page, its row and a barrier, one step ahead.  131072 positions cut to 16384, 8 heads
+// of 128: 355 us with the selection (copied out 70); 8192 to 2048 50 us.
 constexpr int kMoveThreads = 512;
 constexpr int kMoveSlice = 128;    // bytes of a row per block
 __global__ void __launch_bounds__(kMoveThreads)

@@ -19,6 +19,9 @@
 //               element is converted once.  A tile's O starts from zero in the MMA accumulator and is
 //               added to the running one in f32, which undoes the sub-block's scale.
 //
+// Positions far below the largest of those that share their scale (2^-16: their bits would go) have their
+// scores, and their share of O, computed in f32.
+//
 // The order of the contraction index, and of the output columns among the MMA's, is free: both are
 // chosen so that every shared-memory access is a conflict-free 16-byte one of the 128-byte-swizzled
 // tile.  Work is cut as in the table form of the split-KV kernel: block b of G takes an equal share of
