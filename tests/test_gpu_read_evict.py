@@ -987,6 +987,22 @@ def test_many_requests_of_all_sizes_in_one_call(account):
     ctx.close()
 
 
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_the_account_of_thousands_of_like_weights(monkeypatch, path, D):
+    """Equal weights of 1/n: every addition to a long running sum rounds the same way.  In blocks of 256 (32
+    rows of 8 heads) the sums take at most 256 + 2000 / 32 roundings of 2^-24 one after the other, and the
+    weight itself is off by 2^-21 (a logarithm below 8 and an exponential)."""
+    n, R = 79, 2000
+    ctx = context(monkeypatch, path, 1, 16, 2, D, pool_pages=2)
+    st = ctx.new_stream(n)
+    st.write(0, 0, np.zeros((2, n, D), np.float32), np.ones((2, n, D), np.float32))
+    q = rows(np.random.default_rng(0), 16, R, D)
+    _, (w,) = ctx.cross_attention([st], 0, [q], weights=True)
+    assert np.abs(w / (R * 8 / n) - 1).max() <= (256 + 2000 / 32) * 2.0 ** -24 + 2.0 ** -21
+    ctx.close()
+
+
 def test_a_call_that_finds_no_memory_fails_alone():
     """The account's pool does not fit: that call is refused, the stream stays as it is, and the calls behind
     it, of the library and of others, do not inherit the error."""

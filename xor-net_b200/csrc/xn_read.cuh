@@ -53,23 +53,29 @@ struct FewAccount {
     int row_step;          // 1 causal, 0 otherwise
 };
 
+// (32 rows at a time: thousands of like weights added to one running sum round the same way every time --
+// 16 000 of 1/79 were off by 1.6e-4, in blocks 3.5e-6)
 __device__ __forceinline__ float account_sum(const FewAccount& r, int h, int group, int key) {
     float sum = 0.f;
-    for (int t = 0; t < r.rows; ++t) {
-        if (key >= r.row_limit0 + t * r.row_step) continue;
+    for (int t0 = 0; t0 < r.rows; t0 += 32) {
+        float block = 0.f;
+        for (int t = t0; t < min(r.rows, t0 + 32); ++t) {
+            if (key >= r.row_limit0 + t * r.row_step) continue;
 #pragma unroll 4
-        for (int g = 0; g < group; ++g) {
-            const size_t head = size_t(h) * group + g;
-            const float s = r.scores[head * r.sc_hs + size_t(t) * r.sc_ts + key];
-            sum += expf(s - r.lse[head * r.lse_hs + t]);
+            for (int g = 0; g < group; ++g) {
+                const size_t head = size_t(h) * group + g;
+                const float s = r.scores[head * r.sc_hs + size_t(t) * r.sc_ts + key];
+                block += expf(s - r.lse[head * r.lse_hs + t]);
+            }
         }
+        sum += block;
     }
     return sum;
 }
 
 // One thread per cached position, blockIdx.y = KV head, blockIdx.z = request: 4 (G rows + 1..2)
 // bytes per position, read coalesced along the positions; a few per cent of what the attention
-// kernel before it reads.  The sum's order is fixed (rows, then heads): the same bits every time.
+// kernel before it reads.  The sum's order is fixed (blocks of rows, rows, heads): the same bits every time.
 __global__ void __launch_bounds__(256)
 account_few_kernel(const FewAccount* __restrict__ reqs, const int* __restrict__ page_ids,
                    float* __restrict__ pool, long long pool_pages, int num_kv_heads, int group) {

@@ -345,7 +345,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
     t.n_tiles = 0;
     int32_t rc;
     size_t floats = 0;
-    int max_kv = 0;
+    int max_kv = 0, max_rows = 0;
     for (int i = 0; i < n; ++i) {
         const ReadSub& s = subs[i];
         ReadEntry& e = t.e[i];
@@ -360,6 +360,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
         e.tile0 = t.n_tiles;
         t.n_tiles += (long long)e.n_tiles * Hkv * (mt ? e.n_rt : c->subs * s.rows);
         max_kv = std::max(max_kv, s.kv);
+        max_rows = std::max(max_rows, s.rows);
         if (!want) continue;
         e.user = s.acct.user; e.user_hs = s.acct.user_hs;
         e.old_from = s.acct.old_from; e.old_len = s.acct.old_len; e.store = s.acct.store;
@@ -374,7 +375,7 @@ int32_t launch_read_table(xn_ctx* c, const ReadSub* subs, int n, bool want, int 
     // 10.8 without; at 2000, 15.5 beside 17.5 and 15.1 beside 14.1 -- the split-KV kernel adds a launch for
     // the account, and reads faster once every block has a few tiles)
     const int small_max = want ? rs::kMaxTokens : rs::kMaxTokens / 2;
-    if (mt == 0 && c->head_dim <= 128 && n * Hkv <= c->sm_count) {
+    if (mt == 0 && c->head_dim <= 128 && max_rows <= rs::kMaxRows && n * Hkv <= c->sm_count) {
         int cluster = 1;
         while (cluster < ev::kMaxCluster && n * Hkv * cluster * 2 <= c->sm_count && max_kv > cluster * 32) cluster *= 2;
         if ((max_kv + cluster - 1) / cluster <= small_max) {

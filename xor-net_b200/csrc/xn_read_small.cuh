@@ -22,6 +22,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHeads = 4;             // heads per pass over the rows
 constexpr int kMaxTokens = 256;       // positions of one block
+constexpr int kMaxRows = 32;          // one after the other; their weights are one running sum
 constexpr int kKeys = 4;              // pairs of keys that a warp has in flight
 constexpr int kAhead = 8;             // rows of V that a warp has in flight
 
