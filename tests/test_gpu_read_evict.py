@@ -988,6 +988,31 @@ def test_many_requests_of_all_sizes_in_one_call(account):
 
 
 @pytest.mark.parametrize("path", ["few", "mid", "tc"])
+def test_pages_behind_the_32_bit_offsets_of_the_pools(monkeypatch, path):
+    """The last layer of pools of 4.7 thousand million floats each, pages in shuffled order."""
+    rng = np.random.default_rng(4)
+    Hq, Hkv, D, L, n = 16, 8, 128, 8, 700
+    ctx = context(monkeypatch, path, L, Hq, Hkv, D, pool_pages=9000, shuffle_seed=11)
+    assert 9000 * L * Hkv * 64 * D > 2 ** 32
+    st, k, v = filled(ctx, rng, n, layer=L - 1)
+    for R in (1, 9, 70):
+        q = rows(rng, Hq, R, D)
+        (out,), (w,) = ctx.cross_attention([st], L - 1, [q], causal=True, weights=True, account="set")
+        want, want_w = plain(q, k, v, causal=True)
+        near(out, want, f"R={R}")
+        near(w, want_w, f"weights R={R}", abs_tol=ABS * R)
+    acct = st.account(L - 1)
+    assert np.array_equal(acct, w)
+    kept = st.evict(200, 50, layer=L - 1)[0]
+    gk, gv = st.read_range(L - 1, 0, 200)
+    for h in range(Hkv):
+        want = kept_of(acct[h], 200, 50)
+        assert np.array_equal(kept[h], want) and np.array_equal(gk[h], k[h, want]) and np.array_equal(gv[h], v[h, want])
+        assert np.array_equal(st.account(L - 1)[h], acct[h, want])
+    ctx.close()
+
+
+@pytest.mark.parametrize("path", ["few", "mid", "tc"])
 @pytest.mark.parametrize("D", [64, 256])
 def test_the_account_of_thousands_of_like_weights(monkeypatch, path, D):
     """Equal weights of 1/n: every addition to a long running sum rounds the same way.  In blocks of 256 (32
